@@ -42,7 +42,10 @@ EXPORTS = (
     "bt_learner_use_p2p", "bt_learner_exchange_probe", "bt_linear_scan",
     "bt_linear_scan_backward", "bt_threefry2x32_host", "bt_threefry2x32", "bt_random_split",
     "bt_random_fill", "bt_random_permutation_workspace", "bt_random_permutation",
-    "bt_selftest_gru_barrier",
+    "bt_selftest_gru_barrier", "bt_linear_attention_workspace", "bt_linear_attention",
+    "bt_linear_attention_backward", "bt_linear_attention_step", "bt_qk_norm_rotary",
+    "bt_qk_norm_rotary_workspace", "bt_qk_norm_rotary_backward", "bt_glu_workspace", "bt_glu",
+    "bt_glu_backward",
 )
 
 
@@ -90,6 +93,33 @@ class Batch(C.Structure):
         ("log_prob", C.c_void_p), ("value", C.c_void_p), ("first_done", C.c_void_p),
         ("carry", C.c_void_p), ("last_carry", C.c_void_p),
     ]
+
+
+class Heads(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("batch_stride", C.c_int64), ("step_stride", C.c_int64),
+                ("head_stride", C.c_int64)]
+
+
+class LinearAttentionShape(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("steps", C.c_int32), ("heads", C.c_int32), ("key_dim", C.c_int32),
+        ("value_dim", C.c_int32), ("dtype", C.c_int32), ("scale", C.c_float),
+        ("log_decay", C.c_void_p), ("reset", C.c_void_p), ("reset_batch_stride", C.c_int64),
+        ("reset_step_stride", C.c_int64),
+    ]
+
+
+class QkNormRotaryShape(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "steps", "q_heads", "k_heads", "dim", "half",
+                                         "dtype", "weight_dtype", "interleaved")] + [
+        ("eps", C.c_float), ("positions", C.c_void_p), ("positions_batch_stride", C.c_int64),
+        ("positions_step_stride", C.c_int64), ("frequencies", C.c_void_p),
+    ]
+
+
+class GluShape(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("rows", "in_features", "out_features", "dtype",
+                                         "activation")]
 
 
 class BoontaError(RuntimeError):
@@ -160,6 +190,27 @@ def lib() -> C.CDLL:
         "bt_gemm_bf16x3": (C.c_int, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp]),
         "bt_clip_adam": (C.c_int, [vp, vp, vp, vp, i64, i32, C.POINTER(OptimizerC), vp]),
         "bt_clip_adam_noalloc": (C.c_int, [vp, vp, vp, vp, i64, i32, C.POINTER(OptimizerC), vp]),
+    }
+    heads, shape = C.POINTER(Heads), C.POINTER(LinearAttentionShape)
+    sig |= {
+        "bt_linear_attention_workspace": (i64, [shape, i32]),
+        "bt_linear_attention": (C.c_int, [shape, heads, heads, heads, vp, heads, vp, vp, i64, vp]),
+        "bt_linear_attention_backward": (C.c_int, [shape, heads, heads, heads, vp, heads, vp, heads,
+                                                   heads, heads, vp, vp, i64, vp]),
+        "bt_linear_attention_step": (C.c_int, [shape, heads, heads, heads, vp, vp, vp, vp]),
+    }
+    shape = C.POINTER(QkNormRotaryShape)
+    sig |= {
+        "bt_qk_norm_rotary": (C.c_int, [shape, heads, heads, vp, vp, heads, heads, vp]),
+        "bt_qk_norm_rotary_workspace": (i64, [shape]),
+        "bt_qk_norm_rotary_backward": (C.c_int, [shape, heads, heads, vp, vp, heads, heads, heads,
+                                                 heads, vp, vp, vp, i64, vp]),
+    }
+    shape = C.POINTER(GluShape)
+    sig |= {
+        "bt_glu_workspace": (i64, [shape, i32]),
+        "bt_glu": (C.c_int, [shape, vp, vp, vp, vp, vp, i64, vp]),
+        "bt_glu_backward": (C.c_int, [shape, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

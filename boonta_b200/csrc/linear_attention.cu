@@ -1,0 +1,518 @@
+// Linear attention with a decay per head on CUDA cores, its splits along the steps, the
+// single-step form, and the C entry points (the operation: linear_attention.cuh).
+//
+// Chunked form, 32 positions at a time, everything in fp32:
+//   P = (a b^T) * e^{(i - j) g} on and below the diagonal, 0 across a cut
+//   out = out_scale (in_scale P c + e^{(i + e0) g} a S)      rows before the chunk's first cut
+//   S = e^{(n - 1 + e0) g} S + in_scale sum_j e^{(n - 1 - j) g} b_j c_j^T
+// A block owns one (batch row, head) and 64 columns of c; the state stays in shared memory for
+// the block's whole walk. Sequences too few to fill the GPU are split along the steps: a first
+// launch sums each split from an empty state, a second joins the sums into the states that enter
+// the splits (S_{s+1} = e^{len g} S_s + local_s), a third runs the splits from those.
+#include <type_traits>
+
+#include "linear_attention.cuh"
+
+namespace bt {
+namespace la {
+namespace {
+
+constexpr int kC = 32;       // positions of a chunk
+constexpr int kDS = 64;      // columns of c (and of the state) of a block
+constexpr int kThreads = 256;
+
+struct Ops {
+  Op op[3];
+  int n;
+};
+
+template <int DA>
+struct Smem {
+  float a[kC][DA + 4], b[kC][DA + 4], c[kC][kDS + 4], s[DA][kDS + 4], p[kC][kC + 1];
+  float pw[kC + 2], pl[kC + 2];  // e^{i g} and what its rounding left
+  int seg[kC];
+};
+
+template <class T>
+__device__ __forceinline__ void load_rows(const Op& o, const Rows& r, int batch, int head, int i0,
+                                          int n, int d0, int d, int width, float* dst, int ld) {
+  const T* p = static_cast<const T*>(r.p) + batch * r.batch + head * r.head;
+  for (int e = threadIdx.x; e < kC * width; e += kThreads) {
+    const int i = e / width, x = e % width;
+    float v = 0.f;
+    if (i < n && d0 + x < d) v = to_float(p[(int64_t)op_time(o, i0 + i) * r.step + d0 + x]);
+    dst[i * ld + x] = v;
+  }
+}
+
+// kOut: outputs and (split s) from the state that enters the split; else the split's own sum.
+template <class T, int DA, bool kOut>
+__global__ void __launch_bounds__(kThreads) chunk_kernel(const __grid_constant__ Ops ops) {
+  const Op& o = ops.op[blockIdx.z];
+  extern __shared__ __align__(16) uint8_t raw[];
+  Smem<DA>& sm = *reinterpret_cast<Smem<DA>*>(raw);
+  const int slices = ceil_div(o.Dc, kDS);
+  if ((int)blockIdx.x >= o.batch * o.heads * slices) return;
+  const int bh = blockIdx.x / slices, d0 = blockIdx.x % slices * kDS;
+  const int batch = bh / o.heads, head = bh % o.heads;
+  const int split = blockIdx.y;
+  const int begin = split * o.split_len, end = min(o.steps, begin + o.split_len);
+  const int tid = threadIdx.x;
+  const float g = fmaxf(o.log_decay[head], kMinLogDecay);
+  const int DcV = min(kDS, o.Dc - d0);
+  const size_t elems = (size_t)o.Da * o.Dc;
+
+  if (tid < kC + 2) {
+    const double e = exp((double)tid * (double)g);
+    sm.pw[tid] = (float)e;
+    sm.pl[tid] = (float)(e - (double)(float)e);
+  }
+  const float* from = nullptr;
+  int sx = o.sx, sy = o.sy;
+  if (kOut) {
+    if (split > 0) {
+      from = o.local + ((size_t)(split - 1) * o.batch * o.heads + bh) * elems;
+      sx = o.Dc;
+      sy = 1;
+    } else if (o.init) {
+      from = o.init + bh * elems;
+    }
+  }
+  for (int e = tid; e < DA * kDS; e += kThreads) {
+    const int x = e / kDS, y = e % kDS;
+    sm.s[x][y] = from && x < o.Da && y < DcV ? from[(size_t)x * sx + (size_t)(d0 + y) * sy] : 0.f;
+  }
+  bool any_cut = false;
+  // decays that the entering state meets before position `begin`
+  int e0 = (o.reverse && split == 0) ? 0 : 1;
+
+  for (int i0 = begin; i0 < end; i0 += kC) {
+    const int n = min(kC, end - i0);
+    __syncthreads();
+    if (kOut) load_rows<T>(o, o.a, batch, head, i0, n, 0, o.Da, DA, &sm.a[0][0], DA + 4);
+    load_rows<T>(o, o.b, batch, head, i0, n, 0, o.Da, DA, &sm.b[0][0], DA + 4);
+    load_rows<T>(o, o.c, batch, head, i0, n, d0, o.Dc, kDS, &sm.c[0][0], kDS + 4);
+    if (tid < kC) {
+      const unsigned m = __ballot_sync(~0u, tid < n && op_cut(o, batch, i0 + tid));
+      sm.seg[tid] = __popc(m & (~0u >> (31 - tid)));
+    }
+    __syncthreads();
+    const int seg_end = sm.seg[kC - 1];
+    any_cut |= seg_end > 0;
+
+    if (kOut) {
+      {  // P: row i = tid / 8, columns tid % 8 + 8 m
+        const int i = tid >> 3, j0 = tid & 7;
+        float acc[4] = {};
+        for (int k = 0; k < DA; k += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(&sm.a[i][k]);
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const float4 y = *reinterpret_cast<const float4*>(&sm.b[j0 + 8 * m][k]);
+            acc[m] += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const int j = j0 + 8 * m;
+          const bool on = j <= i && sm.seg[i] == sm.seg[j];
+          sm.p[i][j] = on ? acc[m] * sm.pw[i - j] * o.in_scale : 0.f;
+        }
+      }
+      __syncthreads();
+      // out: rows 2 r, 2 r + 1, columns 4 q .. 4 q + 3
+      const int r = tid >> 4, y = (tid & 15) * 4;
+      float acc[2][4] = {}, st[2][4] = {};
+      for (int j = 0; j <= 2 * r + 1; ++j) {
+        const float4 c = *reinterpret_cast<const float4*>(&sm.c[j][y]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (j > 2 * r + u || sm.seg[2 * r + u] != sm.seg[j]) continue;
+          const float p = sm.p[2 * r + u][j];
+          acc[u][0] += p * c.x;
+          acc[u][1] += p * c.y;
+          acc[u][2] += p * c.z;
+          acc[u][3] += p * c.w;
+        }
+      }
+      for (int k = 0; k < DA; k += 4) {
+        float4 x[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) x[u] = *reinterpret_cast<const float4*>(&sm.a[2 * r + u][k]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float4 s = *reinterpret_cast<const float4*>(&sm.s[k + w][y]);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float xv = w == 0 ? x[u].x : w == 1 ? x[u].y : w == 2 ? x[u].z : x[u].w;
+            st[u][0] += xv * s.x;
+            st[u][1] += xv * s.y;
+            st[u][2] += xv * s.z;
+            st[u][3] += xv * s.w;
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int i = 2 * r + u;
+        if (i >= n) continue;
+        const float reach = sm.seg[i] == 0 ? sm.pw[i + e0] : 0.f;
+        T* out = static_cast<T*>(o.out) + batch * o.out_batch +
+                 (int64_t)op_time(o, i0 + i) * o.out_step + head * o.out_head + d0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          if (y + w >= DcV) continue;
+          // a cut drops the state whatever it holds, not 0 times it
+          const float v = reach != 0.f ? acc[u][w] + reach * st[u][w] : acc[u][w];
+          out[y + w] = from_float<T>(v * o.out_scale);
+        }
+      }
+      __syncthreads();
+    }
+    {  // state: rows DA / 16 * r .., columns 4 q ..
+      constexpr int kR = DA / 16;
+      const int x0 = (tid >> 4) * kR, y = (tid & 15) * 4;
+      // the same factor meets the state once a chunk, so its rounding would add up over a long
+      // memory: two parts leave only the roundings of the sums, which do not lean one way
+      const float keep = sm.pw[n - 1 + e0], keep_lo = sm.pl[n - 1 + e0];
+      float acc[kR][4];
+#pragma unroll
+      for (int u = 0; u < kR; ++u)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          acc[u][w] = seg_end == 0 ? fmaf(keep, sm.s[x0 + u][y + w], keep_lo * sm.s[x0 + u][y + w]) : 0.f;
+      for (int j = 0; j < n; ++j) {
+        if (sm.seg[j] != seg_end) continue;
+        const float wj = sm.pw[n - 1 - j] * o.in_scale;
+        const float4 c = *reinterpret_cast<const float4*>(&sm.c[j][y]);
+#pragma unroll
+        for (int u = 0; u < kR; ++u) {
+          const float b = sm.b[j][x0 + u] * wj;
+          acc[u][0] += b * c.x;
+          acc[u][1] += b * c.y;
+          acc[u][2] += b * c.z;
+          acc[u][3] += b * c.w;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kR; ++u)
+        *reinterpret_cast<float4*>(&sm.s[x0 + u][y]) =
+            make_float4(acc[u][0], acc[u][1], acc[u][2], acc[u][3]);
+    }
+    e0 = 1;
+  }
+  __syncthreads();
+  float* to = nullptr;
+  float last = 1.f;
+  if (kOut) {
+    if (o.fin && split == o.nsplit - 1) {
+      to = o.fin + bh * elems;
+      sx = o.sx;
+      sy = o.sy;
+      // backwards: the way out of position steps - 1 passes reset[0] and one decay
+      if (o.reverse && o.steps > 0) {
+        last = sm.pw[1];
+        if (o.reset && o.reset[batch * o.reset_batch]) last = 0.f;
+      }
+    }
+  } else {
+    to = o.local + ((size_t)split * o.batch * o.heads + bh) * elems;
+    sx = o.Dc;
+    sy = 1;
+    if (tid == 0 && d0 == 0 && head == 0) o.cut[split * o.batch + batch] = any_cut;
+  }
+  if (to) {
+    for (int e = tid; e < DA * kDS; e += kThreads) {
+      const int x = e / kDS, y = e % kDS;
+      if (x < o.Da && y < DcV)
+        to[(size_t)x * sx + (size_t)(d0 + y) * sy] = last == 0.f ? 0.f : last * sm.s[x][y];
+    }
+  }
+}
+
+// local[s], the own sum of split s < nsplit - 1, becomes the state that enters split s + 1.
+__global__ void join_kernel(const __grid_constant__ Ops ops) {
+  const Op& o = ops.op[blockIdx.y];
+  const int64_t elems = (int64_t)o.Da * o.Dc, total = elems * o.batch * o.heads;
+  const int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (e >= total) return;
+  const int64_t bh = e / elems;
+  const int batch = (int)(bh / o.heads), x = (int)(e % elems / o.Dc), y = (int)(e % o.Dc);
+  const float g = fmaxf(o.log_decay[bh % o.heads], kMinLogDecay);
+  float s = o.init ? o.init[bh * elems + (int64_t)x * o.sx + (int64_t)y * o.sy] : 0.f;
+  const double full = exp((double)o.split_len * (double)g);
+  const double first = o.reverse ? exp((double)(o.split_len - 1) * (double)g) : full;
+  for (int k = 0; k + 1 < o.nsplit; ++k) {
+    const float own = o.local[(int64_t)k * total + e];
+    s = o.cut[k * o.batch + batch] ? own : (float)((k == 0 ? first : full) * (double)s + (double)own);
+    o.local[(int64_t)k * total + e] = s;
+  }
+}
+
+
+// One position of every (batch row, head): S' = [not reset] e^g S + k v^T, out = scale S'^T q.
+// A block takes one (batch row, head); thread (r, y) holds the columns V y .. V y + V - 1 of the
+// rows r, r + R, ...; the partial sums of out meet in shared memory in a fixed order. `next` may be
+// `state` itself: every element is read and written by one thread.
+template <class T, int V>
+__global__ void __launch_bounds__(kThreads)
+    step_kernel(const Rows q, const Rows k, const Rows v, const float* log_decay,
+                const uint8_t* reset, int64_t reset_batch, const float* state, float* next, T* out,
+                int heads, int Dk, int Dv, float scale) {
+  extern __shared__ float part[];  // [R][Dv padded to V], then q, k [Dk] each
+  const int bh = blockIdx.x, batch = bh / heads, head = bh % heads;
+  const int cols = ceil_div(Dv, V), R = blockDim.x / cols;
+  float* sq = part + R * cols * V;
+  float* sk = sq + Dk;
+  const T* qp = static_cast<const T*>(q.p) + batch * q.batch + head * q.head;
+  const T* kp = static_cast<const T*>(k.p) + batch * k.batch + head * k.head;
+  const T* vp = static_cast<const T*>(v.p) + batch * v.batch + head * v.head;
+  for (int i = threadIdx.x; i < Dk; i += blockDim.x) {
+    sq[i] = to_float(qp[i]);
+    sk[i] = to_float(kp[i]);
+  }
+  const bool cut = reset && reset[batch * reset_batch];
+  const float decay = expf(fmaxf(log_decay[head], kMinLogDecay));
+  const int r = threadIdx.x / cols, y = threadIdx.x % cols * V;
+  const bool on = r < R;
+  float val[V], acc[V];
+#pragma unroll
+  for (int w = 0; w < V; ++w) {
+    val[w] = on && y + w < Dv ? to_float(vp[y + w]) : 0.f;
+    acc[w] = 0.f;
+  }
+  __syncthreads();
+  const int64_t base = (int64_t)bh * Dk * Dv;
+  if (on) {
+#pragma unroll 4
+    for (int x = r; x < Dk; x += R) {
+      float s[V];
+      if (cut) {
+#pragma unroll
+        for (int w = 0; w < V; ++w) s[w] = 0.f;
+      } else if constexpr (V == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(state + base + (int64_t)x * Dv + y);
+        s[0] = f.x, s[1] = f.y, s[2] = f.z, s[3] = f.w;
+      } else {
+        s[0] = state[base + (int64_t)x * Dv + y];
+      }
+#pragma unroll
+      for (int w = 0; w < V; ++w) {
+        s[w] = decay * s[w] + sk[x] * val[w];
+        acc[w] += sq[x] * s[w];
+      }
+      if constexpr (V == 4)
+        *reinterpret_cast<float4*>(next + base + (int64_t)x * Dv + y) = make_float4(s[0], s[1], s[2], s[3]);
+      else
+        next[base + (int64_t)x * Dv + y] = s[0];
+    }
+#pragma unroll
+    for (int w = 0; w < V; ++w) part[r * cols * V + y + w] = acc[w];
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < Dv; c += blockDim.x) {
+    float s = 0.f;
+    for (int u = 0; u < R; ++u) s += part[u * cols * V + c];
+    out[(int64_t)bh * Dv + c] = from_float<T>(s * scale);
+  }
+}
+
+template <class T>
+int run_ops(Ops& ops, cudaStream_t stream) {
+  int da = 0, blocks = 0, elems = 0;
+  for (int i = 0; i < ops.n; ++i) {
+    const Op& o = ops.op[i];
+    da = max(da, o.Da);
+    blocks = max(blocks, o.batch * o.heads * ceil_div(o.Dc, kDS));
+    elems = max(elems, o.Da * o.Dc);
+  }
+  const Op& o = ops.op[0];
+  auto go = [&](auto size) -> int {
+    constexpr int DA = decltype(size)::value;
+    constexpr int kSmem = sizeof(Smem<DA>);
+    BT_CUDA(cudaFuncSetAttribute(chunk_kernel<T, DA, false>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    BT_CUDA(cudaFuncSetAttribute(chunk_kernel<T, DA, true>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    if (o.nsplit > 1) {
+      chunk_kernel<T, DA, false><<<dim3(blocks, o.nsplit - 1, ops.n), kThreads, kSmem, stream>>>(ops);
+      BT_LAUNCH_CHECK("linear attention split sums");
+      const int64_t total = (int64_t)o.batch * o.heads * elems;
+      join_kernel<<<dim3((unsigned)ceil_div64(total, 256), ops.n), 256, 0, stream>>>(ops);
+      BT_LAUNCH_CHECK("linear attention join");
+    }
+    chunk_kernel<T, DA, true><<<dim3(blocks, o.nsplit, ops.n), kThreads, kSmem, stream>>>(ops);
+    BT_LAUNCH_CHECK("linear attention");
+    return BT_OK;
+  };
+  if (da <= 64) return go(std::integral_constant<int, 64>{});
+  return go(std::integral_constant<int, 128>{});
+}
+
+// Splits of the steps: enough blocks to fill the GPU twice, at least 128 positions each.
+void choose_splits(int batch, int heads, int steps, int ops, int* nsplit, int* len) {
+  const int want = ceil_div(2 * kNumSMs, max(1, batch * heads * ops));
+  const int n = max(1, min(want, steps / 128));
+  *len = max(kC, ceil_div(ceil_div(steps, n), kC) * kC);
+  *nsplit = max(1, ceil_div(steps, *len));
+}
+
+int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
+
+int check_shape(const bt_linear_attention_shape* s, const char* who) {
+  BT_CHECK_ARG(s, "%s: null shape", who);
+  BT_CHECK_ARG(s->batch >= 0 && s->steps >= 0 && s->heads >= 0, "%s: negative size", who);
+  BT_CHECK_ARG(s->key_dim >= 1 && s->key_dim <= 128 && s->value_dim >= 1 && s->value_dim <= 128,
+               "%s: heads of %d and %d features (1 to 128 are supported)", who, s->key_dim,
+               s->value_dim);
+  BT_CHECK_ARG((int64_t)s->batch * s->heads <= (1 << 29), "%s: %d x %d sequences are too many", who,
+               s->batch, s->heads);
+  BT_CHECK_ARG(s->dtype == BT_DTYPE_F32 || s->dtype == BT_DTYPE_BF16, "%s: dtype %d", who, s->dtype);
+  BT_CHECK_ARG(s->log_decay || s->batch * s->heads == 0, "%s: null log_decay", who);
+  return BT_OK;
+}
+
+int64_t workspace_bytes(const bt_linear_attention_shape* s, int ops) {
+  int nsplit, len;
+  choose_splits(s->batch, s->heads, s->steps, ops, &nsplit, &len);
+  if (nsplit == 1) return 0;
+  const int64_t state = (int64_t)s->batch * s->heads * s->key_dim * s->value_dim * 4;
+  return ops * (align256((nsplit - 1) * state) + align256((int64_t)(nsplit - 1) * s->batch * 4));
+}
+
+Rows rows_of(const bt_heads& h) { return Rows{h.data, h.batch_stride, h.step_stride, h.head_stride}; }
+
+Op op_of(const bt_linear_attention_shape* s, const bt_heads& a, const bt_heads& b, const bt_heads& c,
+         const bt_heads& out, bool transposed, bool reverse) {
+  Op o{};
+  o.a = rows_of(a);
+  o.b = rows_of(b);
+  o.c = rows_of(c);
+  o.out = out.data;
+  o.out_batch = out.batch_stride;
+  o.out_step = out.step_stride;
+  o.out_head = out.head_stride;
+  o.sx = transposed ? 1 : s->value_dim;
+  o.sy = transposed ? s->value_dim : 1;
+  o.Da = transposed ? s->value_dim : s->key_dim;
+  o.Dc = transposed ? s->key_dim : s->value_dim;
+  o.log_decay = s->log_decay;
+  o.reset = s->reset;
+  o.reset_batch = s->reset_batch_stride;
+  o.reset_step = s->reset_step_stride;
+  o.batch = s->batch;
+  o.steps = s->steps;
+  o.heads = s->heads;
+  o.in_scale = reverse ? s->scale : 1.f;
+  o.out_scale = reverse ? 1.f : s->scale;
+  o.reverse = reverse;
+  return o;
+}
+
+int launch(const bt_linear_attention_shape* s, Ops& ops, void* workspace, int64_t bytes,
+           cudaStream_t stream, const char* who) {
+  int nsplit, len;
+  choose_splits(s->batch, s->heads, s->steps, ops.n, &nsplit, &len);
+  const int64_t need = workspace_bytes(s, ops.n);
+  BT_CHECK_ARG(need == 0 || (workspace && bytes >= need), "%s: workspace of %lld bytes, %lld needed",
+               who, (long long)bytes, (long long)need);
+  BT_CHECK_ARG(((uintptr_t)workspace & 15) == 0, "%s: workspace not 16-byte aligned", who);
+  char* w = static_cast<char*>(workspace);
+  for (int i = 0; i < ops.n; ++i) {
+    Op& o = ops.op[i];
+    o.nsplit = nsplit;
+    o.split_len = len;
+    if (nsplit > 1) {
+      const int64_t state = (int64_t)s->batch * s->heads * s->key_dim * s->value_dim * 4;
+      o.local = reinterpret_cast<float*>(w);
+      w += align256((nsplit - 1) * state);
+      o.cut = reinterpret_cast<int*>(w);
+      w += align256((int64_t)(nsplit - 1) * s->batch * 4);
+    }
+  }
+  if (s->batch == 0 || s->heads == 0) return BT_OK;
+  return s->dtype == BT_DTYPE_BF16 ? run_ops<__nv_bfloat16>(ops, stream) : run_ops<float>(ops, stream);
+}
+
+bool rows_ok(const bt_linear_attention_shape* s, const bt_heads* h) {
+  return h && (h->data || (int64_t)s->batch * s->steps * s->heads == 0);
+}
+
+}  // namespace
+}  // namespace la
+}  // namespace bt
+
+using namespace bt;
+
+extern "C" int64_t bt_linear_attention_workspace(const bt_linear_attention_shape* s, int32_t backward) {
+  if (la::check_shape(s, "bt_linear_attention_workspace") != BT_OK) return -1;
+  return la::workspace_bytes(s, backward ? 3 : 1);
+}
+
+extern "C" int bt_linear_attention(const bt_linear_attention_shape* s, const bt_heads* q,
+                                   const bt_heads* k, const bt_heads* v, const float* state,
+                                   const bt_heads* out, float* final_state, void* workspace,
+                                   int64_t workspace_bytes, void* stream) {
+  BT_TRY(la::check_shape(s, "bt_linear_attention"));
+  BT_CHECK_ARG(la::rows_ok(s, q) && la::rows_ok(s, k) && la::rows_ok(s, v) && la::rows_ok(s, out) &&
+                   (final_state || s->batch * s->heads == 0),
+               "bt_linear_attention: null pointer");
+  la::Ops ops{};
+  ops.n = 1;
+  ops.op[0] = la::op_of(s, *q, *k, *v, *out, false, false);
+  ops.op[0].init = state;
+  ops.op[0].fin = final_state;
+  return la::launch(s, ops, workspace, workspace_bytes, (cudaStream_t)stream, "bt_linear_attention");
+}
+
+extern "C" int bt_linear_attention_backward(const bt_linear_attention_shape* s, const bt_heads* q,
+                                            const bt_heads* k, const bt_heads* v,
+                                            const float* state, const bt_heads* dout,
+                                            const float* dfinal_state, const bt_heads* dq,
+                                            const bt_heads* dk, const bt_heads* dv, float* dstate,
+                                            void* workspace, int64_t workspace_bytes, void* stream) {
+  BT_TRY(la::check_shape(s, "bt_linear_attention_backward"));
+  BT_CHECK_ARG(la::rows_ok(s, q) && la::rows_ok(s, k) && la::rows_ok(s, v) && la::rows_ok(s, dout) &&
+                   la::rows_ok(s, dq) && la::rows_ok(s, dk) && la::rows_ok(s, dv) &&
+                   (dstate || s->batch * s->heads == 0),
+               "bt_linear_attention_backward: null pointer");
+  la::Ops ops{};
+  ops.n = 3;
+  ops.op[0] = la::op_of(s, *dout, *v, *k, *dq, true, false);
+  ops.op[0].init = state;
+  ops.op[1] = la::op_of(s, *k, *q, *dout, *dv, false, true);
+  ops.op[1].init = dfinal_state;
+  ops.op[1].fin = dstate;
+  ops.op[2] = la::op_of(s, *v, *dout, *q, *dk, true, true);
+  ops.op[2].init = dfinal_state;
+  return la::launch(s, ops, workspace, workspace_bytes, (cudaStream_t)stream,
+                    "bt_linear_attention_backward");
+}
+
+extern "C" int bt_linear_attention_step(const bt_linear_attention_shape* s, const bt_heads* q,
+                                        const bt_heads* k, const bt_heads* v, const float* state,
+                                        void* out, float* new_state, void* stream) {
+  BT_TRY(la::check_shape(s, "bt_linear_attention_step"));
+  BT_CHECK_ARG(s->steps == 1, "bt_linear_attention_step: %d steps", s->steps);
+  const int64_t n = (int64_t)s->batch * s->heads;
+  if (n == 0) return BT_OK;
+  BT_CHECK_ARG(la::rows_ok(s, q) && la::rows_ok(s, k) && la::rows_ok(s, v) && state && out && new_state,
+               "bt_linear_attention_step: null pointer");
+  const bool vec = s->value_dim % 4 == 0 && (((uintptr_t)state | (uintptr_t)new_state) & 15) == 0;
+  auto go = [&](auto tag, auto width) -> int {
+    using T = decltype(tag);
+    constexpr int V = decltype(width)::value;
+    const int cols = ceil_div(s->value_dim, V), threads = 128, R = threads / cols;
+    const size_t smem = (size_t)(R * cols * V + 2 * s->key_dim) * 4;
+    la::step_kernel<T, V><<<(unsigned)n, threads, smem, (cudaStream_t)stream>>>(
+        la::rows_of(*q), la::rows_of(*k), la::rows_of(*v), s->log_decay, s->reset,
+        s->reset_batch_stride, state, new_state, static_cast<T*>(out), s->heads, s->key_dim,
+        s->value_dim, s->scale);
+    BT_LAUNCH_CHECK("linear attention step");
+    return BT_OK;
+  };
+  if (s->dtype == BT_DTYPE_BF16)
+    return vec ? go(__nv_bfloat16{}, std::integral_constant<int, 4>{})
+               : go(__nv_bfloat16{}, std::integral_constant<int, 1>{});
+  return vec ? go(float{}, std::integral_constant<int, 4>{}) : go(float{}, std::integral_constant<int, 1>{});
+}

@@ -1,0 +1,84 @@
+"""The gated feed-forward layer h = act(x w_gate) * (x w_up), both projections, the activation and
+the product in one kernel; differentiable through the native backward, which forms the projections
+again tile by tile instead of keeping them.
+
+The weights are kernels as the framework's Dense layers have them ([in features, out features]), the
+activations its own ("silu", "relu", "tanh", "none").
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+from .linear_attention import _DTYPES, _on, _ptr
+
+
+def _check(x, w_gate, w_up, activation):
+    if activation not in _lib.ACT:
+        raise ValueError(f"gated_linear_unit: unknown activation {activation!r}, have "
+                         f"{sorted(_lib.ACT)}")
+    if x.ndim < 1 or w_gate.ndim != 2 or w_up.shape != w_gate.shape or x.shape[-1] != w_gate.shape[0]:
+        raise ValueError(f"gated_linear_unit: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, "
+                         f"w_up {tuple(w_up.shape)}: [..., in], [in, out], [in, out] expected")
+    if x.dtype not in _DTYPES or w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
+        raise TypeError(f"gated_linear_unit: x {x.dtype}, w_gate {w_gate.dtype}, w_up {w_up.dtype}: "
+                        "float32 or bfloat16 expected, the same for all three")
+    if min(w_gate.shape) < 1:
+        raise ValueError(f"gated_linear_unit: weights {tuple(w_gate.shape)} without features")
+    for t in (x, w_gate, w_up):
+        if not t.is_cuda or t.device != x.device:
+            raise ValueError("gated_linear_unit: CUDA tensors on one device expected")
+
+
+def _shape(x, w, activation):
+    return _lib.GluShape(x.shape[0], w.shape[0], w.shape[1], _DTYPES[x.dtype], _lib.ACT[activation])
+
+
+def _workspace(shape, backward, device):
+    n = _lib.lib().bt_glu_workspace(C.byref(shape), backward)
+    return (torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None), n
+
+
+class _Glu(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, activation):
+        x, w_gate, w_up = x.contiguous(), w_gate.contiguous(), w_up.contiguous()
+        out = torch.empty(x.shape[0], w_gate.shape[1], dtype=x.dtype, device=x.device)
+        with _on(x.device):
+            shape = _shape(x, w_gate, activation)
+            ws, n = _workspace(shape, 0, x.device)
+            _lib.check(_lib.lib().bt_glu(C.byref(shape), x.data_ptr(), w_gate.data_ptr(),
+                                         w_up.data_ptr(), out.data_ptr(), _ptr(ws), n,
+                                         torch.cuda.current_stream().cuda_stream))
+        ctx.save_for_backward(x, w_gate, w_up)
+        ctx.activation = activation
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        x, w_gate, w_up = ctx.saved_tensors
+        dout = dout.to(x.dtype).contiguous()
+        dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+        weights = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dwg = torch.empty_like(w_gate) if weights else None
+        dwu = torch.empty_like(w_up) if weights else None
+        with _on(x.device):
+            shape = _shape(x, w_gate, ctx.activation)
+            ws, n = _workspace(shape, 1, x.device)
+            _lib.check(_lib.lib().bt_glu_backward(
+                C.byref(shape), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), dout.data_ptr(),
+                _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(ws), n,
+                torch.cuda.current_stream().cuda_stream))
+        return dx, dwg, dwu, None
+
+
+def gated_linear_unit(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+                      activation: str = "silu") -> torch.Tensor:
+    """act(x @ w_gate) * (x @ w_up): x [..., in], weights [in, out], all float32 or all bfloat16;
+    sums in float32, the result [..., out] in x's dtype."""
+    _check(x, w_gate, w_up, activation)
+    rows = x.reshape(-1, x.shape[-1])
+    return _Glu.apply(rows, w_gate, w_up, activation).reshape(*x.shape[:-1], w_gate.shape[1])

@@ -176,6 +176,88 @@ BT_API int bt_linear_scan_backward(const void* a, const void* h, const void* ini
                             int32_t batch, int32_t steps, int32_t features, int32_t dtype,
                             int32_t init_dtype, void* stream);
 
+/* ---- linear attention with a decay per head -------------------------------------------------
+ *   S_t = [not reset_t] e^{log_decay_h} S_{t-1} + k_t v_t^T,    out_t = scale S_t^T q_t
+ * for every (batch row, head), from S_{-1} = state (null: zeros); final_state = S_{steps-1} (state
+ * itself without steps). q, k [batch, steps, heads, key_dim] and v, out [batch, steps, heads,
+ * value_dim] in `dtype`, features contiguous, other strides free (in elements; only `out` and the
+ * gradients may not overlap themselves); states [batch, heads, key_dim, value_dim] float32,
+ * contiguous. reset (nullable) [batch, steps] bytes clears the state before a step: what lies
+ * before it, the given state included, has no part in that step or a later one. Heads of 1 to 128
+ * features; log_decay [heads] float32, <= 0 (-inf forgets everything at once), taken as a
+ * constant. Sums and states are float32 or better. The backward takes the gradients of out and
+ * final_state (null: zeros) and writes those of q, k, v and state. The step form takes steps = 1
+ * and the rows' batch and head strides; out [batch, heads, value_dim] is contiguous and new_state
+ * may be state. Workspaces are device memory, 16-byte aligned, of the size that
+ * bt_linear_attention_workspace gives (-1: bad shape), free again when the call's work is done. */
+typedef struct bt_heads {
+  void* data;
+  int64_t batch_stride, step_stride, head_stride;
+} bt_heads;
+typedef struct bt_linear_attention_shape {
+  int32_t batch, steps, heads, key_dim, value_dim, dtype;
+  float scale;
+  const float* log_decay;
+  const uint8_t* reset;
+  int64_t reset_batch_stride, reset_step_stride;
+} bt_linear_attention_shape;
+BT_API int64_t bt_linear_attention_workspace(const bt_linear_attention_shape* shape,
+                                             int32_t backward);
+BT_API int bt_linear_attention(const bt_linear_attention_shape* shape, const bt_heads* q,
+                               const bt_heads* k, const bt_heads* v, const float* state,
+                               const bt_heads* out, float* final_state, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+BT_API int bt_linear_attention_backward(const bt_linear_attention_shape* shape, const bt_heads* q,
+                                        const bt_heads* k, const bt_heads* v, const float* state,
+                                        const bt_heads* dout, const float* dfinal_state,
+                                        const bt_heads* dq, const bt_heads* dk, const bt_heads* dv,
+                                        float* dstate, void* workspace, int64_t workspace_bytes,
+                                        void* stream);
+BT_API int bt_linear_attention_step(const bt_linear_attention_shape* shape, const bt_heads* q,
+                                    const bt_heads* k, const bt_heads* v, const float* state,
+                                    void* out, float* new_state, void* stream);
+
+/* ---- norms of queries and keys with the position rotation ------------------------------------
+ * Every row of q [batch, steps, q_heads, dim] and k [.., k_heads, dim] (`dtype`, features
+ * contiguous) divided by its root mean square (eps added to the mean square), times its weight
+ * [dim] (`weight_dtype`; null: ones), its first 2 half features then turned in pairs by
+ * positions[batch, step] (int64) * frequencies[i] (double): (i, i + half), or (2 i, 2 i + 1) where
+ * interleaved. 1 <= dim <= 256, angles up to 1e15. The backward takes the gradients of both
+ * outputs and writes those of q and k and, where wanted (non-null), of the weights, summed in a
+ * fixed order through `workspace` (bt_qk_norm_rotary_workspace bytes). */
+typedef struct bt_qk_norm_rotary_shape {
+  int32_t batch, steps, q_heads, k_heads, dim, half, dtype, weight_dtype, interleaved;
+  float eps;
+  const int64_t* positions;
+  int64_t positions_batch_stride, positions_step_stride;
+  const double* frequencies;
+} bt_qk_norm_rotary_shape;
+BT_API int bt_qk_norm_rotary(const bt_qk_norm_rotary_shape* shape, const bt_heads* q,
+                             const bt_heads* k, const void* q_weight, const void* k_weight,
+                             const bt_heads* q_out, const bt_heads* k_out, void* stream);
+BT_API int64_t bt_qk_norm_rotary_workspace(const bt_qk_norm_rotary_shape* shape);
+BT_API int bt_qk_norm_rotary_backward(const bt_qk_norm_rotary_shape* shape, const bt_heads* q,
+                                      const bt_heads* k, const void* q_weight, const void* k_weight,
+                                      const bt_heads* dq_out, const bt_heads* dk_out,
+                                      const bt_heads* dq, const bt_heads* dk, void* dq_weight,
+                                      void* dk_weight, void* workspace, int64_t workspace_bytes,
+                                      void* stream);
+
+/* ---- gated feed-forward layer --------------------------------------------------------------
+ * out = act(x w_gate) * (x w_up): x [rows, in_features], weights [in_features, out_features], out
+ * [rows, out_features], all row-major in `dtype`; activation BT_ACT_*. Sums are float32. The
+ * backward takes the gradient of out, forms both projections again and writes dx and (both or
+ * neither) dw_gate and dw_up; a null one is not formed. Workspaces as above (bt_glu_workspace). */
+typedef struct bt_glu_shape {
+  int32_t rows, in_features, out_features, dtype, activation;
+} bt_glu_shape;
+BT_API int64_t bt_glu_workspace(const bt_glu_shape* shape, int32_t backward);
+BT_API int bt_glu(const bt_glu_shape* shape, const void* x, const void* w_gate, const void* w_up,
+                  void* out, void* workspace, int64_t workspace_bytes, void* stream);
+BT_API int bt_glu_backward(const bt_glu_shape* shape, const void* x, const void* w_gate,
+                           const void* w_up, const void* dout, void* dx, void* dw_gate, void* dw_up,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- counter-based random numbers in JAX's threefry conventions ---------------------------
  * (jax.random with threefry2x32 keys; boonta/algorithms/ppo.py:200, 230,
  * boonta/networks/distributions.py:21-23). Keys are two uint32 words (jax.random.key_data);
