@@ -1,5 +1,7 @@
 // Thread-local error messages behind bt_last_error(), and the self-test of the bounded
 // waits that every waiting kernel uses.
+#include <atomic>
+
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -16,7 +18,38 @@ void set_error(const char* fmt, ...) {
 
 const char* last_error() { return g_last_error; }
 
+// The word in which kernels of the stateless operators record a bounded wait that gave up, one on
+// each device.
+__device__ int g_operator_error;
+
+int operator_error_word(int** word) {
+  constexpr int kDevices = 64;
+  static std::atomic<int*> words[kDevices];
+  int device = 0;
+  BT_CUDA(cudaGetDevice(&device));
+  if (device < kDevices && (*word = words[device].load()) != nullptr) return BT_OK;
+  void* p = nullptr;
+  BT_CUDA(cudaGetSymbolAddress(&p, g_operator_error));
+  *word = static_cast<int*>(p);
+  if (device < kDevices) words[device].store(*word);
+  return BT_OK;
+}
+
 }  // namespace bt
+
+extern "C" int bt_operators_check(void* stream) {
+  using namespace bt;
+  cudaStream_t s = (cudaStream_t)stream;
+  int* word = nullptr;
+  BT_TRY(operator_error_word(&word));
+  int code = 0;
+  BT_CUDA(cudaMemcpyAsync(&code, word, sizeof(int), cudaMemcpyDeviceToHost, s));
+  BT_CUDA(cudaStreamSynchronize(s));
+  if (code == 0) return BT_OK;
+  BT_CUDA(cudaMemsetAsync(word, 0, sizeof(int), s));
+  set_error("a bounded wait of an operator's kernel gave up (code %d): its outputs are not valid", code);
+  return BT_ERR_TIMEOUT;
+}
 
 extern "C" const char* bt_last_error(void) { return bt::last_error(); }
 

@@ -1,4 +1,4 @@
-// The gated feed-forward layer h = act(x Wg) * (x Wu): what its kernels share.
+// The gated feed-forward layer h = act(x Wg) * (x Wu): what its files share.
 #pragma once
 
 #include "common.cuh"
@@ -6,11 +6,10 @@
 namespace bt {
 namespace glu {
 
-// One gated layer: x [M, K], Wg and Wu [K, N], h and dh [M, N], row-major.
+// One gated layer: x [M, K], Wg and Wu [K, N], dh [M, N], row-major without gaps.
 struct Layer {
   int M, N, K, act;
   const void *x, *wg, *wu, *dh;
-  int64_t ldx, ldw, lddh;
 };
 
 // The gradients of gate and up projection from their values: dg = dh u act'(g), du = dh act(g).
@@ -19,6 +18,11 @@ __device__ __forceinline__ void gate_grads(float g, float u, float dh, float& dg
   dg = dh * u * act_dz<A>(g);
   du = dh * act_fwd<A>(g);
 }
+
+// Tensor cores (glu_sm100.cu). ws: workspace_of bytes.
+int64_t workspace_of(const Layer& l, bool f32, bool backward);
+int forward(const Layer& l, bool f32, void* h, char* ws, cudaStream_t s);
+int backward(const Layer& l, bool f32, void* dx, void* dwg, void* dwu, char* ws, cudaStream_t s);
 
 }  // namespace glu
 }  // namespace bt

@@ -1,0 +1,734 @@
+// The gated feed-forward layer on the tensor cores (tcgen05), bf16 and fp32.
+//
+// One persistent kernel serves the four products of the layer:
+//   kForward  h = act(x Wg) * (x Wu)         a tile is 128 rows x 128 columns of both projections:
+//                                            one MMA of N = 256 over [Wg tile | Wu tile]
+//   kGrads    dG, dU from the same tiles and dh (the projections are formed again, not kept: at
+//             K <= 800 reading two fp32 values per element back costs more than 4 K flops do)
+//   kInput    dx = dG Wg^T + dU Wu^T         the two products in one accumulator
+//   kWeights  dWg = x^T dG, dWu = x^T dU     both from one load of x, split over the rows
+// A CTA per SM walks the output tiles. Warp 0 loads 64-deep blocks of A and B by TMA into a ring of
+// four 48 KB stages, warp 1 issues the MMAs into one of two 256-column accumulators in tensor
+// memory, and eight epilogue warps drain the other: activation and product in registers, the
+// result through 4 KB of shared memory per warp to TMA stores.
+//
+// fp32 operands are three bf16 planes each, x = x0 + x1 + x2 (24 bits), and a product is the six
+// plane products whose size reaches 2^-24 of it: (0,2) (1,1) (2,0) (0,1) (1,0) (0,0), added in that
+// order, smallest first. The accumulator truncates, so for fp32 it is handed to fp32 registers after
+// every 64-deep block (24 MMAs); 270 of the 1622 bf16 TFLOP/s remain, about four times what the
+// CUDA cores' fp32 FMA does.
+//
+// Bound by the tensor cores: 128 x 256 x 64 per 48 KB of operands, 512 cycles of MMA a block.
+#include <type_traits>
+
+#include "gemm_sm100.cuh"
+#include "glu.cuh"
+
+namespace bt {
+
+int operator_error_word(int** word);
+
+namespace glu {
+namespace {
+
+using namespace umma;
+
+enum Mode { kForward, kGrads, kInput, kWeights };
+
+constexpr int kStages = 4, kBN = 256;
+constexpr int kAB = BM * BK * 2, kBB = kBN * BK * 2, kStageBytes = kAB + kBB;
+constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * kEpiWarpBytes + 1024 + 256;
+static_assert(kSmemBytes <= kMaxSmem, "stage ring");
+
+struct Seg {
+  uint8_t a, b0, b1;  // maps of a product's A and of its B (kInput: b0 alone)
+};
+
+struct Params {
+  CUtensorMap map[12];
+  CUtensorMap out[6], in;
+  Seg seg[12];
+  int nseg;
+  int M, N, K;        // of the product: rows and columns of the output, depth
+  int act;
+  int splits, depth;  // kWeights: 64-deep blocks of a split
+  void *o0, *o1;      // outputs where their rows do not suit TMA stores (ldo), else null
+  const void* dh;     // the same for dh
+  int64_t ldo;
+  int plane_rows;     // kWeights with splits: rows of one partial plane
+  int* err;
+};
+
+template <class T>
+__device__ __forceinline__ T from_f32(float x) {
+  if constexpr (sizeof(T) == 2) return __float2bfloat16_rn(x);
+  return x;
+}
+
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, const void* src, int c, int r, int lane) {
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_2d(map, src, c, r);
+    bulk_commit();
+  }
+}
+
+__device__ __forceinline__ void staging_free(int lane) {
+  if (lane == 0) bulk_wait_read_all();
+  __syncwarp();
+}
+
+// A 32 x 32 tile whose rows do not suit TMA: staged as fp32, written with lanes along the columns.
+template <class T>
+__device__ __forceinline__ void store_plain(T* out, int64_t ld, int row0, int col0, int rows, int cols,
+                                            uint8_t* buf, int lane, const float (&v)[32]) {
+  stage_row_f32(buf, lane, v);
+  __syncwarp();
+  const int n = min(32, rows - row0);
+  if (col0 + lane < cols)
+    for (int r = 0; r < n; ++r)
+      out[(row0 + r) * ld + col0 + lane] = from_f32<T>(
+          *reinterpret_cast<const float*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4));
+  __syncwarp();
+}
+
+template <class T>
+__device__ __forceinline__ void load_plain(const T* in, int64_t ld, int row0, int col0, int rows, int cols,
+                                           uint8_t* buf, int lane) {
+  for (int r = 0; r < 32; ++r) {
+    float v = 0.f;
+    if (row0 + r < rows && col0 + lane < cols) {
+      const T x = in[(row0 + r) * ld + col0 + lane];
+      if constexpr (sizeof(T) == 2) v = __bfloat162float(x); else v = x;
+    }
+    *reinterpret_cast<float*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = v;
+  }
+  __syncwarp();
+}
+
+__device__ __forceinline__ void row_f32(const uint8_t* buf, int lane, float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float4 p = load_row_f32(buf, lane, j);
+    v[4 * j] = p.x, v[4 * j + 1] = p.y, v[4 * j + 2] = p.z, v[4 * j + 3] = p.w;
+  }
+}
+__device__ __forceinline__ void row_bf16(const uint8_t* buf, int lane, float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint4 w = *reinterpret_cast<const uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4));
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&ws[i]);
+      v[8 * j + 2 * i] = __low2float(h);
+      v[8 * j + 2 * i + 1] = __high2float(h);
+    }
+  }
+}
+
+// An output tile in T: through a TMA store (map) or plainly (p.o).
+template <class T>
+__device__ __forceinline__ void put(const CUtensorMap* map, void* plain, const Params& p, int row0, int col0,
+                                    uint8_t* buf, int lane, const float (&v)[32]) {
+  staging_free(lane);
+  if (plain) {
+    store_plain(static_cast<T*>(plain), p.ldo, row0, col0, p.M, p.N, buf, lane, v);
+    return;
+  }
+  if constexpr (sizeof(T) == 2) stage_row_bf16(buf, nullptr, lane, v);
+  else stage_row_f32(buf, lane, v);
+  tma_store(map, buf, col0, row0, lane);
+}
+
+// v as three bf16 planes, v = v0 + v1 + v2 to 24 bits.
+__device__ __forceinline__ void put_planes(const CUtensorMap* maps, int row0, int col0, uint8_t* buf, int lane,
+                                           float (&v)[32]) {
+  staging_free(lane);
+  stage_row_bf16(buf, buf + 2048, lane, v);
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_2d(&maps[0], buf, col0, row0);
+    tma_store_2d(&maps[1], buf + 2048, col0, row0);
+    bulk_commit();
+  }
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
+    v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
+  }
+  staging_free(lane);
+  stage_row_bf16(buf, nullptr, lane, v);
+  tma_store(&maps[2], buf, col0, row0, lane);
+}
+
+// T: the layer's type. An fp32 layer's operands are planes and its accumulator is handed over after
+// every 64-deep block.
+template <class T, Mode kMode>
+__global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant__ Params p) {
+  constexpr bool kF32 = sizeof(T) == 4;
+  constexpr bool kDual = kMode != kInput;
+  constexpr bool A_MN = kMode == kWeights, B_MN = kMode != kInput;
+  constexpr int kTileN = kDual ? kBN / 2 : kBN;
+  // 64-deep blocks between two hand-overs of the accumulator: bf16 results keep 2^-8, far above what
+  // the truncation of a whole product leaves
+  constexpr int kHand = kF32 ? 1 : 1 << 30;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* epi_smem = smem + kStages * kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(epi_smem + kEpiWarps * kEpiWarpBytes);
+  uint64_t* empty = full + kStages;
+  uint64_t* acc_full = empty + kStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* epi_in = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(epi_in + kEpiWarps);
+  __shared__ int s_fail;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    s_fail = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], kEpiWarps);
+    }
+    for (int w = 0; w < kEpiWarps; ++w) mbar_init(&epi_in[w], 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, 2 * kBN);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  auto failed = [&]() { return *(volatile int*)&s_fail != 0; };
+  pdl_wait();
+  const int ntn = ceil_div(p.N, kTileN), ntm = ceil_div(p.M, BM);
+  const int nk = ceil_div(p.K, BK);
+  const int tiles = ntm * ntn * p.splits;
+  // the splits of one tile lie far apart, the column tiles of one row block together
+  auto where = [&](int t, int& m0, int& n0, int& k0, int& k1, int& split) {
+    split = t / (ntm * ntn);
+    const int u = t % (ntm * ntn);
+    m0 = u / ntn * BM;
+    n0 = u % ntn * kTileN;
+    k0 = split * p.depth;
+    k1 = min(nk, k0 + p.depth);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int g = 0;
+      for (int t = blockIdx.x; t < tiles && !failed(); t += gridDim.x) {
+        int m0, n0, k0, k1, split;
+        where(t, m0, n0, k0, k1, split);
+        for (int kb = k0; kb < k1 && !failed(); ++kb) {
+          const int k = kb * BK;
+          for (int e = 0; e < p.nseg; ++e, ++g) {
+            const int s = g % kStages;
+            if (g >= kStages && !mbar_wait_bounded(&empty[s], ((g / kStages) - 1) & 1)) {
+              atomicExch(&s_fail, kErrTimeoutEmpty);
+              break;
+            }
+            uint8_t* sa = smem + s * kStageBytes;
+            uint8_t* sb = sa + kAB;
+            mbar_arrive_expect_tx(&full[s], kStageBytes);
+            const Seg sg = p.seg[e];
+            if (A_MN) {
+              tma_load_2d(sa, &p.map[sg.a], m0, k, &full[s]);
+              tma_load_2d(sa + 8192, &p.map[sg.a], m0 + 64, k, &full[s]);
+            } else {
+              tma_load_2d(sa, &p.map[sg.a], k, m0, &full[s]);
+            }
+            if (kDual) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                tma_load_2d(sb + j * 8192, &p.map[j < 2 ? sg.b0 : sg.b1], n0 + 64 * (j & 1), k, &full[s]);
+            } else {
+              tma_load_2d(sb, &p.map[sg.b0], k, n0, &full[s]);
+            }
+          }
+        }
+      }
+      // every copy lands before the CTA may leave
+      for (int i = max(0, g - kStages); i < g; ++i)
+        if (!mbar_wait_bounded(&full[i % kStages], (i / kStages) & 1)) atomicExch(&s_fail, kErrTimeoutFull);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = instr_desc<kBN, A_MN, B_MN>();
+      int g = 0, c = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok && !failed(); t += gridDim.x) {
+        int m0, n0, k0, k1, split;
+        where(t, m0, n0, k0, k1, split);
+        for (int kb = k0; kb < k1 && ok; ++kb) {
+          const bool fresh = (kb - k0) % kHand == 0;
+          if (fresh && c >= 2) {
+            if (!mbar_wait_bounded(&acc_empty[c & 1], ((c >> 1) - 1) & 1)) {
+              atomicExch(&s_fail, kErrTimeoutAcc);
+              ok = false;
+              break;
+            }
+            fence_after_sync();
+          }
+          const uint32_t acc = tmem + (uint32_t)((c & 1) * kBN);
+          for (int e = 0; e < p.nseg; ++e, ++g) {
+            const int s = g % kStages;
+            if (!mbar_wait_bounded(&full[s], (g / kStages) & 1)) {
+              atomicExch(&s_fail, kErrTimeoutFull);
+              ok = false;
+              break;
+            }
+            fence_after_sync();
+            const uint32_t sa = smem_u32(smem + s * kStageBytes), sb = sa + kAB;
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k)
+              mma_bf16(acc, operand_desc<A_MN>(sa, k), operand_desc<B_MN>(sb, k), idesc,
+                       (!fresh || e > 0 || k > 0) ? 1u : 0u);
+            mma_commit(&empty[s]);
+          }
+          if (ok && ((kb - k0) % kHand == kHand - 1 || kb == k1 - 1)) {
+            mma_commit(&acc_full[c & 1]);
+            ++c;
+          }
+        }
+      }
+    }
+  } else {
+    // Epilogue: rows 32 q .. of the tile, thread = row; half of the columns (of each projection).
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* buf = epi_smem + (warp - 2) * kEpiWarpBytes;
+    uint64_t* ibar = &epi_in[warp - 2];
+    const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
+    // TMEM column of this warp's group j: two groups of each projection, or four of the one product
+    auto column = [&](int j) {
+      return kDual ? (j >> 1) * (kBN / 2) + half * 64 + (j & 1) * 32 : half * 128 + j * 32;
+    };
+    float run[kF32 ? 4 : 1][32];
+    int c = 0, loads = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok && !failed(); t += gridDim.x) {
+      int m0, n0, k0, k1, split;
+      where(t, m0, n0, k0, k1, split);
+      const int row0 = m0 + q * 32;
+      if constexpr (kF32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) run[j][i] = 0.f;
+        for (int kb = k0; kb < k1; ++kb, ++c) {
+          ok = mbar_wait_bounded(&acc_full[c & 1], (c >> 1) & 1);
+          if (!ok) break;
+          fence_after_sync();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float v[32];
+            tmem_ld32(lanes + (uint32_t)((c & 1) * kBN + column(j)), v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) run[j][i] += v[i];
+          }
+          fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[c & 1]);
+        }
+      } else {
+        ok = mbar_wait_bounded(&acc_full[c & 1], (c >> 1) & 1);
+        fence_after_sync();
+      }
+      if (!ok) {
+        if (lane == 0) atomicExch(&s_fail, kErrTimeoutAcc);
+        break;
+      }
+      const uint32_t acc = lanes + (uint32_t)((c & 1) * kBN);
+      auto group = [&](int j, float (&v)[32]) {
+        if constexpr (kF32) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = run[j][i];
+        } else {
+          tmem_ld32(acc + (uint32_t)column(j), v);
+        }
+      };
+      auto release = [&]() {
+        if constexpr (!kF32) {
+          fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty[c & 1]);
+          ++c;
+        }
+      };
+      if constexpr (kMode == kForward || kMode == kGrads) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int col0 = n0 + half * 64 + 32 * j;
+          const bool in = col0 < p.N && row0 < p.M;
+          if (kMode == kGrads && in) {
+            staging_free(lane);
+            if (p.dh) {
+              load_plain(static_cast<const T*>(p.dh), (int64_t)p.N, row0, col0, p.M, p.N, buf, lane);
+            } else if (lane == 0) {
+              mbar_arrive_expect_tx(ibar, 32 * 32 * sizeof(T));
+              tma_load_2d(buf, &p.in, col0, row0, ibar);
+            }
+          }
+          float g[32], u[32];
+          group(j, g);
+          group(2 + j, u);
+          if (j == 1) release();
+          if constexpr (kMode == kForward) {
+            if (!in) continue;
+            with_act(p.act, [&](auto tag) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) g[i] = act_fwd<decltype(tag)::value>(g[i]) * u[i];
+            });
+            put<T>(&p.out[0], p.o0, p, row0, col0, buf, lane, g);
+          } else {
+            if (!in) continue;
+            float d[32];
+            if (p.dh) {
+              row_f32(buf, lane, d);
+            } else {
+              if (!mbar_wait_bounded(ibar, loads & 1)) {
+                if (lane == 0) atomicExch(&s_fail, kErrTimeoutEpiIn);
+                ok = false;
+              }
+              ++loads;
+              if constexpr (kF32) row_f32(buf, lane, d);
+              else row_bf16(buf, lane, d);
+            }
+            __syncwarp();
+            with_act(p.act, [&](auto tag) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                float dg, du;
+                gate_grads<decltype(tag)::value>(g[i], u[i], d[i], dg, du);
+                g[i] = dg;
+                u[i] = du;
+              }
+            });
+            if constexpr (kF32) {
+              put_planes(&p.out[0], row0, col0, buf, lane, g);
+              put_planes(&p.out[3], row0, col0, buf, lane, u);
+            } else {
+              stage_row_bf16(buf, nullptr, lane, g);
+              stage_row_bf16(buf + 2048, nullptr, lane, u);
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&p.out[0], buf, col0, row0);
+                tma_store_2d(&p.out[1], buf + 2048, col0, row0);
+                bulk_commit();
+              }
+            }
+          }
+        }
+      } else if constexpr (kMode == kInput) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int col0 = n0 + half * 128 + 32 * j;
+          float v[32];
+          group(j, v);
+          if (j == 3) release();
+          if (col0 < p.N && row0 < p.M) put<T>(&p.out[0], p.o0, p, row0, col0, buf, lane, v);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int which = j >> 1, col0 = n0 + half * 64 + 32 * (j & 1);
+          float v[32];
+          group(j, v);
+          if (j == 3) release();
+          if (col0 >= p.N || row0 >= p.M) continue;
+          if (p.splits > 1) {  // one partial plane for each split and weight
+            put<float>(&p.out[0], nullptr, p, (2 * split + which) * p.plane_rows + row0, col0, buf, lane, v);
+          } else {
+            put<T>(&p.out[which], which ? p.o1 : p.o0, p, row0, col0, buf, lane, v);
+          }
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+    __syncwarp();
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    fence_after_sync();
+    tmem_dealloc(tmem, 2 * kBN);
+  }
+  if (threadIdx.x == 0 && s_fail) atomicExch(p.err, s_fail);
+}
+
+// An operand as the kernel reads it: rows of ld (a multiple of 8) bf16, kPlanes planes of them.
+// Thread: eight columns of a row.
+template <class T, int kPlanes>
+__global__ void __launch_bounds__(256) planes_kernel(const T* src, int64_t rows, int cols, int ld, __nv_bfloat16* dst) {
+  const int per = ld / 8;
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= rows * per) return;
+  const int64_t r = e / per;
+  const int c = (int)(e % per) * 8;
+  const T* s = src + r * cols + c;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = 0.f;
+    if (c + i < cols) {
+      if constexpr (sizeof(T) == 2) v[i] = __bfloat162float(s[i]); else v[i] = s[i];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kPlanes; ++k) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+      const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&w[i]);
+      v[2 * i] -= __low2float(h);
+      v[2 * i + 1] -= __high2float(h);
+    }
+    *reinterpret_cast<uint4*>(dst + (k * rows + r) * ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// dWg and dWu: the splits' partial planes [splits][2][plane_rows][ld] added in their order.
+template <class T>
+__global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int rows, int cols, int plane_rows,
+                                                   int ld, T* dwg, T* dwu) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = ld / 4;
+  if (e >= (int64_t)rows * per) return;
+  const int r = (int)(e / per), c = (int)(e % per) * 4;
+  const float* s = part + ((int64_t)blockIdx.y * plane_rows + r) * ld + c;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < splits; ++k) {
+    const float4 b = *reinterpret_cast<const float4*>(s + (int64_t)2 * k * plane_rows * ld);
+    a.x += b.x, a.y += b.y, a.z += b.z, a.w += b.w;
+  }
+  T* o = (blockIdx.y ? dwu : dwg) + (int64_t)r * cols + c;
+  const float v[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (c + i < cols) o[i] = from_f32<T>(v[i]);
+}
+
+int round_up(int x, int m) { return (x + m - 1) / m * m; }
+int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
+
+// Splits of the rows for the weight gradients: whole waves of tiles against the partial planes' way
+// through memory (written and read once at about 5 TB/s); a 64-deep block of a tile takes 0.33 us
+// (fp32: six times that).
+int choose_splits(int M, int K, int N, int planes) {
+  const int tiles = ceil_div(K, BM) * ceil_div(N, kBN / 2), nk = ceil_div(M, BK);
+  const double block = planes == 3 ? 2.0 : 0.33;
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= 32 && s <= nk; ++s) {
+    const double us = ceil_div(tiles * s, kNumSMs) * ceil_div(nk, s) * block +
+                      (s > 1 ? 2.0 + s * 2.0 * K * N * 8 / 5e6 : 0.0);
+    if (us < least) least = us, best = s;
+  }
+  return ceil_div(nk, ceil_div(nk, best));
+}
+
+// The layer's operands in the workspace: planes of x and of the weights (bf16 layers whose rows suit
+// TMA are read where they are), of dG and dU, and the weight gradients' partial planes.
+struct Plan {
+  int planes, ldk, ldn, splits, plane_rows, ldp;
+  int64_t x, wg, wu, dg, du, part, bytes;  // offsets; x, wg, wu: -1 read in place
+};
+
+Plan plan_of(const Layer& l, bool f32, bool backward) {
+  Plan w{};
+  w.planes = f32 ? 3 : 1;
+  w.ldk = round_up(l.K, 8);
+  w.ldn = round_up(l.N, 8);
+  int64_t at = 0;
+  auto take = [&](int64_t elems, int64_t size) {
+    const int64_t o = at;
+    at += align256(elems * size);
+    return o;
+  };
+  const bool copy_x = f32 || l.K % 8, copy_w = f32 || l.N % 8;
+  w.x = copy_x ? take((int64_t)w.planes * l.M * w.ldk, 2) : -1;
+  w.wg = copy_w ? take((int64_t)w.planes * l.K * w.ldn, 2) : -1;
+  w.wu = copy_w ? take((int64_t)w.planes * l.K * w.ldn, 2) : -1;
+  w.splits = 1;
+  if (backward) {
+    w.dg = take((int64_t)w.planes * l.M * w.ldn, 2);
+    w.du = take((int64_t)w.planes * l.M * w.ldn, 2);
+    w.splits = choose_splits(l.M, l.K, l.N, w.planes);
+    w.plane_rows = round_up(l.K, BM);
+    w.ldp = round_up(l.N, 4);
+    if (w.splits > 1) w.part = take((int64_t)2 * w.splits * w.plane_rows * w.ldp, 4);
+  }
+  w.bytes = at;
+  return w;
+}
+
+template <class T>
+struct Run {
+  static constexpr bool kF32 = sizeof(T) == 4;
+  static constexpr int kP = kF32 ? 3 : 1;
+  const Layer& l;
+  Plan w;
+  char* ws;
+  cudaStream_t s;
+  const __nv_bfloat16 *x, *wg, *wu;
+  int ldx, ldw;
+
+  int operand(const void* src, int64_t rows, int cols, int ld, int64_t at, const __nv_bfloat16** to) {
+    if (at < 0) {
+      *to = static_cast<const __nv_bfloat16*>(src);
+      return BT_OK;
+    }
+    __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(ws + at);
+    planes_kernel<T, kP><<<(unsigned)ceil_div64(rows * (ld / 8), 256), 256, 0, s>>>(static_cast<const T*>(src), rows,
+                                                                                    cols, ld, dst);
+    BT_LAUNCH_CHECK("gated layer operand planes");
+    *to = dst;
+    return BT_OK;
+  }
+  int operands() {
+    ldx = w.x < 0 ? l.K : w.ldk;
+    ldw = w.wg < 0 ? l.N : w.ldn;
+    BT_TRY(operand(l.x, l.M, l.K, w.ldk, w.x, &x));
+    BT_TRY(operand(l.wg, l.K, l.N, w.ldn, w.wg, &wg));
+    return operand(l.wu, l.K, l.N, w.ldn, w.wu, &wu);
+  }
+  // Maps of an operand's planes, `box` rows of 64 columns at a time.
+  int maps(CUtensorMap* m, const __nv_bfloat16* base, int64_t rows, int cols, int ld, int box) {
+    for (int k = 0; k < kP; ++k)
+      BT_TRY(encode_map(&m[k], base + k * rows * ld, cols, rows, (uint64_t)ld * 2, 64, box));
+    return BT_OK;
+  }
+  // The products of planes i and j with i + j <= 2, smallest first; `pairs` operand pairs each.
+  static int segments(Seg* seg, int pairs, bool dual) {
+    static const uint8_t ij[6][2] = {{0, 2}, {1, 1}, {2, 0}, {0, 1}, {1, 0}, {0, 0}};
+    int n = 0;
+    for (int k = kF32 ? 0 : 5; k < 6; ++k)
+      for (int q = 0; q < pairs; ++q) {
+        // dual: A planes, then those of both Bs. Otherwise: A0, A1, B0, B1
+        const int a = dual ? 0 : q * kP, b = dual ? kP : (2 + q) * kP;
+        seg[n++] = {(uint8_t)(a + ij[k][0]), (uint8_t)(b + ij[k][1]), (uint8_t)(b + kP + ij[k][1])};
+      }
+    return n;
+  }
+  template <Mode kMode>
+  int launch(Params& p) {
+    auto kernel = glu_kernel<T, kMode>;
+    BT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+    BT_TRY(operator_error_word(&p.err));
+    const int tiles = ceil_div(p.M, BM) * ceil_div(p.N, kMode == kInput ? kBN : kBN / 2) * p.splits;
+    BT_CUDA(launch_pdl(kernel, dim3(min(tiles, kNumSMs)), dim3(kThreads), kSmemBytes, s, p));
+    return BT_OK;
+  }
+  // A row-major T output (or dh) of `cols` columns: by TMA where its rows suit it.
+  static bool suits(int cols) { return cols % (16 / (int)sizeof(T)) == 0; }
+  int tile_map(CUtensorMap* m, const void* base, int64_t rows, int cols) {
+    return encode_tile_map(m, base, kF32, cols, rows, (uint64_t)cols * sizeof(T), kF32 ? 128 : 64);
+  }
+
+  // G and U of every tile: h, or dG and dU into the workspace.
+  template <Mode kMode>
+  int project(void* h) {
+    Params p{};
+    p.M = l.M, p.N = l.N, p.K = l.K, p.act = l.act, p.splits = 1, p.depth = ceil_div(l.K, BK);
+    BT_TRY(maps(&p.map[0], x, l.M, l.K, ldx, BM));
+    BT_TRY(maps(&p.map[kP], wg, l.K, l.N, ldw, 64));
+    BT_TRY(maps(&p.map[2 * kP], wu, l.K, l.N, ldw, 64));
+    p.nseg = segments(p.seg, 1, true);
+    p.ldo = l.N;
+    if constexpr (kMode == kForward) {
+      if (suits(l.N)) BT_TRY(tile_map(&p.out[0], h, l.M, l.N));
+      else p.o0 = h;
+    } else {
+      for (int k = 0; k < 2 * kP; ++k) {
+        const char* base = ws + (k < kP ? w.dg : w.du) + (int64_t)(k % kP) * l.M * w.ldn * 2;
+        BT_TRY(encode_tile_map(&p.out[k], base, false, l.N, l.M, (uint64_t)w.ldn * 2, 64));
+      }
+      if (suits(l.N)) BT_TRY(tile_map(&p.in, l.dh, l.M, l.N));
+      else p.dh = l.dh;
+    }
+    return launch<kMode>(p);
+  }
+  int input(void* dx) {
+    Params p{};
+    p.M = l.M, p.N = l.K, p.K = l.N, p.splits = 1, p.depth = ceil_div(l.N, BK);
+    BT_TRY(maps(&p.map[0], reinterpret_cast<const __nv_bfloat16*>(ws + w.dg), l.M, l.N, w.ldn, BM));
+    BT_TRY(maps(&p.map[kP], reinterpret_cast<const __nv_bfloat16*>(ws + w.du), l.M, l.N, w.ldn, BM));
+    BT_TRY(maps(&p.map[2 * kP], wg, l.K, l.N, ldw, kBN));
+    BT_TRY(maps(&p.map[3 * kP], wu, l.K, l.N, ldw, kBN));
+    p.nseg = segments(p.seg, 2, false);
+    p.ldo = l.K;
+    if (suits(l.K)) BT_TRY(tile_map(&p.out[0], dx, l.M, l.K));
+    else p.o0 = dx;
+    return launch<kInput>(p);
+  }
+  int weights(void* dwg, void* dwu) {
+    Params p{};
+    p.M = l.K, p.N = l.N, p.K = l.M;
+    p.splits = w.splits;
+    p.depth = ceil_div(ceil_div(l.M, BK), w.splits);
+    BT_TRY(maps(&p.map[0], x, l.M, l.K, ldx, 64));
+    BT_TRY(maps(&p.map[kP], reinterpret_cast<const __nv_bfloat16*>(ws + w.dg), l.M, l.N, w.ldn, 64));
+    BT_TRY(maps(&p.map[2 * kP], reinterpret_cast<const __nv_bfloat16*>(ws + w.du), l.M, l.N, w.ldn, 64));
+    p.nseg = segments(p.seg, 1, true);
+    p.ldo = l.N;
+    p.plane_rows = w.plane_rows;
+    float* part = reinterpret_cast<float*>(ws + w.part);
+    if (w.splits > 1) {
+      BT_TRY(encode_tile_map(&p.out[0], part, true, l.N, (uint64_t)2 * w.splits * w.plane_rows, (uint64_t)w.ldp * 4, 128));
+    } else if (suits(l.N)) {
+      BT_TRY(tile_map(&p.out[0], dwg, l.K, l.N));
+      BT_TRY(tile_map(&p.out[1], dwu, l.K, l.N));
+    } else {
+      p.o0 = dwg;
+      p.o1 = dwu;
+    }
+    BT_TRY(launch<kWeights>(p));
+    if (w.splits > 1) {
+      const dim3 grid((unsigned)ceil_div64((int64_t)l.K * (w.ldp / 4), 256), 2);
+      join_kernel<T><<<grid, 256, 0, s>>>(part, w.splits, l.K, l.N, w.plane_rows, w.ldp, static_cast<T*>(dwg),
+                                          static_cast<T*>(dwu));
+      BT_LAUNCH_CHECK("gated layer weight gradients");
+    }
+    return BT_OK;
+  }
+};
+
+}  // namespace
+
+int64_t workspace_of(const Layer& l, bool f32, bool backward) { return plan_of(l, f32, backward).bytes; }
+
+template <class T>
+static int forward_t(const Layer& l, void* h, char* ws, cudaStream_t s) {
+  Run<T> r{l, plan_of(l, sizeof(T) == 4, false), ws, s};
+  BT_TRY(r.operands());
+  return r.template project<kForward>(h);
+}
+
+template <class T>
+static int backward_t(const Layer& l, void* dx, void* dwg, void* dwu, char* ws, cudaStream_t s) {
+  Run<T> r{l, plan_of(l, sizeof(T) == 4, true), ws, s};
+  BT_TRY(r.operands());
+  BT_TRY(r.template project<kGrads>(nullptr));
+  if (dx) BT_TRY(r.input(dx));
+  if (dwg) BT_TRY(r.weights(dwg, dwu));
+  return BT_OK;
+}
+
+int forward(const Layer& l, bool f32, void* h, char* ws, cudaStream_t s) {
+  return f32 ? forward_t<float>(l, h, ws, s) : forward_t<__nv_bfloat16>(l, h, ws, s);
+}
+
+int backward(const Layer& l, bool f32, void* dx, void* dwg, void* dwu, char* ws, cudaStream_t s) {
+  return f32 ? backward_t<float>(l, dx, dwg, dwu, ws, s) : backward_t<__nv_bfloat16>(l, dx, dwg, dwu, ws, s);
+}
+
+}  // namespace glu
+}  // namespace bt

@@ -32,6 +32,12 @@ def _check(x, w_gate, w_up, activation):
             raise ValueError("gated_linear_unit: CUDA tensors on one device expected")
 
 
+def _aligned(t):
+    """t without gaps, from a 16-byte boundary."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _shape(x, w, activation):
     return _lib.GluShape(x.shape[0], w.shape[0], w.shape[1], _DTYPES[x.dtype], _lib.ACT[activation])
 
@@ -44,7 +50,7 @@ def _workspace(shape, backward, device):
 class _Glu(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, activation):
-        x, w_gate, w_up = x.contiguous(), w_gate.contiguous(), w_up.contiguous()
+        x, w_gate, w_up = _aligned(x), _aligned(w_gate), _aligned(w_up)
         out = torch.empty(x.shape[0], w_gate.shape[1], dtype=x.dtype, device=x.device)
         with _on(x.device):
             shape = _shape(x, w_gate, activation)
@@ -60,7 +66,7 @@ class _Glu(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         x, w_gate, w_up = ctx.saved_tensors
-        dout = dout.to(x.dtype).contiguous()
+        dout = _aligned(dout.to(x.dtype))
         dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
         weights = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dwg = torch.empty_like(w_gate) if weights else None

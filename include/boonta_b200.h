@@ -247,7 +247,8 @@ BT_API int bt_qk_norm_rotary_backward(const bt_qk_norm_rotary_shape* shape, cons
  * out = act(x w_gate) * (x w_up): x [rows, in_features], weights [in_features, out_features], out
  * [rows, out_features], all row-major in `dtype`; activation BT_ACT_*. Sums are float32. The
  * backward takes the gradient of out, forms both projections again and writes dx and (both or
- * neither) dw_gate and dw_up; a null one is not formed. Workspaces as above (bt_glu_workspace). */
+ * neither) dw_gate and dw_up; a null one is not formed. Pointers are 16-byte aligned. Workspaces as
+ * above (bt_glu_workspace). */
 typedef struct bt_glu_shape {
   int32_t rows, in_features, out_features, dtype, activation;
 } bt_glu_shape;
@@ -257,6 +258,11 @@ BT_API int bt_glu(const bt_glu_shape* shape, const void* x, const void* w_gate, 
 BT_API int bt_glu_backward(const bt_glu_shape* shape, const void* x, const void* w_gate,
                            const void* w_up, const void* dout, void* dx, void* dw_gate, void* dw_up,
                            void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Synchronises `stream` and reports (once) a bounded wait that gave up inside a kernel of the
+ * operators above on the current device: BT_ERR_TIMEOUT, the outputs of calls since the last check
+ * are then not valid. */
+BT_API int bt_operators_check(void* stream);
 
 /* ---- counter-based random numbers in JAX's threefry conventions ---------------------------
  * (jax.random with threefry2x32 keys; boonta/algorithms/ppo.py:200, 230,
