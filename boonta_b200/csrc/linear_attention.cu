@@ -21,11 +21,6 @@ constexpr int kC = 32;       // positions of a chunk
 constexpr int kDS = 64;      // columns of c (and of the state) of a block
 constexpr int kThreads = 256;
 
-struct Ops {
-  Op op[3];
-  int n;
-};
-
 template <int DA>
 struct Smem {
   float a[kC][DA + 4], b[kC][DA + 4], c[kC][kDS + 4], s[DA][kDS + 4], p[kC][kC + 1];
@@ -319,12 +314,11 @@ __global__ void __launch_bounds__(kThreads)
 
 template <class T>
 int run_ops(Ops& ops, cudaStream_t stream) {
-  int da = 0, blocks = 0, elems = 0;
+  int da = 0, blocks = 0;
   for (int i = 0; i < ops.n; ++i) {
     const Op& o = ops.op[i];
     da = max(da, o.Da);
     blocks = max(blocks, o.batch * o.heads * ceil_div(o.Dc, kDS));
-    elems = max(elems, o.Da * o.Dc);
   }
   const Op& o = ops.op[0];
   auto go = [&](auto size) -> int {
@@ -337,9 +331,7 @@ int run_ops(Ops& ops, cudaStream_t stream) {
     if (o.nsplit > 1) {
       chunk_kernel<T, DA, false><<<dim3(blocks, o.nsplit - 1, ops.n), kThreads, kSmem, stream>>>(ops);
       BT_LAUNCH_CHECK("linear attention split sums");
-      const int64_t total = (int64_t)o.batch * o.heads * elems;
-      join_kernel<<<dim3((unsigned)ceil_div64(total, 256), ops.n), 256, 0, stream>>>(ops);
-      BT_LAUNCH_CHECK("linear attention join");
+      BT_TRY(launch_join(ops, stream));
     }
     chunk_kernel<T, DA, true><<<dim3(blocks, o.nsplit, ops.n), kThreads, kSmem, stream>>>(ops);
     BT_LAUNCH_CHECK("linear attention");
@@ -349,12 +341,19 @@ int run_ops(Ops& ops, cudaStream_t stream) {
   return go(std::integral_constant<int, 128>{});
 }
 
-// Splits of the steps: enough blocks to fill the GPU twice, at least 128 positions each.
-void choose_splits(int batch, int heads, int steps, int ops, int* nsplit, int* len) {
-  const int want = ceil_div(2 * kNumSMs, max(1, batch * heads * ops));
-  const int n = max(1, min(want, steps / 128));
-  *len = max(kC, ceil_div(ceil_div(steps, n), kC) * kC);
-  *nsplit = max(1, ceil_div(steps, *len));
+// Splits of the steps: the number whose launches fill the GPU best, a walk over all splits counted
+// as two blocks an SM, and the sums of the splits (two of the four streams of a full walk, and a launch)
+// as two fifths more. At least four of the tensor cores' chunks each.
+void choose_splits(const bt_linear_attention_shape* s, int ops, int* nsplit, int* len) {
+  const int64_t blocks = (int64_t)s->batch * s->heads * ceil_div(max(s->key_dim, s->value_dim), kDS) * ops;
+  int best = 1;
+  double least = 1e300;
+  for (int n = 1; n <= 32 && n <= max(1, s->steps / 512); ++n) {
+    const double t = (double)ceil_div64(blocks * n, 2 * kNumSMs) / n * (n > 1 ? 1.4 : 1.0);
+    if (t < least) least = t, best = n;
+  }
+  *len = max(128, ceil_div(ceil_div(s->steps, best), 128) * 128);
+  *nsplit = max(1, ceil_div(s->steps, *len));
 }
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
@@ -374,7 +373,7 @@ int check_shape(const bt_linear_attention_shape* s, const char* who) {
 
 int64_t workspace_bytes(const bt_linear_attention_shape* s, int ops) {
   int nsplit, len;
-  choose_splits(s->batch, s->heads, s->steps, ops, &nsplit, &len);
+  choose_splits(s, ops, &nsplit, &len);
   if (nsplit == 1) return 0;
   const int64_t state = (int64_t)s->batch * s->heads * s->key_dim * s->value_dim * 4;
   return ops * (align256((nsplit - 1) * state) + align256((int64_t)(nsplit - 1) * s->batch * 4));
@@ -412,7 +411,7 @@ Op op_of(const bt_linear_attention_shape* s, const bt_heads& a, const bt_heads& 
 int launch(const bt_linear_attention_shape* s, Ops& ops, void* workspace, int64_t bytes,
            cudaStream_t stream, const char* who) {
   int nsplit, len;
-  choose_splits(s->batch, s->heads, s->steps, ops.n, &nsplit, &len);
+  choose_splits(s, ops.n, &nsplit, &len);
   const int64_t need = workspace_bytes(s, ops.n);
   BT_CHECK_ARG(need == 0 || (workspace && bytes >= need), "%s: workspace of %lld bytes, %lld needed",
                who, (long long)bytes, (long long)need);
@@ -431,8 +430,24 @@ int launch(const bt_linear_attention_shape* s, Ops& ops, void* workspace, int64_
     }
   }
   if (s->batch == 0 || s->heads == 0) return BT_OK;
-  return s->dtype == BT_DTYPE_BF16 ? run_ops<__nv_bfloat16>(ops, stream) : run_ops<float>(ops, stream);
+  if (s->dtype == BT_DTYPE_F32) return run_ops<float>(ops, stream);
+  bool suits = s->steps > 0;
+  for (int i = 0; i < ops.n; ++i) suits = suits && suits_tensor_cores(ops.op[i]);
+  return suits ? run_tensor_cores(ops, stream) : run_ops<__nv_bfloat16>(ops, stream);
 }
+
+}  // namespace
+
+int launch_join(const Ops& ops, cudaStream_t stream) {
+  int64_t total = 0;
+  for (int i = 0; i < ops.n; ++i)
+    total = max(total, (int64_t)ops.op[i].batch * ops.op[i].heads * ops.op[i].Da * ops.op[i].Dc);
+  join_kernel<<<dim3((unsigned)ceil_div64(total, 256), ops.n), 256, 0, stream>>>(ops);
+  BT_LAUNCH_CHECK("linear attention join");
+  return BT_OK;
+}
+
+namespace {
 
 bool rows_ok(const bt_linear_attention_shape* s, const bt_heads* h) {
   return h && (h->data || (int64_t)s->batch * s->steps * s->heads == 0);

@@ -45,6 +45,17 @@ struct Op {
   int* cut;
 };
 
+struct Ops {  // one launch's operations, of the same sequences
+  Op op[3];
+  int n;
+};
+
+// bf16 on the tensor cores (linear_attention_sm100.cu): where every row starts on a 16-byte boundary.
+bool suits_tensor_cores(const Op& o);
+int run_tensor_cores(Ops& ops, cudaStream_t stream);
+// Turns the splits' own sums into the states that enter the splits (linear_attention.cu).
+int launch_join(const Ops& ops, cudaStream_t stream);
+
 // A log decay below this has e^{n g} = 0 for n >= 1 and keeps e^{0 g} = 1 (an infinite one
 // would give 0 * inf).
 constexpr float kMinLogDecay = -1e4f;
