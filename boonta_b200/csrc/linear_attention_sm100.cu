@@ -2,24 +2,32 @@
 // linear_attention.cuh).
 //
 // A block owns one (batch row, head), 64 columns of c and of the state, and walks its positions 128 at
-// a time. In a chunk, with p the position of a row and everything accumulated in fp32:
+// a time. In a chunk, with p the position of a row, w_j = in_scale e^{(n - 1 - p_j) g}, and everything
+// accumulated in fp32:
 //   P0 = a b^T                                     [128 x 128]  tensor memory
-//   O2 = a S                                       [128 x 64]   S: bf16 copy of the state in shared memory
-//   P  = P0 * e^{(p_i - p_j) g}, 0 above the diagonal and across a cut, to bf16 in tensor memory
-//   O1 = P c                                       [128 x 64]   P is the A operand from tensor memory
-//   L  = b^T (w c), w_j = e^{(n - 1 - p_j) g}      [Da x 64]    w c as three bf16 planes (24 bits)
-//   out = in_scale O1 + e^{(p + e0) g} O2, times out_scale;   S = e^{(n - 1 + e0) g} S + in_scale L
+//   O  = a S                                       [128 x 64]   S: bf16 copy of the state in shared memory
+//   L  = b^T (w c)                                 [Da x 64]    w c as three bf16 planes (24 bits)
+//   S  = e^{(n - 1 + e0) g} S + L
+// and for a head with |g| <= 0.23 (its weights across a chunk stay above e^-30), where S is copied with
+// its decay over the chunk to come:
+//   P  = P0, 0 above the diagonal and across a cut, to bf16 in place of P0
+//   O += P (w c), the first two planes;   out = out_scale e^{(p - n + 1) g} O
+// so that no weight meets the 128 x 128 scores. For a head that decays faster those factors would leave
+// the range of fp32, and the weights go where they are at most 1:
+//   P  = in_scale P0 e^{(p_i - p_j) g}, 0 above the diagonal and across a cut
+//   O  = e^{(p + e0) g} O + P c;   out = out_scale O
 // The state itself stays in fp32 registers for the whole walk. Only two factors are rounded to bf16, P
-// and the copy of S that O2 reads, and both go only into outputs that are rounded to bf16 themselves
+// and the copy of S that O reads, and both go only into outputs that are rounded to bf16 themselves
 // (each adds 2^-9 root mean square at most); the state, which is handed on in fp32, comes from exact
-// products: b is bf16 already, and w c keeps 24 bits.
+// products: b is bf16 already, and w c keeps its 24 bits.
 //
 // Backwards the tiles stay in the order of time and the positions run against it: p = 127 - r.
 //
-// Bound by HBM (4 elements of traffic per element of out); a chunk is a chain of dependent steps
-// (load, MMA, registers, MMA, ...), so two blocks share an SM and fill each other's waits: 256 of the
-// 512 columns of tensor memory each (P in place of P0, L in the half of P0 that P leaves), and at most
-// 113 KB of shared memory (two planes of w c in place of a, which O2 is done with).
+// Warp 8 loads the tiles and issues the MMAs; warps 0 to 7 do everything in registers, two threads
+// to a row. A chunk is a chain of dependent steps, so the chain is cut where it can be (w c is formed
+// while a b^T runs, L runs while P is formed, the outputs are written while the next tiles come), and two
+// blocks share an SM: 256 of the 512 columns of tensor memory each, and at most 113 KB of shared memory
+// (planes of w c in place of a, which P0 and O are done with).
 #include <type_traits>
 
 #include "gemm_sm100.cuh"
@@ -40,11 +48,13 @@ using umma::pack_bf16;
 using umma::smem_desc;
 using umma::tmem_ld32;
 
-constexpr int kC = 128, kDS = 64, kThreads = 256;
+constexpr int kC = 128, kDS = 64;
+constexpr int kWorkers = 256, kThreads = kWorkers + 32;
 constexpr int kBlock = kC * 128;  // 128 rows of 64 bf16, 128-byte swizzle
-constexpr uint32_t kCols = 256;   // tensor memory: P0 / P | L, O1, O2
+constexpr uint32_t kCols = 256;   // tensor memory: P0 (P in the first quarter of each half), L, O
+constexpr uint32_t kLCol = 128, kOCol = 192;
 constexpr int kErrAlignment = 15;
-constexpr uint32_t kLCol = 64, kO1Col = 128, kO2Col = 192;
+constexpr float kWeakDecay = -0.23f;
 
 template <int DA>
 struct Cfg {
@@ -53,7 +63,7 @@ struct Cfg {
   static constexpr int kP2 = kS + DA * 128;  // planes that do not fit into a's buffer
   static constexpr int kPlanes = kP2 + (3 - kNA) * kBlock;
   static constexpr int kBar = kPlanes;
-  static constexpr int kBytes = kBar + 64 + 4 * (kC + 4) + 16 + kC + 16;
+  static constexpr int kBytes = kBar + 80 + 4 * (kC + 4) + 16 + 32;
   __device__ static int plane(int k) { return k < kNA ? kA + k * kBlock : kP2 + (k - kNA) * kBlock; }
 };
 static_assert(2 * (Cfg<128>::kBytes + 1024) <= 228 * 1024, "two blocks on an SM");
@@ -105,10 +115,34 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  return (uint64_t)__float_as_uint(hi) << 32 | __float_as_uint(lo);
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t sub2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// The bits lo .. hi of a word (positions outside 0 .. 31 allowed).
+__device__ __forceinline__ unsigned bits(int lo, int hi) {
+  const unsigned from = lo <= 0 ? ~0u : lo > 31 ? 0u : ~0u << lo;
+  const unsigned to = hi < 0 ? 0u : hi >= 31 ? ~0u : ~0u >> (31 - hi);
+  return from & to;
+}
+
 template <bool A_MN, bool B_MN, int N>
 __device__ __forceinline__ constexpr uint32_t idesc() {
   return umma::instr_desc<N, A_MN, B_MN>();
 }
+
+// The eight worker warps (named barrier 1).
+__device__ __forceinline__ void sync_workers() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // kOut: outputs, from the state that enters the split; else the split's own sum.
 template <int DA, bool kOut>
@@ -117,15 +151,17 @@ __global__ void __launch_bounds__(kThreads, 2)
   using F = Cfg<DA>;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F::kBar);
-  uint64_t *full = bars, *bar_p = bars + 1, *bar_a = bars + 2, *bar_o = bars + 3, *bar_l = bars + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 5);
-  float* pw = reinterpret_cast<float*>(smem + F::kBar + 64);  // e^{i g}
+  // full: tiles loaded; done_a: P0 and a S computed; done_l, done_o: L, O computed; has_w, has_p,
+  // has_s: the workers' planes, P and state (and tensor memory read) are in place
+  uint64_t *full = bars, *done_a = bars + 1, *done_l = bars + 2, *done_o = bars + 3, *has_w = bars + 4,
+           *has_p = bars + 5, *has_s = bars + 6;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 7);
+  volatile int* s_fail = reinterpret_cast<int*>(bars + 8);
+  float* pw = reinterpret_cast<float*>(smem + F::kBar + 80);  // e^{i g}
   float* pl = pw + kC + 4;  // what the rounding left of e^{i g}, i = 127, 128, n and n - 1 of the last chunk
-  uint8_t* seg = reinterpret_cast<uint8_t*>(pl + 4);  // cuts up to and with a position
-  unsigned* s_cut = reinterpret_cast<unsigned*>(seg + kC);
+  unsigned* s_cut = reinterpret_cast<unsigned*>(pl + 4);  // [2][4] the cuts of a chunk, a bit a position
 
   const Op& o = ops.op[blockIdx.z];
-  const CUtensorMap *ma = &maps.a[blockIdx.z], *mb = &maps.b[blockIdx.z], *mc = &maps.c[blockIdx.z];
   const int slices = ceil_div(o.Dc, kDS);
   if ((int)blockIdx.x >= o.batch * o.heads * slices) return;
   if (smem_u32(smem) & 1023) {  // the swizzled tiles count on it
@@ -137,34 +173,60 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int split = blockIdx.y;
   const int begin = split * o.split_len, end = min(o.steps, begin + o.split_len);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int row = (warp & 3) * 32 + lane, half = warp >> 2;  // tensor memory lane, column half
-  const float g = fmaxf(o.log_decay[head], kMinLogDecay);
-  const size_t elems = (size_t)o.Da * o.Dc;
   const int na = min(F::kNA, ceil_div(o.Da, 64));
+  const uint32_t base = smem_u32(smem);
 
-  if (tid == 0) {
-    mbar_init(full, 1);
-    mbar_init(bar_p, 1);
-    mbar_init(bar_a, 1);
-    mbar_init(bar_o, 1);
-    mbar_init(bar_l, 1);
-    fence_mbar_init();
+  auto load = [&](int i0) {
+    const int t0 = o.reverse ? o.steps - i0 - kC : i0;
+    mbar_arrive_expect_tx(full, ((kOut ? 2 : 1) * na + 1) * kBlock);
+    tma_load_4d(smem + F::kCc, &maps.c[blockIdx.z], d0, t0, head, batch, full);
+    for (int x = 0; x < na; ++x) {
+      if (kOut) tma_load_4d(smem + F::kA + x * kBlock, &maps.a[blockIdx.z], 64 * x, t0, head, batch, full);
+      tma_load_4d(smem + F::kB + x * kBlock, &maps.b[blockIdx.z], 64 * x, t0, head, batch, full);
+    }
+  };
+  if (warp == 8) {
+    if (lane == 0) {
+      *s_fail = 0;
+      for (int i = 0; i < 4; ++i) mbar_init(bars + i, 1);
+      for (int i = 4; i < 7; ++i) mbar_init(bars + i, kWorkers / 32);
+      fence_mbar_init();
+      if (begin < end) load(begin);
+    }
+    __syncwarp();
+    umma::tmem_alloc(tmem_slot, kCols);
   }
-  if (warp == 0) umma::tmem_alloc(tmem_slot, kCols);
+  const float g = fmaxf(o.log_decay[head], kMinLogDecay);
+  const bool weak = g >= kWeakDecay;
   if (tid <= kC) pw[tid] = (float)exp((double)tid * (double)g);
-  if (tid >= 252) {
+  if (tid >= kWorkers && tid < kWorkers + 4) {
     const int last = max(1, end - begin) - (max(1, end - begin) - 1) / kC * kC;
-    const int i = tid == 252 ? kC - 1 : tid == 253 ? kC : tid == 254 ? last : last - 1;
-    const double e = exp((double)i * (double)g);
-    pl[tid - 252] = (float)(e - (double)(float)e);
+    const int x = tid - kWorkers;
+    const double e = exp((double)(x == 0 ? kC - 1 : x == 1 ? kC : x == 2 ? last : last - 1) * (double)g);
+    pl[x] = (float)(e - (double)(float)e);
   }
-  // This thread's piece of the state: row k, columns y0 .. (the rows of L repeat where Da <= 64, and
-  // the second copy takes the other half of the columns).
+
+  const int row = (warp & 3) * 32 + lane, half = warp >> 2;  // tensor memory lane, column half
+  const size_t elems = (size_t)o.Da * o.Dc;
+  // A worker's piece of the state: row k, columns y0 .. (the rows of L repeat where Da <= 64, and the
+  // second copy takes the other half of the columns).
   constexpr int kSC = DA == 128 ? 32 : 16;
   const int k = DA == 128 ? row : row & 63;
   const int y0 = DA == 128 ? half * 32 : (row >> 6) * 32 + half * 16;
   float s[kSC];
-  {
+  auto put_state = [&]() {
+#pragma unroll
+    for (int i = 0; i < kSC; i += 8) {
+      uint32_t w[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) w[u] = pack_bf16(s[i + 2 * u], s[i + 2 * u + 1]);
+      *reinterpret_cast<uint4*>(smem + F::kS + k * 128 + ((((y0 + i) >> 3) ^ (k & 7)) << 4)) =
+          make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  };
+  bool cut = false;  // of position tid of the coming chunk
+  if (warp < 8) {
+    if (tid < kC && begin + tid < end) cut = op_cut(o, batch, begin + tid);
     const float* from = nullptr;
     int64_t sx = o.sx, sy = o.sy;
     if (kOut) {
@@ -176,260 +238,276 @@ __global__ void __launch_bounds__(kThreads, 2)
         from = o.init + bh * elems;
       }
     }
+    const bool whole = from && sy == 1 && o.Dc % 4 == 0 && ((uintptr_t)from & 15) == 0;
 #pragma unroll
-    for (int i = 0; i < kSC; ++i)
-      s[i] = from && k < o.Da && d0 + y0 + i < o.Dc ? from[k * sx + (d0 + y0 + i) * sy] : 0.f;
-  }
-  auto put_state = [&]() {
+    for (int i = 0; i < kSC; i += 4) {
+      const int y = d0 + y0 + i;
+      if (whole) {
+        const float4 f = k < o.Da && y < o.Dc ? *reinterpret_cast<const float4*>(from + k * sx + y)
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+        s[i] = f.x, s[i + 1] = f.y, s[i + 2] = f.z, s[i + 3] = f.w;
+      } else {
 #pragma unroll
-    for (int i = 0; i < kSC; i += 8) {
-      uint32_t w[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) w[u] = pack_bf16(s[i + 2 * u], s[i + 2 * u + 1]);
-      *reinterpret_cast<uint4*>(smem + F::kS + k * 128 + ((((y0 + i) >> 3) ^ (k & 7)) << 4)) =
-          make_uint4(w[0], w[1], w[2], w[3]);
+        for (int u = 0; u < 4; ++u)
+          s[i + u] = from && k < o.Da && y + u < o.Dc ? from[k * sx + (y + u) * sy] : 0.f;
+      }
     }
-  };
-  if (kOut) put_state();
+    if (kOut && !weak) put_state();
+  }
   fence_proxy_async_smem();
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-  const uint32_t base = smem_u32(smem);
-
-  auto load = [&](int i0) {
-    const int t0 = o.reverse ? o.steps - i0 - kC : i0;
-    mbar_arrive_expect_tx(full, ((kOut ? 2 : 1) * na + 1) * kBlock);
-    for (int x = 0; x < na; ++x) {
-      if (kOut) tma_load_4d(smem + F::kA + x * kBlock, ma, 64 * x, t0, head, batch, full);
-      tma_load_4d(smem + F::kB + x * kBlock, mb, 64 * x, t0, head, batch, full);
-    }
-    tma_load_4d(smem + F::kCc, mc, d0, t0, head, batch, full);
+  // A wait that gives up is recorded, and no wait after it is taken: the block runs to its end.
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (*s_fail) return;
+    if (!mbar_wait_bounded(bar, parity)) *s_fail = 1;
+    fence_after_sync();
   };
-  bool ok = true;
-  bool loading = false;
-  if (tid == 0 && begin < end) {
-    load(begin);
-    loading = true;
-  }
-  bool any_cut = false;
-  int e0 = (o.reverse && split == 0) ? 0 : 1;
-  uint32_t parity = 0;
-  const int p = o.reverse ? kC - 1 - row : row;  // the position of this thread's row
 
-  for (int i0 = begin; i0 < end; i0 += kC, parity ^= 1) {
-    const int n = min(kC, end - i0);
-    // the cuts of the chunk's positions
-    if (o.reset) {
-      if (tid < kC) {
-        const unsigned m = __ballot_sync(~0u, tid < n && op_cut(o, batch, i0 + tid));
-        if (lane == 0) s_cut[warp] = m;
-      }
-      __syncthreads();
-      if (tid < kC) {
-        int c = __popc(s_cut[warp] & (~0u >> (31 - lane)));
-        for (int w = 0; w < warp; ++w) c += __popc(s_cut[w]);
-        seg[tid] = (uint8_t)c;
-      }
-      __syncthreads();
-    }
-    const int seg_end = o.reset ? seg[kC - 1] : 0;
-    const int seg_p = o.reset ? seg[p] : 0;
-    any_cut |= seg_end > 0;
-
-    ok &= mbar_wait_bounded(full, parity);
-    if (tid == 0) loading = false;
-    if (kOut) {
-      if (tid == 0) {
-        fence_after_sync();
+  if (warp == 8) {
+    if (lane == 0) {
+      uint32_t parity = 0;
+      for (int i0 = begin; i0 < end; i0 += kC, parity ^= 1) {
+        wait(full, parity);
+        if (kOut) {
+          wait(has_s, parity);
+          if (*s_fail) break;
 #pragma unroll
-        for (int x = 0; x < DA / 16; ++x) {
-          if (x >= na * 4) break;
-          const uint32_t off = (x >> 2) * kBlock + (x & 3) * 32;
-          mma_bf16(tmem, smem_desc(base + F::kA + off, 16, 1024), smem_desc(base + F::kB + off, 16, 1024),
-                   idesc<false, false, 128>(), x > 0);
-        }
-        mma_commit(bar_p);
-#pragma unroll
-        for (int x = 0; x < DA / 16; ++x) {
-          if (x >= na * 4) break;
-          const uint32_t off = (x >> 2) * kBlock + (x & 3) * 32;
-          mma_bf16(tmem + kO2Col, smem_desc(base + F::kA + off, 16, 1024),
-                   smem_desc(base + F::kS + x * 2048, 8192, 1024), idesc<false, true, 64>(), x > 0);
-        }
-        mma_commit(bar_a);
-      }
-      ok &= mbar_wait_bounded(bar_p, parity);
-      fence_after_sync();
-      // P: this warp's 32 rows against the column blocks 2 half and 2 half + 1
-      uint32_t pk[2][16];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int blk = 2 * half + u, wr = warp & 3;
-        const bool past = o.reverse ? blk < wr : blk > wr;  // every position of it comes later
-        if (past) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pk[u][i] = 0;
-          continue;
-        }
-        float v[32];
-        tmem_ld32(lanes + 32 * blk, v);
-        const int gap0 = o.reverse ? 32 * blk - row : row - 32 * blk;  // p_i - p_j of column 0
-        const int dir = o.reverse ? 1 : -1;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int gap = gap0 + dir * i;
-          v[i] = gap >= 0 ? v[i] * pw[gap >= 0 ? gap : 0] : 0.f;
-        }
-        if (seg_end > 0) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int c = 32 * blk + i;
-            if (seg[o.reverse ? kC - 1 - c : c] != seg_p) v[i] = 0.f;
+          for (int x = 0; x < DA / 16; ++x) {
+            if (x >= na * 4) break;
+            const uint32_t off = (x >> 2) * kBlock + (x & 3) * 32;
+            mma_bf16(tmem, smem_desc(base + F::kA + off, 16, 1024), smem_desc(base + F::kB + off, 16, 1024),
+                     idesc<false, false, 128>(), x > 0);
           }
+#pragma unroll
+          for (int x = 0; x < DA / 16; ++x) {
+            if (x >= na * 4) break;
+            const uint32_t off = (x >> 2) * kBlock + (x & 3) * 32;
+            mma_bf16(tmem + kOCol, smem_desc(base + F::kA + off, 16, 1024),
+                     smem_desc(base + F::kS + x * 2048, 8192, 1024), idesc<false, true, 64>(), x > 0);
+          }
+          mma_commit(done_a);
         }
+        wait(has_w, parity);
+        if (*s_fail) break;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) pk[u][i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-      }
-      fence_before_sync();
-      __syncthreads();  // P0 is read everywhere before P replaces it
-      fence_after_sync();
-      tmem_st16(lanes + 32 * half, pk[0]);
-      tmem_st16(lanes + 32 * half + 16, pk[1]);
-      tmem_wait_st();
-      fence_before_sync();
-      __syncthreads();
-      if (tid == 0) {
-        fence_after_sync();
+        for (int q = 2; q >= 0; --q)  // smallest first
 #pragma unroll
-        for (int x = 0; x < kC / 16; ++x)
-          mma_bf16_ts(tmem + kO1Col, tmem + x * 8, smem_desc(base + F::kCc + x * 2048, 8192, 1024),
-                      idesc<false, true, 64>(), x > 0);
-        mma_commit(bar_o);
+          for (int x = 0; x < kC / 16; ++x)
+            // the second 64 rows of a 64-wide b are its first ones again
+            mma_bf16(tmem + kLCol, smem_desc(base + F::kB + x * 2048, na == 2 ? kBlock : 0, 1024),
+                     smem_desc(base + F::plane(q) + x * 2048, 8192, 1024), idesc<true, true, 64>(), q < 2 || x > 0);
+        mma_commit(done_l);
+        if (kOut) {
+          wait(has_p, parity);
+          if (*s_fail) break;
+          for (int q = weak ? 1 : 0; q >= 0; --q) {
+            const uint32_t b = base + (weak ? F::plane(q) : F::kCc);
+#pragma unroll
+            for (int x = 0; x < kC / 16; ++x)
+              mma_bf16_ts(tmem + kOCol, tmem + (x >> 2) * 64 + (x & 3) * 8, smem_desc(b + x * 2048, 8192, 1024), idesc<false, true, 64>(), 1);
+          }
+          mma_commit(done_o);
+          wait(done_o, parity);
+        }
+        wait(done_l, parity);
+        if (*s_fail) break;
+        if (i0 + kC < end) load(i0 + kC);
       }
-      ok &= mbar_wait_bounded(bar_a, parity);  // O2 has read a: its buffer takes planes
+      if (*s_fail) {
+        // let copies and MMAs in flight end before the block's memory goes
+        mbar_wait_bounded(full, parity);
+        mbar_wait_bounded(done_a, parity);
+        mbar_wait_bounded(done_l, parity);
+        mbar_wait_bounded(done_o, parity);
+      }
     }
-    {  // w c: this thread's row, half of the columns
-      const bool in = p < n && seg_p == seg_end;
-      const float w = in ? pw[n - 1 - p] : 0.f;
+  } else {
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int p = o.reverse ? kC - 1 - row : row;  // the position of this thread's row
+    const float in_scale = o.in_scale;
+    const bool reverse = o.reverse, resets = o.reset != nullptr;
+    bool any_cut = false;
+    int e0 = (reverse && split == 0) ? 0 : 1;
+    uint32_t parity = 0;
+    auto arrive = [&](uint64_t* bar) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    // s takes its decay over the n positions to come, and its copy goes where O's product reads it. The
+    // factor in two parts: its rounding, met once a chunk, would add up over a long memory.
+    auto hand_state = [&](int n) {
+      if (kOut && !weak) put_state();
+      const float keep = pw[n - 1 + e0], keep_lo = pl[n == kC ? e0 : 3 - e0];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int off = row * 128 + (((half * 4 + u) ^ (row & 7)) << 4);
-        const uint4 x = *reinterpret_cast<const uint4*>(smem + F::kCc + off);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&xs[i]);
-          v[2 * i] = in ? w * __low2float(h) : 0.f;
-          v[2 * i + 1] = in ? w * __high2float(h) : 0.f;
+      for (int i = 0; i < kSC; ++i) s[i] = fmaf(keep, s[i], keep_lo * s[i]);
+      if (kOut && weak) put_state();
+      fence_proxy_async_smem();
+    };
+    if (begin < end) hand_state(min(kC, end - begin));
+    if (kOut) arrive(has_s);
+
+    for (int i0 = begin; i0 < end; i0 += kC, parity ^= 1) {
+      const int n = min(kC, end - i0);
+      // the last cut of the chunk, and the last one at or before p (-1: none)
+      int last = -1, lo = -1;
+      if (resets) {
+        unsigned* cuts = s_cut + 4 * parity;
+        if (tid < kC) {
+          const unsigned m = __ballot_sync(~0u, cut);
+          if (lane == 0) cuts[warp] = m;
+          cut = i0 + kC + tid < end && op_cut(o, batch, i0 + kC + tid);
         }
+        sync_workers();
 #pragma unroll
-        for (int q = 0; q < 3; ++q) {
-          uint32_t y[4];
+        for (int w = 0; w < 4; ++w) {
+          const unsigned m = cuts[w], own = m & bits(0, p - 32 * w);
+          if (m) last = 32 * w + 31 - __clz(m);
+          if (own) lo = 32 * w + 31 - __clz(own);
+        }
+        any_cut |= last >= 0;
+      }
+
+      wait(full, parity);
+      {  // w c: this thread's row, half of the columns; the planes that go into a's place wait for it
+        const float wf = p < n ? in_scale * pw[n - 1 - p] : 0.f;
+        const uint64_t w = pair(wf, wf);
+        uint4 held[F::kNA][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int off = row * 128 + (((half * 4 + u) ^ (row & 7)) << 4);
+          const uint4 x = *reinterpret_cast<const uint4*>(smem + F::kCc + off);
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+          uint32_t y[3][4];
+          // 24 bits cut into 8 + 8 + 8: each plane takes the leading bits, the rest is exact
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            y[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-            const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&y[i]);
-            v[2 * i] -= __low2float(h);
-            v[2 * i + 1] -= __high2float(h);
+            uint64_t v = mul2(w, (uint64_t)(xs[i] & 0xffff0000u) << 32 | (xs[i] << 16));
+#pragma unroll
+            for (int q = 0; q < 3; ++q) {
+              y[q][i] = __byte_perm((uint32_t)v, (uint32_t)(v >> 32), 0x7632);
+              if (q < 2) v = sub2(v, v & 0xffff0000ffff0000ull);
+            }
           }
-          *reinterpret_cast<uint4*>(smem + F::plane(q) + off) = make_uint4(y[0], y[1], y[2], y[3]);
+#pragma unroll
+          for (int q = 0; q < 3; ++q) {
+            const uint4 z = make_uint4(y[q][0], y[q][1], y[q][2], y[q][3]);
+            if (q < F::kNA) held[q < F::kNA ? q : 0][u] = z;
+            else *reinterpret_cast<uint4*>(smem + F::plane(q) + off) = z;
+          }
+        }
+        if (kOut) wait(done_a, parity);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int off = row * 128 + (((half * 4 + u) ^ (row & 7)) << 4);
+#pragma unroll
+          for (int q = 0; q < F::kNA; ++q) *reinterpret_cast<uint4*>(smem + F::plane(q) + off) = held[q][u];
+        }
+        if (last > p) {  // what a cut hides has no part in L; P0 is done with its row of b
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int x = 0; x < F::kNA; ++x)
+              *reinterpret_cast<uint4*>(smem + F::kB + x * kBlock + row * 128 + (half * 4 + u) * 16) =
+                  make_uint4(0, 0, 0, 0);
         }
       }
-    }
-    fence_proxy_async_smem();
-    __syncthreads();
-    if (tid == 0) {
-      fence_after_sync();
-      bool acc = false;
+      fence_proxy_async_smem();
+      fence_before_sync();
+      arrive(has_w);
+      if (kOut) {
+        if (!weak || last >= 0) {
+          // the rows of a S by the decay since the state; a cut drops it whatever it holds
+          const float reach = lo >= 0 || p >= n ? 0.f : weak ? 1.f : pw[p + e0];
+          float v[32];
+          tmem_ld32(lanes + kOCol + 32 * half, v);
 #pragma unroll
-      for (int q = 2; q >= 0; --q)  // smallest first
+          for (int j = 0; j < 2; ++j) {
+            uint32_t w[16];
 #pragma unroll
-        for (int x = 0; x < kC / 16; ++x) {
-          // the second 64 rows of a 64-wide b are its first ones again
-          mma_bf16(tmem + kLCol, smem_desc(base + F::kB + x * 2048, na == 2 ? kBlock : 0, 1024),
-                   smem_desc(base + F::plane(q) + x * 2048, 8192, 1024), idesc<true, true, 64>(), acc);
-          acc = true;
+            for (int i = 0; i < 16; ++i) w[i] = reach != 0.f ? __float_as_uint(reach * v[16 * j + i]) : 0u;
+            tmem_st16(lanes + kOCol + 32 * half + 16 * j, w);
+          }
         }
-      mma_commit(bar_l);
-    }
-    if (kOut) {
-      ok &= mbar_wait_bounded(bar_o, parity);
-      fence_after_sync();
-      float o1[32], o2[32];
-      tmem_ld32(lanes + kO1Col + 32 * half, o1);
-      tmem_ld32(lanes + kO2Col + 32 * half, o2);
-      if (p < n) {
-        const float reach = seg_p == 0 ? pw[p + e0] * o.out_scale : 0.f;
-        const float own = o.in_scale * o.out_scale;
-        const int t = o.reverse ? o.steps - 1 - i0 - p : i0 + p;
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(o.out) + batch * o.out_batch +
-                             (int64_t)t * o.out_step + head * o.out_head + d0 + 32 * half;
-        // a cut drops the state whatever it holds, not 0 times it
+        // P: this warp's 32 rows against the column blocks 2 half and 2 half + 1. It takes the place of
+        // the first of the two, which is read by then.
+        const int from = max(lo, 0);  // columns of positions from .. p count
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o1[i] = reach != 0.f ? own * o1[i] + reach * o2[i] : own * o1[i];
-        const int left = o.Dc - d0 - 32 * half;
+        for (int u = 0; u < 2; ++u) {
+          const int blk = 2 * half + u;
+          const unsigned m = reverse ? bits(kC - 1 - 32 * blk - p, kC - 1 - 32 * blk - from)
+                                     : bits(from - 32 * blk, p - 32 * blk);
+          uint32_t pk[16];
+          if (__all_sync(~0u, m == 0)) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          if (i + 8 <= left) {
-            *reinterpret_cast<uint4*>(out + i) =
-                make_uint4(pack_bf16(o1[i], o1[i + 1]), pack_bf16(o1[i + 2], o1[i + 3]),
-                           pack_bf16(o1[i + 4], o1[i + 5]), pack_bf16(o1[i + 6], o1[i + 7]));
+            for (int i = 0; i < 16; ++i) pk[i] = 0;
           } else {
+            float v[32];
+            tmem_ld32(lanes + 32 * blk, v);
+            if (!weak) {
+              // e^{(p_i - p_j) g}: only where the column comes no later than the row
+              const int gap0 = reverse ? 32 * blk - row : row - 32 * blk, dir = reverse ? 1 : -1;
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-              if (i + u < left) out[i + u] = __float2bfloat16_rn(o1[i + u]);
+              for (int i = 0; i < 32; ++i) v[i] *= in_scale * pw[max(0, gap0 + dir * i)];
+            }
+            if (!__all_sync(~0u, m == ~0u)) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = m >> i & 1 ? v[i] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pk[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
           }
+          tmem_st16(lanes + 64 * half + 16 * u, pk);
         }
+        tmem_wait_st();
+        fence_before_sync();
+        arrive(has_p);
       }
-    }
-    ok &= mbar_wait_bounded(bar_l, parity);
-    fence_after_sync();
-    if (tid == 0 && ok && i0 + kC < end) {
-      load(i0 + kC);
-      loading = true;
-    }
-    {
-      // the factor in two parts: its rounding, met once a chunk, would add up over a long memory
-      const float keep = pw[n - 1 + e0], keep_lo = pl[n == kC ? e0 : 3 - e0];
-      float l[kSC];
-      if constexpr (kSC == 32) tmem_ld32(lanes + kLCol + y0, l);
-      else tmem_ld16(lanes + kLCol + y0, l);
+      wait(done_l, parity);
+      {
+        float l[kSC];
+        if constexpr (kSC == 32) tmem_ld32(lanes + kLCol + y0, l);
+        else tmem_ld16(lanes + kLCol + y0, l);
 #pragma unroll
-      for (int i = 0; i < kSC; ++i) {
-        const float old = seg_end == 0 ? fmaf(keep, s[i], keep_lo * s[i]) : 0.f;
-        s[i] = old + o.in_scale * l[i];
+        for (int i = 0; i < kSC; ++i) s[i] = (last < 0 ? s[i] : 0.f) + l[i];
+      }
+      e0 = 1;
+      if (i0 + kC < end) hand_state(min(kC, end - i0 - kC));
+      if (kOut) {
+        wait(done_o, parity);
+        float v[32];
+        tmem_ld32(lanes + kOCol + 32 * half, v);
+        fence_before_sync();
+        arrive(has_s);
+        if (p < n) {
+          const int t = reverse ? o.steps - 1 - i0 - p : i0 + p;
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(o.out) + batch * o.out_batch +
+                               (int64_t)t * o.out_step + head * o.out_head + d0 + 32 * half;
+          const int left = o.Dc - d0 - 32 * half;
+          const float f = weak ? o.out_scale / pw[n - 1 - p] : o.out_scale;
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            // Dc is a multiple of 8, as the rows' strides are
+            if (i < left)
+              *reinterpret_cast<uint4*>(out + i) =
+                  make_uint4(pack_bf16(f * v[i], f * v[i + 1]), pack_bf16(f * v[i + 2], f * v[i + 3]),
+                             pack_bf16(f * v[i + 4], f * v[i + 5]), pack_bf16(f * v[i + 6], f * v[i + 7]));
+        }
+      } else {
+        fence_before_sync();
       }
     }
-    if (kOut) put_state();
-    e0 = 1;
-    fence_proxy_async_smem();
-    fence_before_sync();
-    if (__syncthreads_or(!ok)) {
-      ok = false;
-      break;
-    }
-    fence_after_sync();
-  }
-  if (!ok && tid == 0) {
-    // let the copies and MMAs in flight end before the block's memory goes
-    if (loading) mbar_wait_bounded(full, parity ^ 1);
-    mbar_wait_bounded(bar_l, parity);
-    atomicExch(err, umma::kErrTimeoutFull);
-  }
-  {
     float* to = nullptr;
     int64_t sx = o.sx, sy = o.sy;
-    float last = 1.f;
+    float way_out = 1.f;
     if (kOut) {
       if (o.fin && split == o.nsplit - 1) {
         to = o.fin + bh * elems;
         if (o.reverse && o.steps > 0) {
-          last = pw[1];
-          if (o.reset && o.reset[batch * o.reset_batch]) last = 0.f;
+          way_out = pw[1];
+          if (o.reset && o.reset[batch * o.reset_batch]) way_out = 0.f;
         }
       }
     } else {
@@ -439,16 +517,29 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (tid == 0 && d0 == 0 && head == 0) o.cut[split * o.batch + batch] = any_cut;
     }
     if (to && k < o.Da) {
+      const bool whole = sy == 1 && o.Dc % 4 == 0 && ((uintptr_t)to & 15) == 0;
 #pragma unroll
-      for (int i = 0; i < kSC; ++i)
-        if (d0 + y0 + i < o.Dc) to[k * sx + (d0 + y0 + i) * sy] = last == 0.f ? 0.f : last * s[i];
+      for (int i = 0; i < kSC; i += 4) {
+        const int y = d0 + y0 + i;
+        float f[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) f[u] = way_out == 0.f ? 0.f : way_out * s[i + u];
+        if (whole) {
+          if (y < o.Dc) *reinterpret_cast<float4*>(to + k * sx + y) = make_float4(f[0], f[1], f[2], f[3]);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (y + u < o.Dc) to[k * sx + (y + u) * sy] = f[u];
+        }
+      }
     }
   }
   fence_before_sync();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == 8) {
     fence_after_sync();
     umma::tmem_dealloc(tmem, kCols);
+    if (lane == 0 && *s_fail) atomicExch(err, umma::kErrTimeoutFull);
   }
 }
 
