@@ -224,3 +224,27 @@ def lib() -> C.CDLL:
 def check(code: int) -> None:
     if code != BT_OK:
         raise BoontaError(code, lib().bt_last_error().decode(errors="replace"))
+
+
+class on_device:
+    """Makes a CUDA device (its index) the current one for a call, and gives its current stream's
+    handle; nothing is switched where it is current already."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self) -> int:
+        import torch
+
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch._C._cuda_setDevice(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            import torch
+
+            torch._C._cuda_setDevice(self.before)

@@ -9,11 +9,12 @@
 //
 // Bound by HBM: forward 2, backward 3 elements per element of x. A block takes a few tokens: it
 // forms their cosines and sines once in shared memory (angle in 64 bits, reduced to one turn
-// before the 32-bit sine, so far positions keep their phase), then a group of lanes takes one row
-// (a token's query or key head) with 16-byte loads; the partner of an element, half a rotation
-// away, comes through the group's row in shared memory. The weight gradients are summed per thread
-// over the block's rows, over the block's groups in shared memory, and over the blocks by a second
-// launch, each in a fixed order.
+// before the 32-bit sine, so far positions keep their phase). A group of lanes then walks rows (query
+// or key heads) of one token with 16-byte loads, its cosines and sines in registers, the next row on
+// its way while one is worked on; the partner of an element, half a rotation away, comes from another
+// lane. Where the rotated half does not fall on whole lanes, partners go through the group's row
+// in shared memory. The weight gradients are summed per thread over its rows, over the block's groups
+// in shared memory, and over the blocks by a second launch, each in a fixed order.
 #include <type_traits>
 
 #include "common.cuh"
@@ -23,7 +24,7 @@ namespace rot {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 8;  // tokens of a block's pass
+constexpr int kMaxTokens = 16;  // tokens of a block's pass
 constexpr int kMaxDim = 256;
 
 struct Rows {
@@ -81,58 +82,99 @@ __device__ __forceinline__ void store(T* p, const float (&v)[V]) {
   }
 }
 
-// x[c][i] holds feature (c * G + lane) * V + i of the row. Turns it by the token's angles (sign 1),
-// or back (-1); `row` is the group's staging row.
-template <int V, int NC>
-__device__ __forceinline__ void turn(const Args& a, float (&x)[NC][V], float* row, const float* cs,
-                                     float sign, int lane, int G, bool on) {
-  const int rd = 2 * a.half;
-  if (V > 1 && a.interleaved && (rd % V) == 0) {
+// Where a lane's elements find their angles and partners. x[c][i] holds feature (c * G + lane) * V + i.
+enum Pairing {
+  kLanes,     // (i, i + half), half a multiple of V, one chunk per lane: the partner is another lane's
+  kNeighbours,  // (2 i, 2 i + 1) and V even: the partner is the lane's own
+  kStaged     // anything else, through shared memory
+};
+
+template <int V>
+struct Turn {  // a lane's cosines and signed sines (kLanes: V, kNeighbours: V / 2)
+  float c[V], s[V];
+};
+
+template <Pairing kP, int V, int NC>
+__device__ __forceinline__ void load_turn(const Args& a, const float* cs, int lane, Turn<V>& t) {
+  if constexpr (kP == kStaged) return;
+  const int d = lane * V;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int d = (c * G + lane) * V;
-      if (!on || d >= rd) continue;
+  for (int i = 0; i < V; ++i) t.c[i] = 1.f, t.s[i] = 0.f;
+  if (d >= 2 * a.half) return;
+  if constexpr (kP == kLanes) {
+    const bool second = d >= a.half;
+    const int pair = second ? d - a.half : d;
 #pragma unroll
-      for (int i = 0; i + 1 < V; i += 2) {
-        const float co = cs[(d + i) >> 1], si = sign * cs[a.half + ((d + i) >> 1)];
-        const float p = x[c][i], q = x[c][i + 1];
-        x[c][i] = p * co - q * si;
-        x[c][i + 1] = q * co + p * si;
+    for (int i = 0; i < V; ++i) {
+      t.c[i] = cs[pair + i];
+      t.s[i] = second ? cs[a.half + pair + i] : -cs[a.half + pair + i];
+    }
+  } else if constexpr (kP == kNeighbours) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i)
+      if (d / 2 + i < a.half) {
+        t.c[i] = cs[d / 2 + i];
+        t.s[i] = cs[a.half + d / 2 + i];
       }
-    }
-    return;
   }
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int d = (c * G + lane) * V + i;
-      if (d < rd) row[d] = x[c][i];
-    }
-  __syncwarp();
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int d = (c * G + lane) * V + i;
-      if (d >= rd) continue;
-      const int pair = a.interleaved ? d >> 1 : d % a.half;
-      const bool second = a.interleaved ? d & 1 : d >= a.half;
-      const float other = row[a.interleaved ? d ^ 1 : (second ? d - a.half : d + a.half)];
-      const float co = cs[pair], si = sign * cs[a.half + pair];
-      x[c][i] = second ? x[c][i] * co + other * si : x[c][i] * co - other * si;
-    }
-  __syncwarp();
 }
 
-template <class T, class W, int V, int NC, bool kBack>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ Args a, int G) {
-  extern __shared__ float sm[];
+// Turns x by the token's angles (sign 1), or back (-1).
+template <Pairing kP, int V, int NC>
+__device__ __forceinline__ void turn(const Args& a, float (&x)[NC][V], const Turn<V>& t, float* row, const float* cs,
+                                     float sign, int lane, int G, unsigned mask) {
+  if constexpr (kP == kLanes) {
+    const int h = a.half / V;
+    const int from = lane < h ? lane + h : lane < 2 * h ? lane - h : lane;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float other = __shfl_sync(mask, x[0][i], from, G);
+      x[0][i] = x[0][i] * t.c[i] + other * (sign * t.s[i]);
+    }
+  } else if constexpr (kP == kNeighbours) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const float p = x[0][2 * i], q = x[0][2 * i + 1], si = sign * t.s[i];
+      x[0][2 * i] = p * t.c[i] - q * si;
+      x[0][2 * i + 1] = q * t.c[i] + p * si;
+    }
+  } else {
+    const int rd = 2 * a.half;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int d = (c * G + lane) * V + i;
+        if (d < rd) row[d] = x[c][i];
+      }
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int d = (c * G + lane) * V + i;
+        if (d >= rd) continue;
+        const bool second = a.interleaved ? d & 1 : d >= a.half;
+        const int pair = a.interleaved ? d >> 1 : second ? d - a.half : d;
+        const float other = row[a.interleaved ? d ^ 1 : (second ? d - a.half : d + a.half)];
+        const float co = cs[pair], si = sign * cs[a.half + pair];
+        x[c][i] = second ? x[c][i] * co + other * si : x[c][i] * co - other * si;
+      }
+    __syncwarp();
+  }
+}
+
+// G lanes to a row; a token's rows go round `share` groups, and a block's pass takes a.per tokens.
+template <class T, class W, int V, int NC, Pairing kP, bool kBack>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ Args a, int G, int share) {
+  extern __shared__ __align__(16) float sm[];
   float* cs = sm;                                 // [per][2 half]
   float* rows = sm + a.per * 2 * a.half;          // [groups][D] staging rows
+  __shared__ int64_t s_off[kMaxTokens][6];        // element offsets of a token in q, k, yq, yk, gq, gk
   const int lane = threadIdx.x % G, group = threadIdx.x / G, groups = kThreads / G;
   float* row = rows + group * a.D;
   const unsigned mask = G == 32 ? ~0u : ((1u << G) - 1u) << ((threadIdx.x & 31) / G * G);
+  const int tok = group / share, first = group % share;
   float w[2][NC][V], dw[kBack ? 2 : 1][NC][V];
 #pragma unroll
   for (int c = 0; c < NC; ++c)
@@ -144,99 +186,111 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
       w[1][c][i] = in && a.wk ? to_float(static_cast<const W*>(a.wk)[d]) : 1.f;
       if (kBack) dw[0][c][i] = dw[kBack ? 1 : 0][c][i] = 0.f;
     }
-  const int H = a.hq + a.hk;
   const float inv = 1.f / (float)a.D;
   for (int64_t t0 = (int64_t)blockIdx.x * a.per; t0 < a.tokens; t0 += (int64_t)gridDim.x * a.per) {
     const int n = (int)min((int64_t)a.per, a.tokens - t0);
     __syncthreads();
+    if (threadIdx.x < n) {
+      const int64_t t = t0 + threadIdx.x, b = t / a.steps, st = t % a.steps;
+      int64_t* f = s_off[threadIdx.x];
+      f[0] = b * a.q.batch + st * a.q.step;
+      f[1] = b * a.k.batch + st * a.k.step;
+      f[2] = b * a.yq.batch + st * a.yq.step;
+      f[3] = b * a.yk.batch + st * a.yk.step;
+      f[4] = b * a.gq.batch + st * a.gq.step;
+      f[5] = b * a.gk.batch + st * a.gk.step;
+    }
     for (int e = threadIdx.x; e < n * a.half; e += kThreads) {
-      const int64_t t = t0 + e / a.half;
-      const double ang = (double)a.pos[t / a.steps * a.pos_batch + t % a.steps * a.pos_step] *
-                         a.freq[e % a.half];
-      // one turn: 2 pi as the sum of two doubles
-      const double k = rint(ang * 0.15915494309189535);
-      const double red = fma(-k, 2.4492935982947064e-16, fma(-k, 6.283185307179586, ang));
+      const int u = e / a.half, i = e - u * a.half;
+      const int64_t t = t0 + u, b = t / a.steps;
+      // in turns, so that the whole ones drop out exactly before the 32-bit functions
+      const double ang = (double)a.pos[b * a.pos_batch + (t - b * a.steps) * a.pos_step] * a.freq[i] * 0.15915494309189535;
       float s, c;
-      sincosf((float)red, &s, &c);
-      cs[e / a.half * 2 * a.half + e % a.half] = c;
-      cs[e / a.half * 2 * a.half + a.half + e % a.half] = s;
+      sincospif((float)(2.0 * (ang - rint(ang))), &s, &c);
+      cs[u * 2 * a.half + i] = c;
+      cs[u * 2 * a.half + a.half + i] = s;
     }
     __syncthreads();
-    // every group walks the same number of rows, so that its warp's shuffles meet
-    for (int r0 = 0; r0 < n * H; r0 += groups) {
-      const int r = r0 + group;
-      const bool on = r < n * H;
-      const int tok = on ? r / H : 0, h = on ? r % H : 0;
-      const int64_t t = t0 + tok, b = t / a.steps, st = t % a.steps;
-      const bool key = h >= a.hq;
-      const int hh = key ? h - a.hq : h;
-      const Rows& src = key ? a.k : a.q;
-      const T* xp = static_cast<const T*>(src.p) + b * src.batch + st * src.step + hh * src.head;
-      float x[NC][V], g[kBack ? NC : 1][V];
-      float ss = 0.f;
+    // groups without a token walk along: a warp's lanes stay together
+    const bool mine = tok < n;
+    const float* ct = cs + (mine ? tok : 0) * 2 * a.half;
+    Turn<V> tn;
+    load_turn<kP, V, NC>(a, ct, lane, tn);
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int d = (c * G + lane) * V;
-        if (on && d < a.D) {
-          load<T, V>(xp + d, x[c]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) x[c][i] = 0.f;
-        }
-      }
-      if constexpr (kBack) {
-        const Rows& gs = key ? a.gk : a.gq;
-        const T* gp = static_cast<const T*>(gs.p) + b * gs.batch + st * gs.step + hh * gs.head;
+    for (int which = 0; which < 2; ++which) {  // the queries, then the keys
+      const int H = which ? a.hk : a.hq;
+      const Rows &src = which ? a.k : a.q, &dst = which ? a.yk : a.yq, &gsrc = which ? a.gk : a.gq;
+      const int64_t* f = s_off[mine ? tok : 0];
+      const T* xp = static_cast<const T*>(src.p) + f[which];
+      T* yp = static_cast<T*>(dst.p) + f[2 + which];
+      const T* gp = static_cast<const T*>(gsrc.p) + f[4 + which];
+      float nx[NC][V], ng[kBack ? NC : 1][V];
+      auto fetch = [&](int h) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const int d = (c * G + lane) * V;
-          if (on && d < a.D) {
-            load<T, V>(gp + d, g[c]);
-          } else {
+          const bool in = mine && h < H && d < a.D;
 #pragma unroll
-            for (int i = 0; i < V; ++i) g[c][i] = 0.f;
+          for (int i = 0; i < V; ++i) {
+            nx[c][i] = 0.f;
+            if (kBack) ng[kBack ? c : 0][i] = 0.f;
+          }
+          if (in) {
+            load<T, V>(xp + h * src.head + d, nx[c]);
+            if constexpr (kBack) load<T, V>(gp + h * gsrc.head + d, ng[c]);
           }
         }
-      }
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int i = 0; i < V; ++i) ss += x[c][i] * x[c][i];
-      for (int o = G >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-      const float rs = rsqrtf(ss * inv + a.eps);
-      const float* ct = cs + tok * 2 * a.half;
-      if constexpr (!kBack) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int i = 0; i < V; ++i) x[c][i] *= rs * (key ? w[1][c][i] : w[0][c][i]);
-        turn<V, NC>(a, x, row, ct, 1.f, lane, G, on);
-      } else {
-        turn<V, NC>(a, g, row, ct, -1.f, lane, G, on);
-        float m = 0.f;
+      };
+      fetch(first);
+      for (int h0 = 0; h0 < H; h0 += share) {
+        const int h = h0 + first;
+        const bool on = mine && h < H;
+        float x[NC][V], g[kBack ? NC : 1][V];
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
           for (int i = 0; i < V; ++i) {
-            x[c][i] *= rs;
-            const float p = on ? g[c][i] * x[c][i] : 0.f;
-            if (key) dw[kBack ? 1 : 0][c][i] += p; else dw[0][c][i] += p;
-            g[c][i] *= key ? w[1][c][i] : w[0][c][i];
-            m += g[c][i] * x[c][i];
+            x[c][i] = nx[c][i];
+            if (kBack) g[kBack ? c : 0][i] = ng[kBack ? c : 0][i];
           }
-        for (int o = G >> 1; o > 0; o >>= 1) m += __shfl_xor_sync(mask, m, o);
-        m *= inv;
+        fetch(h + share);
+        float ss = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int i = 0; i < V; ++i) x[c][i] = rs * (g[c][i] - x[c][i] * m);
-      }
-      const Rows& dst = key ? a.yk : a.yq;
-      T* yp = static_cast<T*>(dst.p) + b * dst.batch + st * dst.step + hh * dst.head;
+          for (int i = 0; i < V; ++i) ss += x[c][i] * x[c][i];
+        for (int o = G >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+        const float rs = rsqrtf(ss * inv + a.eps);
+        if constexpr (!kBack) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int d = (c * G + lane) * V;
-        if (on && d < a.D) store<T, V>(yp + d, x[c]);
+          for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[c][i] *= rs * w[which][c][i];
+          turn<kP, V, NC>(a, x, tn, row, ct, 1.f, lane, G, mask);
+        } else {
+          turn<kP, V, NC>(a, g, tn, row, ct, -1.f, lane, G, mask);
+          float m = 0.f;
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              x[c][i] *= rs;
+              dw[kBack ? which : 0][c][i] += on ? g[c][i] * x[c][i] : 0.f;
+              g[c][i] *= w[which][c][i];
+              m += g[c][i] * x[c][i];
+            }
+          for (int o = G >> 1; o > 0; o >>= 1) m += __shfl_xor_sync(mask, m, o);
+          m *= inv;
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[c][i] = rs * (g[c][i] - x[c][i] * m);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const int d = (c * G + lane) * V;
+          if (on && d < a.D) store<T, V>(yp + h * dst.head + d, x[c]);
+        }
       }
     }
   }
@@ -262,40 +316,47 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
 }
 
 // dw[which][d] = sum over the blocks: one block per (which, 32 features), a warp's lanes on
-// neighbouring features, its eight warps on every eighth partial.
+// neighbouring features, its 32 warps on every 32nd partial.
 template <class W>
-__global__ void __launch_bounds__(256) weight_kernel(const float* partial, int blocks, int D, W* dwq, W* dwk) {
-  __shared__ double part[8][33];
+__global__ void __launch_bounds__(1024) weight_kernel(const float* partial, int blocks, int D, W* dwq, W* dwk) {
+  __shared__ double part[32][33];
   const int which = blockIdx.y, d = blockIdx.x * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
   double s = 0.0;
   if (d < D)
-    for (int b = warp; b < blocks; b += 8) s += (double)partial[((size_t)b * 2 + which) * D + d];
+#pragma unroll 4
+    for (int b = warp; b < blocks; b += 32) s += (double)partial[((size_t)b * 2 + which) * D + d];
   part[warp][threadIdx.x & 31] = s;
   __syncthreads();
   W* to = which ? dwk : dwq;
   if (warp == 0 && d < D && to) {
     double t = 0.0;
-    for (int u = 0; u < 8; ++u) t += part[u][threadIdx.x];
+#pragma unroll
+    for (int u = 0; u < 32; ++u) t += part[u][threadIdx.x];
     to[d] = from_float<W>((float)t);
   }
 }
 
-// Blocks of the backward: its partial sums have one row for each.
+// Blocks of the backward: its partial sums have one row for each. At most three an SM, which fit.
+constexpr int kMaxBlocks = 3 * kNumSMs;
 int backward_blocks(int64_t tokens, int per) {
   const int64_t n = ceil_div64(tokens, per);
-  return (int)(n < 4 * kNumSMs ? n : 4 * kNumSMs);
+  return (int)(n < kMaxBlocks ? n : kMaxBlocks);
 }
 
-int tokens_per_pass(int64_t tokens, int rows) {
-  // enough rows for every group of a block, but a block for every SM first
-  int per = 1;
-  while (per < kMaxTokens && per * rows < 64 && ceil_div64(tokens, per * 2) >= 2 * kNumSMs) per *= 2;
-  return per;
+// Lanes of a row, and the groups that share a token's rows: at most one for each row, fewer where
+// there are tokens enough to fill the GPU twice over with the rest.
+void shape_of(int64_t tokens, int rows, int chunks, int* G, int* share) {
+  *G = 1;
+  while (*G < 32 && *G < chunks) *G *= 2;
+  const int groups = kThreads / *G;
+  int s = max(1, groups / kMaxTokens);
+  while (s < groups && (s * 2 <= rows || s < 2) && ceil_div64(tokens * s, groups) < 2 * kNumSMs) s *= 2;
+  *share = min(s, groups);
 }
 
 struct Call {
   Args a;
-  int dtype, wdtype;
+  int dtype, wdtype, G, share;
   bool vec;
 };
 
@@ -303,26 +364,32 @@ template <class T, class W, bool kBack>
 int launch(const Call& c, int blocks, cudaStream_t s) {
   const Args& a = c.a;
   const int V = c.vec ? 16 / (int)sizeof(T) : 1;
-  const int chunks = ceil_div(a.D, V);
-  int G = 1;
-  while (G < 32 && G < chunks) G *= 2;
-  const int nc = ceil_div(chunks, G);
-  const size_t smem = ((size_t)a.per * 2 * a.half + (size_t)(kThreads / G) * a.D) * 4;
-  auto go = [&](auto vv, auto cc) -> int {
+  const int nc = ceil_div(ceil_div(a.D, V), c.G);
+  auto go = [&](auto vv, auto cc, auto pp) -> int {
     constexpr int VV = decltype(vv)::value, CC = decltype(cc)::value;
-    auto kernel = rotary_kernel<T, W, VV, CC, kBack>;
+    constexpr Pairing kP = decltype(pp)::value;
+    auto kernel = rotary_kernel<T, W, VV, CC, kP, kBack>;
+    const bool staged = kP == kStaged || kBack;
+    const size_t smem = ((size_t)a.per * 2 * a.half + (staged ? (size_t)(kThreads / c.G) * a.D : 0)) * 4;
     if (smem > 48 * 1024)
       BT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kernel<<<blocks, kThreads, smem, s>>>(a, G);
+    kernel<<<blocks, kThreads, smem, s>>>(a, c.G, c.share);
     BT_LAUNCH_CHECK("query/key norms with rotation");
     return BT_OK;
   };
-  if (c.vec) {
-    constexpr int VT = 16 / (int)sizeof(T);
-    if (nc == 1) return go(std::integral_constant<int, VT>{}, std::integral_constant<int, 1>{});
-    return go(std::integral_constant<int, VT>{}, std::integral_constant<int, 2>{});
+  constexpr int VT = 16 / (int)sizeof(T);
+  using Lanes = std::integral_constant<Pairing, kLanes>;
+  using Neighbours = std::integral_constant<Pairing, kNeighbours>;
+  using Staged = std::integral_constant<Pairing, kStaged>;
+  using Vec = std::integral_constant<int, VT>;
+  using One = std::integral_constant<int, 1>;
+  if (c.vec && nc == 1) {
+    if (a.interleaved) return go(Vec{}, One{}, Neighbours{});
+    if (a.half % VT == 0) return go(Vec{}, One{}, Lanes{});
+    return go(Vec{}, One{}, Staged{});
   }
-  return go(std::integral_constant<int, 1>{}, std::integral_constant<int, kMaxDim / 32>{});
+  if (c.vec) return go(Vec{}, std::integral_constant<int, 2>{}, Staged{});
+  return go(One{}, std::integral_constant<int, kMaxDim / 32>{}, Staged{});
 }
 
 template <bool kBack>
@@ -359,6 +426,13 @@ bool aligned(const bt_heads* h, int heads, int esize) {
          h->head_stride % m == 0;
 }
 
+// The launch's shape, once it is known whether rows are read in vectors.
+void shape_call(Call& c) {
+  const int V = c.vec ? (c.dtype == BT_DTYPE_BF16 ? 8 : 4) : 1;
+  shape_of(c.a.tokens, max(1, c.a.hq + c.a.hk), ceil_div(c.a.D, V), &c.G, &c.share);
+  c.a.per = kThreads / c.G / c.share;
+}
+
 Call call_of(const bt_qk_norm_rotary_shape* s, const bt_heads* q, const bt_heads* k, const void* wq,
              const void* wk, const bt_heads* yq, const bt_heads* yk) {
   Call c{};
@@ -381,12 +455,12 @@ Call call_of(const bt_qk_norm_rotary_shape* s, const bt_heads* q, const bt_heads
   a.half = s->half;
   a.interleaved = s->interleaved != 0;
   a.eps = s->eps;
-  a.per = tokens_per_pass(a.tokens, max(1, a.hq + a.hk));
   c.dtype = s->dtype;
   c.wdtype = s->weight_dtype;
   const int e = s->dtype == BT_DTYPE_BF16 ? 2 : 4;
   c.vec = (s->dim * e) % 16 == 0 && aligned(q, a.hq, e) && aligned(k, a.hk, e) && aligned(yq, a.hq, e) &&
           aligned(yk, a.hk, e);
+  shape_call(c);
   return c;
 }
 
@@ -415,9 +489,9 @@ extern "C" int bt_qk_norm_rotary(const bt_qk_norm_rotary_shape* s, const bt_head
 
 extern "C" int64_t bt_qk_norm_rotary_workspace(const bt_qk_norm_rotary_shape* s) {
   if (rot::check(s, "bt_qk_norm_rotary_workspace") != BT_OK) return -1;
+  // one row of sums for each block, of which there are at most so many whatever the launch's shape
   const int64_t tokens = (int64_t)s->batch * s->steps;
-  const int per = rot::tokens_per_pass(tokens, max(1, s->q_heads + s->k_heads));
-  return (int64_t)rot::backward_blocks(tokens, per) * 2 * s->dim * 4;
+  return (int64_t)rot::backward_blocks(tokens, 1) * 2 * s->dim * 4;
 }
 
 extern "C" int bt_qk_norm_rotary_backward(const bt_qk_norm_rotary_shape* s, const bt_heads* q,
@@ -436,6 +510,7 @@ extern "C" int bt_qk_norm_rotary_backward(const bt_qk_norm_rotary_shape* s, cons
   c.a.gq = rot::rows_of(dq_out);
   c.a.gk = rot::rows_of(dk_out);
   c.vec = c.vec && rot::aligned(dq_out, c.a.hq, e) && rot::aligned(dk_out, c.a.hk, e);
+  rot::shape_call(c);
   const int blocks = rot::backward_blocks(c.a.tokens, c.a.per);
   const int64_t need = (int64_t)blocks * 2 * s->dim * 4;
   BT_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
@@ -446,10 +521,10 @@ extern "C" int bt_qk_norm_rotary_backward(const bt_qk_norm_rotary_shape* s, cons
   if (dq_weight || dk_weight) {
     const dim3 grid(ceil_div(s->dim, 32), 2);
     if (s->weight_dtype == BT_DTYPE_BF16)
-      rot::weight_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(
+      rot::weight_kernel<<<grid, 1024, 0, (cudaStream_t)stream>>>(
           c.a.partial, blocks, s->dim, static_cast<__nv_bfloat16*>(dq_weight), static_cast<__nv_bfloat16*>(dk_weight));
     else
-      rot::weight_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(
+      rot::weight_kernel<<<grid, 1024, 0, (cudaStream_t)stream>>>(
           c.a.partial, blocks, s->dim, static_cast<float*>(dq_weight), static_cast<float*>(dk_weight));
     BT_LAUNCH_CHECK("query/key norm weight gradients");
   }

@@ -7,12 +7,10 @@ activations its own ("silu", "relu", "tanh", "none").
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import _lib
-from .linear_attention import _DTYPES, _on, _ptr
+from .linear_attention import _DTYPES, _device, _ptr, _wants_grad
 
 
 def _check(x, w_gate, w_up, activation):
@@ -27,9 +25,7 @@ def _check(x, w_gate, w_up, activation):
                         "float32 or bfloat16 expected, the same for all three")
     if min(w_gate.shape) < 1:
         raise ValueError(f"gated_linear_unit: weights {tuple(w_gate.shape)} without features")
-    for t in (x, w_gate, w_up):
-        if not t.is_cuda or t.device != x.device:
-            raise ValueError("gated_linear_unit: CUDA tensors on one device expected")
+    _device("gated_linear_unit", x, w_gate, w_up)
 
 
 def _aligned(t):
@@ -43,22 +39,27 @@ def _shape(x, w, activation):
 
 
 def _workspace(shape, backward, device):
-    n = _lib.lib().bt_glu_workspace(C.byref(shape), backward)
+    n = _lib.lib().bt_glu_workspace(shape, backward)
     return (torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None), n
+
+
+def _forward(x, w_gate, w_up, activation):
+    """The output, and the tensors that the call read."""
+    x, w_gate, w_up = _aligned(x), _aligned(w_gate), _aligned(w_up)
+    out = torch.empty((x.shape[0], w_gate.shape[1]), dtype=x.dtype, device=x.device)
+    with _lib.on_device(x.get_device()) as stream:
+        shape = _shape(x, w_gate, activation)
+        ws, n = _workspace(shape, 0, x.device)
+        _lib.check(_lib.lib().bt_glu(shape, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(),
+                                     out.data_ptr(), _ptr(ws), n, stream))
+    return out, (x, w_gate, w_up)
 
 
 class _Glu(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, activation):
-        x, w_gate, w_up = _aligned(x), _aligned(w_gate), _aligned(w_up)
-        out = torch.empty(x.shape[0], w_gate.shape[1], dtype=x.dtype, device=x.device)
-        with _on(x.device):
-            shape = _shape(x, w_gate, activation)
-            ws, n = _workspace(shape, 0, x.device)
-            _lib.check(_lib.lib().bt_glu(C.byref(shape), x.data_ptr(), w_gate.data_ptr(),
-                                         w_up.data_ptr(), out.data_ptr(), _ptr(ws), n,
-                                         torch.cuda.current_stream().cuda_stream))
-        ctx.save_for_backward(x, w_gate, w_up)
+        out, read = _forward(x, w_gate, w_up, activation)
+        ctx.save_for_backward(*read)
         ctx.activation = activation
         return out
 
@@ -71,13 +72,12 @@ class _Glu(torch.autograd.Function):
         weights = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dwg = torch.empty_like(w_gate) if weights else None
         dwu = torch.empty_like(w_up) if weights else None
-        with _on(x.device):
+        with _lib.on_device(x.get_device()) as stream:
             shape = _shape(x, w_gate, ctx.activation)
             ws, n = _workspace(shape, 1, x.device)
             _lib.check(_lib.lib().bt_glu_backward(
-                C.byref(shape), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), dout.data_ptr(),
-                _ptr(dx), _ptr(dwg), _ptr(dwu), _ptr(ws), n,
-                torch.cuda.current_stream().cuda_stream))
+                shape, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), dout.data_ptr(), _ptr(dx),
+                _ptr(dwg), _ptr(dwu), _ptr(ws), n, stream))
         return dx, dwg, dwu, None
 
 
@@ -87,4 +87,8 @@ def gated_linear_unit(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     sums in float32, the result [..., out] in x's dtype."""
     _check(x, w_gate, w_up, activation)
     rows = x.reshape(-1, x.shape[-1])
-    return _Glu.apply(rows, w_gate, w_up, activation).reshape(*x.shape[:-1], w_gate.shape[1])
+    if _wants_grad(x, w_gate, w_up):
+        out = _Glu.apply(rows, w_gate, w_up, activation)
+    else:
+        out = _forward(rows, w_gate, w_up, activation)[0]
+    return out.reshape(*x.shape[:-1], w_gate.shape[1])

@@ -17,8 +17,6 @@ that is not finite may reach other steps of its own (batch row, head) sequence, 
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import _lib
@@ -35,38 +33,47 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _on(device):
-    """The device's context where it is not the current one."""
-    return torch.cuda.device(device)
+def _device(name, first, *others) -> int:
+    """The CUDA device of all the tensors (those that are not None)."""
+    index = first.get_device()
+    if index < 0:
+        raise ValueError(f"{name}: CUDA tensors on one device expected")
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{name}: CUDA tensors on one device expected")
+    return index
 
 
-def _check(name, q, k, v, log_decay, state, reset):
-    lead = "[batch, steps, heads" if name == "linear_attention" else "[batch, heads"
-    ndim = 4 if name == "linear_attention" else 3
-    if q.ndim != ndim or k.shape != q.shape or v.shape[:-1] != q.shape[:-1] or v.ndim != ndim:
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _check(name, ndim, q, k, v, log_decay, state, reset) -> int:
+    """The device's index."""
+    shape, vshape = q.shape, v.shape
+    if len(shape) != ndim or k.shape != shape or len(vshape) != ndim or vshape[:-1] != shape[:-1]:
+        lead = "[batch, steps, heads" if ndim == 4 else "[batch, heads"
         raise ValueError(f"{name}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: "
                          f"{lead}, features] expected, alike in all but v's features")
     if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f"{name}: q {q.dtype}, k {k.dtype}, v {v.dtype}: float32 or bfloat16 "
                         "expected, the same for all three")
-    if not (1 <= q.shape[-1] <= 128 and 1 <= v.shape[-1] <= 128):
-        raise ValueError(f"{name}: heads of {q.shape[-1]} and {v.shape[-1]} features: 1 to 128 "
+    if not (1 <= shape[-1] <= 128 and 1 <= vshape[-1] <= 128):
+        raise ValueError(f"{name}: heads of {shape[-1]} and {vshape[-1]} features: 1 to 128 "
                          "are supported")
-    batch, heads = q.shape[0], q.shape[-2]
-    if log_decay.shape != (heads,) or log_decay.dtype != torch.float32:
+    if log_decay.shape != shape[-2:-1] or log_decay.dtype != torch.float32:
         raise ValueError(f"{name}: log_decay {tuple(log_decay.shape)} {log_decay.dtype}: "
-                         f"({heads},) float32 expected")
+                         f"({shape[-2]},) float32 expected")
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name}: log_decay is a constant and has no gradient; detach it")
-    want = (batch, heads, q.shape[-1], v.shape[-1])
-    if state is not None and (tuple(state.shape) != want or state.dtype != torch.float32):
-        raise ValueError(f"{name}: state {tuple(state.shape)} {state.dtype}: {want} float32 expected")
-    if reset is not None and (reset.shape != q.shape[:ndim - 2] or reset.dtype != torch.bool):
+    if state is not None:
+        want = (shape[0], shape[-2], shape[-1], vshape[-1])
+        if state.shape != want or state.dtype != torch.float32:
+            raise ValueError(f"{name}: state {tuple(state.shape)} {state.dtype}: {want} float32 expected")
+    if reset is not None and (reset.shape != shape[:ndim - 2] or reset.dtype != torch.bool):
         raise ValueError(f"{name}: reset {tuple(reset.shape)} {reset.dtype}: "
-                         f"{tuple(q.shape[:ndim - 2])} bool expected")
-    for t in (q, k, v, log_decay, state, reset):
-        if t is not None and (not t.is_cuda or t.device != q.device):
-            raise ValueError(f"{name}: CUDA tensors on one device expected")
+                         f"{tuple(shape[:ndim - 2])} bool expected")
+    return _device(name, q, k, v, log_decay, state, reset)
 
 
 def _shape(q, v, log_decay, reset, scale) -> _lib.LinearAttentionShape:
@@ -82,25 +89,31 @@ def _ptr(t):
 
 
 def _workspace(shape, backward, device):
-    n = _lib.lib().bt_linear_attention_workspace(C.byref(shape), backward)
+    n = _lib.lib().bt_linear_attention_workspace(shape, backward)
     return (torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None), n
+
+
+def _forward(q, k, v, log_decay, state, reset, scale):
+    """(out, final state) and the tensors that the call read."""
+    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
+    state = None if state is None else state.contiguous()
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    final = torch.empty((q.shape[0], q.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32,
+                        device=q.device)
+    with _lib.on_device(q.get_device()) as stream:
+        shape = _shape(q, v, log_decay, reset, scale)
+        ws, n = _workspace(shape, 0, q.device)
+        _lib.check(_lib.lib().bt_linear_attention(
+            shape, _heads(q), _heads(k), _heads(v), _ptr(state), _heads(out), final.data_ptr(),
+            _ptr(ws), n, stream))
+    return out, final, (q, k, v, log_decay, state, reset)
 
 
 class _LinearAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, state, reset, scale):
-        q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
-        state = None if state is None else state.contiguous()
-        out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-        final = torch.empty(q.shape[0], q.shape[2], q.shape[3], v.shape[3], dtype=torch.float32,
-                            device=q.device)
-        with _on(q.device):
-            shape = _shape(q, v, log_decay, reset, scale)
-            ws, n = _workspace(shape, 0, q.device)
-            _lib.check(_lib.lib().bt_linear_attention(
-                C.byref(shape), _heads(q), _heads(k), _heads(v), _ptr(state), _heads(out),
-                final.data_ptr(), _ptr(ws), n, torch.cuda.current_stream().cuda_stream))
-        ctx.save_for_backward(q, k, v, log_decay, state, reset)
+        out, final, read = _forward(q, k, v, log_decay, state, reset, scale)
+        ctx.save_for_backward(*read)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return out, final
@@ -114,15 +127,14 @@ class _LinearAttention(torch.autograd.Function):
         dout = torch.zeros_like(v) if dout is None else _rows(dout.to(v.dtype))
         dfinal = None if dfinal is None else dfinal.contiguous()
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        dstate = torch.empty(q.shape[0], q.shape[2], q.shape[3], v.shape[3], dtype=torch.float32,
+        dstate = torch.empty((q.shape[0], q.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32,
                              device=q.device)
-        with _on(q.device):
+        with _lib.on_device(q.get_device()) as stream:
             shape = _shape(q, v, log_decay, reset, ctx.scale)
             ws, n = _workspace(shape, 1, q.device)
             _lib.check(_lib.lib().bt_linear_attention_backward(
-                C.byref(shape), _heads(q), _heads(k), _heads(v), _ptr(state), _heads(dout),
-                _ptr(dfinal), _heads(dq), _heads(dk), _heads(dv), dstate.data_ptr(), _ptr(ws), n,
-                torch.cuda.current_stream().cuda_stream))
+                shape, _heads(q), _heads(k), _heads(v), _ptr(state), _heads(dout), _ptr(dfinal),
+                _heads(dq), _heads(dk), _heads(dv), dstate.data_ptr(), _ptr(ws), n, stream))
         return dq, dk, dv, None, (dstate if ctx.needs_input_grad[4] else None), None, None
 
 
@@ -131,8 +143,10 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
                      scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(out, final state) of the steps, from `state` (None: zeros). `scale` is 1 / sqrt(key
     features) unless given."""
-    _check("linear_attention", q, k, v, log_decay, state, reset)
+    _check("linear_attention", 4, q, k, v, log_decay, state, reset)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if not _wants_grad(q, k, v, state):
+        return _forward(q, k, v, log_decay, state, reset, scale)[:2]
     return _LinearAttention.apply(q, k, v, log_decay, state, reset, scale)
 
 
@@ -144,17 +158,16 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """(out, new state) of one acting step: q, k [batch, heads, key features], v [batch, heads,
     value features], reset [batch]. `new_state` takes the updated state (it may be `state` itself);
     a new tensor unless given. It has no gradient: train through `linear_attention`."""
-    _check("linear_attention_step", q, k, v, log_decay, state, reset)
+    device = _check("linear_attention_step", 3, q, k, v, log_decay, state, reset)
     if state is None:
         raise ValueError("linear_attention_step: a state is expected")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                    or state.requires_grad):
+    if _wants_grad(q, k, v, state, new_state):
         raise ValueError("linear_attention_step has no gradient: use linear_attention, or detach")
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
     if new_state is None:
         new_state = torch.empty(state.shape, dtype=torch.float32, device=q.device)
     elif (new_state.shape != state.shape or new_state.dtype != torch.float32
-          or new_state.device != q.device or not new_state.is_contiguous()):
+          or new_state.get_device() != device or not new_state.is_contiguous()):
         raise ValueError(f"linear_attention_step: new_state {tuple(new_state.shape)} "
                          f"{new_state.dtype}: a contiguous {tuple(state.shape)} float32 tensor expected")
     elif new_state.data_ptr() != state.data_ptr() and _overlap(new_state, state):
@@ -162,11 +175,10 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     state = state.contiguous()
     out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    with _on(q.device):
-        shape = _shape(q, v, log_decay, reset, scale)
+    with _lib.on_device(device) as stream:
         _lib.check(_lib.lib().bt_linear_attention_step(
-            C.byref(shape), _heads(q), _heads(k), _heads(v), state.data_ptr(), out.data_ptr(),
-            new_state.data_ptr(), torch.cuda.current_stream().cuda_stream))
+            _shape(q, v, log_decay, reset, scale), _heads(q), _heads(k), _heads(v),
+            state.data_ptr(), out.data_ptr(), new_state.data_ptr(), stream))
     return out, new_state
 
 

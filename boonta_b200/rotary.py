@@ -7,12 +7,10 @@ takes as its queries and keys. Differentiable in q, k and the weights through th
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import _lib
-from .linear_attention import _DTYPES, _heads, _on, _ptr, _rows
+from .linear_attention import _DTYPES, _device, _heads, _ptr, _rows, _wants_grad
 
 
 def rotary_frequencies(dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -41,31 +39,34 @@ def _check(q, k, q_weight, k_weight, positions, frequencies):
     if frequencies.ndim != 1 or frequencies.dtype != torch.float64 or 2 * len(frequencies) > dim:
         raise ValueError(f"qk_norm_rotary: frequencies {tuple(frequencies.shape)} "
                          f"{frequencies.dtype}: at most {dim // 2} in float64 expected")
-    if positions.dtype != torch.int64 or positions.shape not in (q.shape[:2], q.shape[1:2]):
+    if positions.dtype != torch.int64 or (positions.shape != q.shape[:2] and positions.shape != q.shape[1:2]):
         raise ValueError(f"qk_norm_rotary: positions {tuple(positions.shape)} {positions.dtype}: "
                          f"{tuple(q.shape[:2])} or {tuple(q.shape[1:2])} int64 expected")
-    for t in (q, k, *weights, positions, frequencies):
-        if not t.is_cuda or t.device != q.device:
-            raise ValueError("qk_norm_rotary: CUDA tensors on one device expected")
+    _device("qk_norm_rotary", q, k, q_weight, k_weight, positions, frequencies)
+
+
+def _forward(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
+    """The outputs, and the tensors that the call read."""
+    q, k = _rows(q), _rows(k)
+    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    frequencies = frequencies.contiguous()
+    if positions.ndim == 1:
+        positions = positions.expand(q.shape[0], -1)
+    yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    with _lib.on_device(q.get_device()) as stream:
+        _lib.check(_lib.lib().bt_qk_norm_rotary(
+            _shape(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved), _heads(q),
+            _heads(k), _ptr(q_weight), _ptr(k_weight), _heads(yq), _heads(yk), stream))
+    return yq, yk, (q, k, q_weight, k_weight, positions, frequencies)
 
 
 class _QkNormRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
-        q, k = _rows(q), _rows(k)
-        q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
-        frequencies = frequencies.contiguous()
-        if positions.ndim == 1:
-            positions = positions.expand(q.shape[0], -1)
         ctx.eps, ctx.interleaved = eps, interleaved
-        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        with _on(q.device):
-            _lib.check(_lib.lib().bt_qk_norm_rotary(
-                C.byref(_shape(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)),
-                _heads(q), _heads(k), _ptr(q_weight), _ptr(k_weight), _heads(yq), _heads(yk),
-                torch.cuda.current_stream().cuda_stream))
-        ctx.save_for_backward(q, k, q_weight, k_weight, positions, frequencies)
+        yq, yk, read = _forward(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved)
+        ctx.save_for_backward(*read)
         return yq, yk
 
     @staticmethod
@@ -77,14 +78,13 @@ class _QkNormRotary(torch.autograd.Function):
         dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
         dwq = torch.empty_like(q_weight) if ctx.needs_input_grad[2] else None
         dwk = torch.empty_like(k_weight) if ctx.needs_input_grad[3] else None
-        with _on(q.device):
+        with _lib.on_device(q.get_device()) as stream:
             shape = _shape(q, k, q_weight, k_weight, positions, frequencies, ctx.eps, ctx.interleaved)
-            n = _lib.lib().bt_qk_norm_rotary_workspace(C.byref(shape))
+            n = _lib.lib().bt_qk_norm_rotary_workspace(shape)
             ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n > 0 else None
             _lib.check(_lib.lib().bt_qk_norm_rotary_backward(
-                C.byref(shape), _heads(q), _heads(k), _ptr(q_weight), _ptr(k_weight), _heads(gq),
-                _heads(gk), _heads(dq), _heads(dk), _ptr(dwq), _ptr(dwk), _ptr(ws), n,
-                torch.cuda.current_stream().cuda_stream))
+                shape, _heads(q), _heads(k), _ptr(q_weight), _ptr(k_weight), _heads(gq), _heads(gk),
+                _heads(dq), _heads(dk), _ptr(dwq), _ptr(dwk), _ptr(ws), n, stream))
         return dq, dk, dwq, dwk, None, None, None, None
 
 
@@ -106,5 +106,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
     (`rotary_frequencies`): the first 2 r features are turned, feature i with feature i + r, or
     2 i with 2 i + 1 where `interleaved`, the others only normed."""
     _check(q, k, q_weight, k_weight, positions, frequencies)
+    if not _wants_grad(q, k, q_weight, k_weight):
+        return _forward(q, k, q_weight, k_weight, positions, frequencies, float(eps),
+                        bool(interleaved))[:2]
     return _QkNormRotary.apply(q, k, q_weight, k_weight, positions, frequencies, float(eps),
                                bool(interleaved))
