@@ -58,17 +58,32 @@ __device__ __forceinline__ T from_float(float x) {
   return x;
 }
 
+// V neighbouring elements as they lie in memory.
 template <class T, int V>
-__device__ __forceinline__ void load(const T* p, float (&v)[V]) {
-  if constexpr (V == 1) {
-    v[0] = to_float(*p);
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const T* t = reinterpret_cast<const T*>(&u);
+struct Raw {
+  uint4 u;
+  __device__ __forceinline__ void load(const T* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float (&v)[V]) const {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = to_float(t[i]);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        v[i] = __uint_as_float(w[i]);
+      }
+    }
   }
-}
+};
+template <class T>
+struct Raw<T, 1> {
+  T t;
+  __device__ __forceinline__ void load(const T* p) { t = *p; }
+  __device__ __forceinline__ void zero() { t = from_float<T>(0.f); }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = to_float(t); }
+};
 template <class T, int V>
 __device__ __forceinline__ void store(T* p, const float (&v)[V]) {
   if constexpr (V == 1) {
@@ -164,34 +179,35 @@ __device__ __forceinline__ void turn(const Args& a, float (&x)[NC][V], const Tur
   }
 }
 
-// G lanes to a row; a token's rows go round `share` groups, and a block's pass takes a.per tokens.
+// G lanes to a row; a token's rows go round `share` groups, kRows of them on their way at a time, and a
+// block's pass takes a.per tokens.
 template <class T, class W, int V, int NC, Pairing kP, bool kBack>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ Args a, int G, int share) {
+__global__ void __launch_bounds__(kThreads, NC == 1 ? 3 : 1)
+    rotary_kernel(const __grid_constant__ Args a, int G, int share) {
+  constexpr int kRows = NC > 2 ? 1 : kBack ? 2 : 4;
   extern __shared__ __align__(16) float sm[];
   float* cs = sm;                                 // [per][2 half]
   float* rows = sm + a.per * 2 * a.half;          // [groups][D] staging rows
   __shared__ int64_t s_off[kMaxTokens][6];        // element offsets of a token in q, k, yq, yk, gq, gk
+  __shared__ double s_pos[kMaxTokens];
   const int lane = threadIdx.x % G, group = threadIdx.x / G, groups = kThreads / G;
   float* row = rows + group * a.D;
   const unsigned mask = G == 32 ? ~0u : ((1u << G) - 1u) << ((threadIdx.x & 31) / G * G);
   const int tok = group / share, first = group % share;
-  float w[2][NC][V], dw[kBack ? 2 : 1][NC][V];
+  float dw[kBack ? 2 : 1][NC][V];
 #pragma unroll
   for (int c = 0; c < NC; ++c)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int d = (c * G + lane) * V + i;
-      const bool in = d < a.D;
-      w[0][c][i] = in && a.wq ? to_float(static_cast<const W*>(a.wq)[d]) : 1.f;
-      w[1][c][i] = in && a.wk ? to_float(static_cast<const W*>(a.wk)[d]) : 1.f;
+    for (int i = 0; i < V; ++i)
       if (kBack) dw[0][c][i] = dw[kBack ? 1 : 0][c][i] = 0.f;
-    }
   const float inv = 1.f / (float)a.D;
   for (int64_t t0 = (int64_t)blockIdx.x * a.per; t0 < a.tokens; t0 += (int64_t)gridDim.x * a.per) {
     const int n = (int)min((int64_t)a.per, a.tokens - t0);
     __syncthreads();
     if (threadIdx.x < n) {
-      const int64_t t = t0 + threadIdx.x, b = t / a.steps, st = t % a.steps;
+      const int64_t t = t0 + threadIdx.x;
+      const int64_t b = a.tokens >> 31 ? t / a.steps : (int64_t)((unsigned)t / (unsigned)a.steps), st = t - b * a.steps;
+      s_pos[threadIdx.x] = a.half ? (double)a.pos[b * a.pos_batch + st * a.pos_step] : 0.0;
       int64_t* f = s_off[threadIdx.x];
       f[0] = b * a.q.batch + st * a.q.step;
       f[1] = b * a.k.batch + st * a.k.step;
@@ -200,96 +216,107 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
       f[4] = b * a.gq.batch + st * a.gq.step;
       f[5] = b * a.gk.batch + st * a.gk.step;
     }
+    __syncthreads();
+    // groups without a token walk along: a warp's lanes stay together
+    const bool mine = tok < n;
+    const int64_t* f = s_off[mine ? tok : 0];
+    Raw<T, V> nx[kRows][NC], ng[kBack ? kRows : 1][NC];
+    // the rows h, h + share, .. of queries (0) or keys (1)
+    auto fetch = [&](int which, int h) {
+      const T* xp = static_cast<const T*>(which ? a.k.p : a.q.p) + f[which];
+      const T* gp = static_cast<const T*>(which ? a.gk.p : a.gq.p) + f[4 + which];
+      const int64_t xh = which ? a.k.head : a.q.head, gh = which ? a.gk.head : a.gq.head;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r, h += share)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const int d = (c * G + lane) * V;
+          nx[r][c].zero();
+          if (kBack) ng[kBack ? r : 0][c].zero();
+          if (mine && h < (which ? a.hk : a.hq) && d < a.D) {
+            nx[r][c].load(xp + h * xh + d);
+            if (kBack) ng[kBack ? r : 0][c].load(gp + h * gh + d);
+          }
+        }
+    };
+    fetch(0, first);  // on their way while the angles are formed
     for (int e = threadIdx.x; e < n * a.half; e += kThreads) {
-      const int u = e / a.half, i = e - u * a.half;
-      const int64_t t = t0 + u, b = t / a.steps;
+      const int u = (unsigned)e / (unsigned)a.half, i = e - u * a.half;
       // in turns, so that the whole ones drop out exactly before the 32-bit functions
-      const double ang = (double)a.pos[b * a.pos_batch + (t - b * a.steps) * a.pos_step] * a.freq[i] * 0.15915494309189535;
+      const double ang = s_pos[u] * a.freq[i] * 0.15915494309189535;
       float s, c;
       sincospif((float)(2.0 * (ang - rint(ang))), &s, &c);
       cs[u * 2 * a.half + i] = c;
       cs[u * 2 * a.half + a.half + i] = s;
     }
     __syncthreads();
-    // groups without a token walk along: a warp's lanes stay together
-    const bool mine = tok < n;
     const float* ct = cs + (mine ? tok : 0) * 2 * a.half;
     Turn<V> tn;
     load_turn<kP, V, NC>(a, ct, lane, tn);
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {  // the queries, then the keys
+    for (int which = 0; which < 2; ++which) {
       const int H = which ? a.hk : a.hq;
-      const Rows &src = which ? a.k : a.q, &dst = which ? a.yk : a.yq, &gsrc = which ? a.gk : a.gq;
-      const int64_t* f = s_off[mine ? tok : 0];
-      const T* xp = static_cast<const T*>(src.p) + f[which];
-      T* yp = static_cast<T*>(dst.p) + f[2 + which];
-      const T* gp = static_cast<const T*>(gsrc.p) + f[4 + which];
-      float nx[NC][V], ng[kBack ? NC : 1][V];
-      auto fetch = [&](int h) {
+      float w[NC][V];
+      const void* wp = which ? a.wk : a.wq;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const int d = (c * G + lane) * V;
-          const bool in = mine && h < H && d < a.D;
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            nx[c][i] = 0.f;
-            if (kBack) ng[kBack ? c : 0][i] = 0.f;
-          }
-          if (in) {
-            load<T, V>(xp + h * src.head + d, nx[c]);
-            if constexpr (kBack) load<T, V>(gp + h * gsrc.head + d, ng[c]);
-          }
+        for (int i = 0; i < V; ++i) {
+          const int d = (c * G + lane) * V + i;
+          w[c][i] = d < a.D && wp ? to_float(static_cast<const W*>(wp)[d]) : 1.f;
         }
-      };
-      fetch(first);
-      for (int h0 = 0; h0 < H; h0 += share) {
-        const int h = h0 + first;
-        const bool on = mine && h < H;
-        float x[NC][V], g[kBack ? NC : 1][V];
+      T* yp = static_cast<T*>(which ? a.yk.p : a.yq.p) + f[2 + which];
+      const int64_t yh = which ? a.yk.head : a.yq.head;
+      if (which) fetch(1, first);
+      for (int h0 = 0; h0 < H; h0 += kRows * share) {
+        if (h0) fetch(which, h0 + first);
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+        for (int r = 0; r < kRows; ++r) {
+          const int h = h0 + r * share + first;
+          const bool on = mine && h < H;
+          float x[NC][V], g[kBack ? NC : 1][V];
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            x[c][i] = nx[c][i];
-            if (kBack) g[kBack ? c : 0][i] = ng[kBack ? c : 0][i];
+          for (int c = 0; c < NC; ++c) {
+            nx[r][c].get(x[c]);
+            if constexpr (kBack) ng[r][c].get(g[c]);
           }
-        fetch(h + share);
-        float ss = 0.f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int i = 0; i < V; ++i) ss += x[c][i] * x[c][i];
-        for (int o = G >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const float rs = rsqrtf(ss * inv + a.eps);
-        if constexpr (!kBack) {
+          float ss = 0.f;
 #pragma unroll
           for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int i = 0; i < V; ++i) x[c][i] *= rs * w[which][c][i];
-          turn<kP, V, NC>(a, x, tn, row, ct, 1.f, lane, G, mask);
-        } else {
-          turn<kP, V, NC>(a, g, tn, row, ct, -1.f, lane, G, mask);
-          float m = 0.f;
+            for (int i = 0; i < V; ++i) ss += x[c][i] * x[c][i];
+          for (int o = G >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+          const float rs = rsqrtf(ss * inv + a.eps);
+          if constexpr (!kBack) {
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              x[c][i] *= rs;
-              dw[kBack ? which : 0][c][i] += on ? g[c][i] * x[c][i] : 0.f;
-              g[c][i] *= w[which][c][i];
-              m += g[c][i] * x[c][i];
-            }
-          for (int o = G >> 1; o > 0; o >>= 1) m += __shfl_xor_sync(mask, m, o);
-          m *= inv;
+              for (int i = 0; i < V; ++i) x[c][i] *= rs * w[c][i];
+            turn<kP, V, NC>(a, x, tn, row, ct, 1.f, lane, G, mask);
+          } else {
+            turn<kP, V, NC>(a, g, tn, row, ct, -1.f, lane, G, mask);
+            float m = 0.f;
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int i = 0; i < V; ++i) x[c][i] = rs * (g[c][i] - x[c][i] * m);
-        }
+              for (int i = 0; i < V; ++i) {
+                x[c][i] *= rs;
+                dw[kBack ? which : 0][c][i] += on ? g[c][i] * x[c][i] : 0.f;
+                g[c][i] *= w[c][i];
+                m += g[c][i] * x[c][i];
+              }
+            for (int o = G >> 1; o > 0; o >>= 1) m += __shfl_xor_sync(mask, m, o);
+            m *= inv;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const int d = (c * G + lane) * V;
-          if (on && d < a.D) store<T, V>(yp + h * dst.head + d, x[c]);
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+              for (int i = 0; i < V; ++i) x[c][i] = rs * (g[c][i] - x[c][i] * m);
+          }
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            const int d = (c * G + lane) * V;
+            if (on && d < a.D) store<T, V>(yp + h * yh + d, x[c]);
+          }
         }
       }
     }
