@@ -30,6 +30,7 @@
 // (planes of w c in place of a, which P0 and O are done with).
 #include <type_traits>
 
+#include "f32x2.cuh"
 #include "gemm_sm100.cuh"
 #include "linear_attention.cuh"
 
@@ -113,20 +114,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  return (uint64_t)__float_as_uint(hi) << 32 | __float_as_uint(lo);
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t sub2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
 }
 
 // The bits lo .. hi of a word (positions outside 0 .. 31 allowed).
@@ -384,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           // 24 bits cut into 8 + 8 + 8: each plane takes the leading bits, the rest is exact
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            uint64_t v = mul2(w, (uint64_t)(xs[i] & 0xffff0000u) << 32 | (xs[i] << 16));
+            uint64_t v = mul2(w, pair_of_bf16(xs[i]));
 #pragma unroll
             for (int q = 0; q < 3; ++q) {
               y[q][i] = __byte_perm((uint32_t)v, (uint32_t)(v >> 32), 0x7632);

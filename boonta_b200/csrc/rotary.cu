@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace bt {
 namespace rot {
@@ -58,23 +59,33 @@ __device__ __forceinline__ T from_float(float x) {
   return x;
 }
 
-// V neighbouring elements as they lie in memory.
+// V neighbouring elements as they lie in memory; as values, and (V even) as pairs.
 template <class T, int V>
 struct Raw {
-  uint4 u;
-  __device__ __forceinline__ void load(const T* p) { u = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void get(float (&v)[V]) const {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const T* p) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+  }
+  __device__ __forceinline__ void zero() { w[0] = w[1] = w[2] = w[3] = 0; }
+  __device__ __forceinline__ Raw from_lane(unsigned mask, int lane, int G) const {
+    Raw r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 2) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      } else {
-        v[i] = __uint_as_float(w[i]);
-      }
+    for (int i = 0; i < 4; ++i) r.w[i] = __shfl_sync(mask, w[i], lane, G);
+    return r;
+  }
+  __device__ __forceinline__ void get(uint64_t (&v)[V / 2]) const {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      if constexpr (sizeof(T) == 2) v[i] = pair_of_bf16(w[i]);
+      else v[i] = (uint64_t)w[2 * i + 1] << 32 | w[2 * i];
     }
+  }
+  __device__ __forceinline__ void get(float (&v)[V]) const {
+    uint64_t p[V / 2];
+    get(p);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) v[2 * i] = low(p[i]), v[2 * i + 1] = high(p[i]);
   }
 };
 template <class T>
@@ -84,6 +95,14 @@ struct Raw<T, 1> {
   __device__ __forceinline__ void zero() { t = from_float<T>(0.f); }
   __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = to_float(t); }
 };
+
+template <class T, int N>
+__device__ __forceinline__ void store(T* p, const uint64_t (&v)[N]) {
+  if constexpr (sizeof(T) == 2)
+    *reinterpret_cast<uint4*>(p) = make_uint4(bf16_of_pair(v[0]), bf16_of_pair(v[1]), bf16_of_pair(v[2]), bf16_of_pair(v[3]));
+  else
+    *reinterpret_cast<float4*>(p) = make_float4(low(v[0]), high(v[0]), low(v[1]), high(v[1]));
+}
 template <class T, int V>
 __device__ __forceinline__ void store(T* p, const float (&v)[V]) {
   if constexpr (V == 1) {
@@ -104,79 +123,66 @@ enum Pairing {
   kStaged     // anything else, through shared memory
 };
 
-template <int V>
-struct Turn {  // a lane's cosines and signed sines (kLanes: V, kNeighbours: V / 2)
-  float c[V], s[V];
+// A lane's pairs of the rotation x -> x c + partner(x) s (the sign of the sine in s), kept for a token's
+// rows. In kLanes the partner is the same element of another lane, in kNeighbours the other one of the pair.
+template <int N>
+struct Turn {
+  uint64_t c[N], s[N];
 };
 
-template <Pairing kP, int V, int NC>
-__device__ __forceinline__ void load_turn(const Args& a, const float* cs, int lane, Turn<V>& t) {
-  if constexpr (kP == kStaged) return;
-  const int d = lane * V;
+template <Pairing kP, int N>
+__device__ __forceinline__ void load_turn(const Args& a, const float* cs, int lane, Turn<N>& t) {
+  const int d = lane * 2 * N;
 #pragma unroll
-  for (int i = 0; i < V; ++i) t.c[i] = 1.f, t.s[i] = 0.f;
+  for (int i = 0; i < N; ++i) t.c[i] = pair(1.f, 1.f), t.s[i] = 0;
   if (d >= 2 * a.half) return;
+  const float* sn = cs + a.half;
   if constexpr (kP == kLanes) {
     const bool second = d >= a.half;
-    const int pair = second ? d - a.half : d;
+    const int k = second ? d - a.half : d;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      t.c[i] = cs[pair + i];
-      t.s[i] = second ? cs[a.half + pair + i] : -cs[a.half + pair + i];
+    for (int i = 0; i < N; ++i) {
+      t.c[i] = pair(cs[k + 2 * i], cs[k + 2 * i + 1]);
+      t.s[i] = second ? pair(sn[k + 2 * i], sn[k + 2 * i + 1]) : pair(-sn[k + 2 * i], -sn[k + 2 * i + 1]);
     }
-  } else if constexpr (kP == kNeighbours) {
+  } else {
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i)
+    for (int i = 0; i < N; ++i)
       if (d / 2 + i < a.half) {
-        t.c[i] = cs[d / 2 + i];
-        t.s[i] = cs[a.half + d / 2 + i];
+        t.c[i] = pair(cs[d / 2 + i], cs[d / 2 + i]);
+        t.s[i] = pair(-sn[d / 2 + i], sn[d / 2 + i]);
       }
   }
 }
 
-// Turns x by the token's angles (sign 1), or back (-1).
-template <Pairing kP, int V, int NC>
-__device__ __forceinline__ void turn(const Args& a, float (&x)[NC][V], const Turn<V>& t, float* row, const float* cs,
-                                     float sign, int lane, int G, unsigned mask) {
-  if constexpr (kP == kLanes) {
-    const int h = a.half / V;
-    const int from = lane < h ? lane + h : lane < 2 * h ? lane - h : lane;
+__device__ __forceinline__ uint64_t swapped(uint64_t a) { return a << 32 | a >> 32; }
+
+// Turns x by the token's angles (sign 1), or back (-1), through the group's row in shared memory.
+template <int V, int NC>
+__device__ __forceinline__ void turn(const Args& a, float (&x)[NC][V], float* row, const float* cs, float sign,
+                                     int lane, int G) {
+  const int rd = 2 * a.half;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float other = __shfl_sync(mask, x[0][i], from, G);
-      x[0][i] = x[0][i] * t.c[i] + other * (sign * t.s[i]);
+      const int d = (c * G + lane) * V + i;
+      if (d < rd) row[d] = x[c][i];
     }
-  } else if constexpr (kP == kNeighbours) {
+  __syncwarp();
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      const float p = x[0][2 * i], q = x[0][2 * i + 1], si = sign * t.s[i];
-      x[0][2 * i] = p * t.c[i] - q * si;
-      x[0][2 * i + 1] = q * t.c[i] + p * si;
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int d = (c * G + lane) * V + i;
+      if (d >= rd) continue;
+      const bool second = a.interleaved ? d & 1 : d >= a.half;
+      const int k = a.interleaved ? d >> 1 : second ? d - a.half : d;
+      const float other = row[a.interleaved ? d ^ 1 : (second ? d - a.half : d + a.half)];
+      const float co = cs[k], si = sign * cs[a.half + k];
+      x[c][i] = second ? x[c][i] * co + other * si : x[c][i] * co - other * si;
     }
-  } else {
-    const int rd = 2 * a.half;
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int d = (c * G + lane) * V + i;
-        if (d < rd) row[d] = x[c][i];
-      }
-    __syncwarp();
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int d = (c * G + lane) * V + i;
-        if (d >= rd) continue;
-        const bool second = a.interleaved ? d & 1 : d >= a.half;
-        const int pair = a.interleaved ? d >> 1 : second ? d - a.half : d;
-        const float other = row[a.interleaved ? d ^ 1 : (second ? d - a.half : d + a.half)];
-        const float co = cs[pair], si = sign * cs[a.half + pair];
-        x[c][i] = second ? x[c][i] * co + other * si : x[c][i] * co - other * si;
-      }
-    __syncwarp();
-  }
+  __syncwarp();
 }
 
 // G lanes to a row; a token's rows go round `share` groups, kRows of them on their way at a time, and a
@@ -251,8 +257,11 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 3 : 1)
     }
     __syncthreads();
     const float* ct = cs + (mine ? tok : 0) * 2 * a.half;
-    Turn<V> tn;
-    load_turn<kP, V, NC>(a, ct, lane, tn);
+    constexpr int N = kP == kStaged ? 1 : V / 2;
+    Turn<N> tn;
+    if constexpr (kP != kStaged) load_turn<kP, N>(a, ct, lane, tn);
+    const int half_lanes = a.half / V;  // kLanes
+    const int partner = lane < half_lanes ? lane + half_lanes : lane < 2 * half_lanes ? lane - half_lanes : lane;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       const int H = which ? a.hk : a.hq;
@@ -265,6 +274,10 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 3 : 1)
           const int d = (c * G + lane) * V + i;
           w[c][i] = d < a.D && wp ? to_float(static_cast<const W*>(wp)[d]) : 1.f;
         }
+      float wo[V];  // the partner lane's weights
+      if constexpr (kP == kLanes && !kBack)
+#pragma unroll
+        for (int i = 0; i < V; ++i) wo[i] = __shfl_sync(mask, w[0][i], partner, G);
       T* yp = static_cast<T*>(which ? a.yk.p : a.yq.p) + f[2 + which];
       const int64_t yh = which ? a.yk.head : a.yq.head;
       if (which) fetch(1, first);
@@ -274,48 +287,106 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 3 : 1)
         for (int r = 0; r < kRows; ++r) {
           const int h = h0 + r * share + first;
           const bool on = mine && h < H;
-          float x[NC][V], g[kBack ? NC : 1][V];
+          if constexpr (kP != kStaged) {
+            const int d = lane * V;
+            uint64_t x[N], sq = 0;
+            nx[r][0].get(x);
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            nx[r][c].get(x[c]);
-            if constexpr (kBack) ng[r][c].get(g[c]);
-          }
-          float ss = 0.f;
+            for (int i = 0; i < N; ++i) sq = fma2(x[i], x[i], sq);
+            float ss = low(sq) + high(sq);
+            for (int o = G >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+            const float rs = rsqrtf(ss * inv + a.eps);
+            const uint64_t rr = pair(rs, rs);
+            if constexpr (!kBack) {
+              // the weights before the exchange: the partner's own
+              uint64_t y[N], z[N];
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
+              for (int i = 0; i < N; ++i) y[i] = mul2(x[i], pair(w[0][2 * i], w[0][2 * i + 1]));
+              if constexpr (kP == kLanes) {
+                nx[r][0].from_lane(mask, partner, G).get(z);
 #pragma unroll
-            for (int i = 0; i < V; ++i) ss += x[c][i] * x[c][i];
-          for (int o = G >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-          const float rs = rsqrtf(ss * inv + a.eps);
-          if constexpr (!kBack) {
+                for (int i = 0; i < N; ++i) z[i] = mul2(z[i], pair(wo[2 * i], wo[2 * i + 1]));
+              } else {
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-              for (int i = 0; i < V; ++i) x[c][i] *= rs * w[c][i];
-            turn<kP, V, NC>(a, x, tn, row, ct, 1.f, lane, G, mask);
-          } else {
-            turn<kP, V, NC>(a, g, tn, row, ct, -1.f, lane, G, mask);
-            float m = 0.f;
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-              for (int i = 0; i < V; ++i) {
-                x[c][i] *= rs;
-                dw[kBack ? which : 0][c][i] += on ? g[c][i] * x[c][i] : 0.f;
-                g[c][i] *= w[c][i];
-                m += g[c][i] * x[c][i];
+                for (int i = 0; i < N; ++i) z[i] = swapped(y[i]);
               }
-            for (int o = G >> 1; o > 0; o >>= 1) m += __shfl_xor_sync(mask, m, o);
-            m *= inv;
+#pragma unroll
+              for (int i = 0; i < N; ++i) x[i] = mul2(rr, fma2(y[i], tn.c[i], mul2(z[i], tn.s[i])));
+            } else {
+              uint64_t g[N], z[N], m2 = 0;
+              ng[r][0].get(g);
+              if constexpr (kP == kLanes) {
+                ng[r][0].from_lane(mask, partner, G).get(z);
+              } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) z[i] = swapped(g[i]);
+              }
+              // back: the sines change their sign
+#pragma unroll
+              for (int i = 0; i < N; ++i) {
+                g[i] = sub2(mul2(g[i], tn.c[i]), mul2(z[i], tn.s[i]));
+                const uint64_t gx = mul2(g[i], x[i]);
+                const uint64_t ww = pair(w[0][2 * i], w[0][2 * i + 1]);
+                const uint64_t was = pair(dw[kBack ? which : 0][0][2 * i], dw[kBack ? which : 0][0][2 * i + 1]);
+                const uint64_t sum = fma2(gx, rr, was);
+                dw[kBack ? which : 0][0][2 * i] = on ? low(sum) : low(was);
+                dw[kBack ? which : 0][0][2 * i + 1] = on ? high(sum) : high(was);
+                m2 = fma2(gx, ww, m2);
+                g[i] = mul2(g[i], ww);
+              }
+              float m = low(m2) + high(m2);
+              for (int o = G >> 1; o > 0; o >>= 1) m += __shfl_xor_sync(mask, m, o);
+              // dx = r (u - x r^2 mean(u x))
+              m *= inv * rs * rs;
+              const uint64_t mm = pair(-m, -m);
+#pragma unroll
+              for (int i = 0; i < N; ++i) x[i] = mul2(rr, fma2(x[i], mm, g[i]));
+            }
+            if (on && d < a.D) store<T, N>(yp + h * yh + d, x);
+          } else {
+            float x[NC][V], g[kBack ? NC : 1][V];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              nx[r][c].get(x[c]);
+              if constexpr (kBack) ng[r][c].get(g[c]);
+            }
+            float ss = 0.f;
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
-              for (int i = 0; i < V; ++i) x[c][i] = rs * (g[c][i] - x[c][i] * m);
-          }
+              for (int i = 0; i < V; ++i) ss += x[c][i] * x[c][i];
+            for (int o = G >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+            const float rs = rsqrtf(ss * inv + a.eps);
+            if constexpr (!kBack) {
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            const int d = (c * G + lane) * V;
-            if (on && d < a.D) store<T, V>(yp + h * yh + d, x[c]);
+              for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[c][i] *= rs * w[c][i];
+              turn<V, NC>(a, x, row, ct, 1.f, lane, G);
+            } else {
+              turn<V, NC>(a, g, row, ct, -1.f, lane, G);
+              float m = 0.f;
+#pragma unroll
+              for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                  x[c][i] *= rs;
+                  dw[kBack ? which : 0][c][i] += on ? g[c][i] * x[c][i] : 0.f;
+                  g[c][i] *= w[c][i];
+                  m += g[c][i] * x[c][i];
+                }
+              for (int o = G >> 1; o > 0; o >>= 1) m += __shfl_xor_sync(mask, m, o);
+              m *= inv;
+#pragma unroll
+              for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[c][i] = rs * (g[c][i] - x[c][i] * m);
+            }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              const int d = (c * G + lane) * V;
+              if (on && d < a.D) store<T, V>(yp + h * yh + d, x[c]);
+            }
           }
         }
       }

@@ -36,7 +36,7 @@ def _check(q, k, q_weight, k_weight, positions, frequencies):
         if w.shape != (dim,) or w.dtype not in _DTYPES or w.dtype != weights[0].dtype:
             raise ValueError(f"qk_norm_rotary: weights of ({dim},) in float32 or bfloat16 expected, "
                              f"alike: got {tuple(w.shape)} {w.dtype}")
-    if frequencies.ndim != 1 or frequencies.dtype != torch.float64 or 2 * len(frequencies) > dim:
+    if frequencies.ndim != 1 or frequencies.dtype != torch.float64 or 2 * frequencies.shape[0] > dim:
         raise ValueError(f"qk_norm_rotary: frequencies {tuple(frequencies.shape)} "
                          f"{frequencies.dtype}: at most {dim // 2} in float64 expected")
     if positions.dtype != torch.int64 or (positions.shape != q.shape[:2] and positions.shape != q.shape[1:2]):
@@ -91,7 +91,7 @@ class _QkNormRotary(torch.autograd.Function):
 def _shape(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved):
     w = q_weight if q_weight is not None else k_weight
     return _lib.QkNormRotaryShape(
-        q.shape[0], q.shape[1], q.shape[2], k.shape[2], q.shape[3], len(frequencies),
+        q.shape[0], q.shape[1], q.shape[2], k.shape[2], q.shape[3], frequencies.shape[0],
         _DTYPES[q.dtype], 0 if w is None else _DTYPES[w.dtype], int(interleaved), eps,
         positions.data_ptr(), positions.stride(0), positions.stride(1), frequencies.data_ptr())
 
