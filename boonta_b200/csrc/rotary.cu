@@ -8,8 +8,8 @@
 //   u = g w,  dx = r (u - xh mean(u xh)); r is formed again from x, which is read anyway.
 //
 // Bound by HBM: forward 2, backward 3 elements per element of x. A block takes a few tokens: it
-// forms their cosines and sines once in shared memory (angle in 64 bits, reduced to one turn
-// before the 32-bit sine, so far positions keep their phase). A group of lanes then walks rows (query
+// forms their cosines and sines once in shared memory (a frequency is a 64-bit fraction of a turn, so
+// that a position's product with it drops whole turns exactly and far positions keep their phase). A group of lanes then walks rows (query
 // or key heads) of one token with 16-byte loads, its cosines and sines in registers, the next row on
 // its way while one is worked on; the partner of an element, half a rotation away, comes from another
 // lane. Where the rotated half does not fall on whole lanes, partners go through the group's row
@@ -185,17 +185,19 @@ __device__ __forceinline__ void turn(const Args& a, float (&x)[NC][V], float* ro
   __syncwarp();
 }
 
-// G lanes to a row; a token's rows go round `share` groups, kRows of them on their way at a time, and a
+// G lanes to a row (kG where the launch knows them); a token's rows go round `share` groups, kRows of them on their way at a time, and a
 // block's pass takes a.per tokens.
-template <class T, class W, int V, int NC, Pairing kP, bool kBack>
+template <class T, class W, int V, int NC, Pairing kP, int kG, bool kBack>
 __global__ void __launch_bounds__(kThreads, NC == 1 ? 3 : 1)
-    rotary_kernel(const __grid_constant__ Args a, int G, int share) {
+    rotary_kernel(const __grid_constant__ Args a, int lanes, int share) {
+  const int G = kG ? kG : lanes;
   constexpr int kRows = NC > 2 ? 1 : kBack ? 2 : 4;
   extern __shared__ __align__(16) float sm[];
   float* cs = sm;                                 // [per][2 half]
   float* rows = sm + a.per * 2 * a.half;          // [groups][D] staging rows
   __shared__ int64_t s_off[kMaxTokens][6];        // element offsets of a token in q, k, yq, yk, gq, gk
-  __shared__ double s_pos[kMaxTokens];
+  __shared__ int64_t s_pos[kMaxTokens];
+  __shared__ uint64_t s_freq[kMaxDim / 2];        // turns a position, in 2^-64
   const int lane = threadIdx.x % G, group = threadIdx.x / G, groups = kThreads / G;
   float* row = rows + group * a.D;
   const unsigned mask = G == 32 ? ~0u : ((1u << G) - 1u) << ((threadIdx.x & 31) / G * G);
@@ -206,6 +208,11 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 3 : 1)
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (kBack) dw[0][c][i] = dw[kBack ? 1 : 0][c][i] = 0.f;
+  for (int i = threadIdx.x; i < a.half; i += kThreads) {
+    const double turns = a.freq[i] * 0.15915494309189535;
+    const double part = turns - floor(turns);
+    s_freq[i] = (uint64_t)(part * 0x1p32) << 32 | (uint64_t)(uint32_t)((part * 0x1p32 - floor(part * 0x1p32)) * 0x1p32);
+  }
   const float inv = 1.f / (float)a.D;
   for (int64_t t0 = (int64_t)blockIdx.x * a.per; t0 < a.tokens; t0 += (int64_t)gridDim.x * a.per) {
     const int n = (int)min((int64_t)a.per, a.tokens - t0);
@@ -213,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 3 : 1)
     if (threadIdx.x < n) {
       const int64_t t = t0 + threadIdx.x;
       const int64_t b = a.tokens >> 31 ? t / a.steps : (int64_t)((unsigned)t / (unsigned)a.steps), st = t - b * a.steps;
-      s_pos[threadIdx.x] = a.half ? (double)a.pos[b * a.pos_batch + st * a.pos_step] : 0.0;
+      s_pos[threadIdx.x] = a.half ? a.pos[b * a.pos_batch + st * a.pos_step] : 0;
       int64_t* f = s_off[threadIdx.x];
       f[0] = b * a.q.batch + st * a.q.step;
       f[1] = b * a.k.batch + st * a.k.step;
@@ -248,10 +255,10 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 3 : 1)
     fetch(0, first);  // on their way while the angles are formed
     for (int e = threadIdx.x; e < n * a.half; e += kThreads) {
       const int u = (unsigned)e / (unsigned)a.half, i = e - u * a.half;
-      // in turns, so that the whole ones drop out exactly before the 32-bit functions
-      const double ang = s_pos[u] * a.freq[i] * 0.15915494309189535;
+      // the product's whole turns leave a 64-bit word by themselves; what stays, in half turns
+      const int32_t turn = (int32_t)((uint64_t)s_pos[u] * s_freq[i] >> 32);
       float s, c;
-      sincospif((float)(2.0 * (ang - rint(ang))), &s, &c);
+      sincospif((float)turn * 0x1p-31f, &s, &c);
       cs[u * 2 * a.half + i] = c;
       cs[u * 2 * a.half + a.half + i] = s;
     }
@@ -283,19 +290,33 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 3 : 1)
       if (which) fetch(1, first);
       for (int h0 = 0; h0 < H; h0 += kRows * share) {
         if (h0) fetch(which, h0 + first);
+        float rss[kRows];
+        if constexpr (kP != kStaged) {
+          // the rows' sums side by side: their shuffles do not wait for one another
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) {
+            uint64_t x[N], sq = 0;
+            nx[r][0].get(x);
+#pragma unroll
+            for (int i = 0; i < N; ++i) sq = fma2(x[i], x[i], sq);
+            rss[r] = low(sq) + high(sq);
+          }
+#pragma unroll
+          for (int o = G >> 1; o > 0; o >>= 1)
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) rss[r] += __shfl_xor_sync(mask, rss[r], o);
+#pragma unroll
+          for (int r = 0; r < kRows; ++r) rss[r] = rsqrtf(rss[r] * inv + a.eps);
+        }
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
           const int h = h0 + r * share + first;
           const bool on = mine && h < H;
           if constexpr (kP != kStaged) {
             const int d = lane * V;
-            uint64_t x[N], sq = 0;
+            uint64_t x[N];
             nx[r][0].get(x);
-#pragma unroll
-            for (int i = 0; i < N; ++i) sq = fma2(x[i], x[i], sq);
-            float ss = low(sq) + high(sq);
-            for (int o = G >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-            const float rs = rsqrtf(ss * inv + a.eps);
+            const float rs = rss[r];
             const uint64_t rr = pair(rs, rs);
             if constexpr (!kBack) {
               // the weights before the exchange: the partner's own
@@ -335,6 +356,7 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 3 : 1)
                 g[i] = mul2(g[i], ww);
               }
               float m = low(m2) + high(m2);
+#pragma unroll
               for (int o = G >> 1; o > 0; o >>= 1) m += __shfl_xor_sync(mask, m, o);
               // dx = r (u - x r^2 mean(u x))
               m *= inv * rs * rs;
@@ -463,10 +485,10 @@ int launch(const Call& c, int blocks, cudaStream_t s) {
   const Args& a = c.a;
   const int V = c.vec ? 16 / (int)sizeof(T) : 1;
   const int nc = ceil_div(ceil_div(a.D, V), c.G);
-  auto go = [&](auto vv, auto cc, auto pp) -> int {
+  auto go = [&](auto vv, auto cc, auto pp, auto gg) -> int {
     constexpr int VV = decltype(vv)::value, CC = decltype(cc)::value;
     constexpr Pairing kP = decltype(pp)::value;
-    auto kernel = rotary_kernel<T, W, VV, CC, kP, kBack>;
+    auto kernel = rotary_kernel<T, W, VV, CC, kP, decltype(gg)::value, kBack>;
     const bool staged = kP == kStaged || kBack;
     const size_t smem = ((size_t)a.per * 2 * a.half + (staged ? (size_t)(kThreads / c.G) * a.D : 0)) * 4;
     if (smem > 48 * 1024)
@@ -481,13 +503,18 @@ int launch(const Call& c, int blocks, cudaStream_t s) {
   using Staged = std::integral_constant<Pairing, kStaged>;
   using Vec = std::integral_constant<int, VT>;
   using One = std::integral_constant<int, 1>;
-  if (c.vec && nc == 1) {
-    if (a.interleaved) return go(Vec{}, One{}, Neighbours{});
-    if (a.half % VT == 0) return go(Vec{}, One{}, Lanes{});
-    return go(Vec{}, One{}, Staged{});
+  using Any = std::integral_constant<int, 0>;
+  if (c.vec && nc == 1 && c.G >= 8 && (a.interleaved || a.half % VT == 0)) {
+    // rows of 8, 16 or 32 lanes (bf16: 64, 128, 256 features) know their reductions' depth
+    auto wide = [&](auto pp) -> int {
+      if (c.G == 8) return go(Vec{}, One{}, pp, std::integral_constant<int, 8>{});
+      if (c.G == 16) return go(Vec{}, One{}, pp, std::integral_constant<int, 16>{});
+      return go(Vec{}, One{}, pp, std::integral_constant<int, 32>{});
+    };
+    return a.interleaved ? wide(Neighbours{}) : wide(Lanes{});
   }
-  if (c.vec) return go(Vec{}, std::integral_constant<int, 2>{}, Staged{});
-  return go(One{}, std::integral_constant<int, kMaxDim / 32>{}, Staged{});
+  if (c.vec) return go(Vec{}, std::integral_constant<int, 2>{}, Staged{}, Any{});
+  return go(One{}, std::integral_constant<int, kMaxDim / 32>{}, Staged{}, Any{});
 }
 
 template <bool kBack>
