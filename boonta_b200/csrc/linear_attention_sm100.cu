@@ -116,6 +116,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// One lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // The bits lo .. hi of a word (positions outside 0 .. 31 allowed).
 __device__ __forceinline__ unsigned bits(int lo, int hi) {
   const unsigned from = lo <= 0 ? ~0u : lo > 31 ? 0u : ~0u << lo;
@@ -159,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int batch = bh / o.heads, head = bh % o.heads;
   const int split = blockIdx.y;
   const int begin = split * o.split_len, end = min(o.steps, begin + o.split_len);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
   const int na = min(F::kNA, ceil_div(o.Da, 64));
   const uint32_t base = smem_u32(smem);
 
@@ -254,62 +261,81 @@ __global__ void __launch_bounds__(kThreads, 2)
   };
 
   if (warp == 8) {
-    if (lane == 0) {
-      uint32_t parity = 0;
-      for (int i0 = begin; i0 < end; i0 += kC, parity ^= 1) {
-        wait(full, parity);
-        if (kOut) {
-          wait(has_s, parity);
-          if (*s_fail) break;
+    // Descriptors of the tiles; a step along the contraction adds to the address field (16-byte units).
+    const uint64_t da = smem_desc(base + F::kA, 16, 1024), db = smem_desc(base + F::kB, 16, 1024);
+    const uint64_t ds = smem_desc(base + F::kS, 8192, 1024), dc = smem_desc(base + F::kCc, 8192, 1024);
+    // b by columns: the second 64 rows of a 64-wide b are its first ones again
+    const uint64_t dbt = smem_desc(base + F::kB, na == 2 ? kBlock : 0, 1024);
+    const uint64_t dp[3] = {smem_desc(base + F::plane(0), 8192, 1024), smem_desc(base + F::plane(1), 8192, 1024),
+                            smem_desc(base + F::plane(2), 8192, 1024)};
+    const bool leader = elect_one();
+    uint32_t parity = 0;
+    for (int i0 = begin; i0 < end; i0 += kC, parity ^= 1) {
+      wait(full, parity);
+      if (kOut) {
+        wait(has_s, parity);
+        if (*s_fail) break;
+        if (leader) {
 #pragma unroll
-          for (int x = 0; x < DA / 16; ++x) {
-            if (x >= na * 4) break;
-            const uint32_t off = (x >> 2) * kBlock + (x & 3) * 32;
-            mma_bf16(tmem, smem_desc(base + F::kA + off, 16, 1024), smem_desc(base + F::kB + off, 16, 1024),
-                     idesc<false, false, 128>(), x > 0);
-          }
+          for (int x = 0; x < DA / 16; ++x)
+            if (x < 4 || na == 2) {
+              const uint64_t off = ((x >> 2) * kBlock + (x & 3) * 32) >> 4;
+              mma_bf16(tmem, da + off, db + off, idesc<false, false, 128>(), x > 0);
+            }
 #pragma unroll
-          for (int x = 0; x < DA / 16; ++x) {
-            if (x >= na * 4) break;
-            const uint32_t off = (x >> 2) * kBlock + (x & 3) * 32;
-            mma_bf16(tmem + kOCol, smem_desc(base + F::kA + off, 16, 1024),
-                     smem_desc(base + F::kS + x * 2048, 8192, 1024), idesc<false, true, 64>(), x > 0);
-          }
+          for (int x = 0; x < DA / 16; ++x)
+            if (x < 4 || na == 2) {
+              const uint64_t off = ((x >> 2) * kBlock + (x & 3) * 32) >> 4;
+              mma_bf16(tmem + kOCol, da + off, ds + (x * 2048 >> 4), idesc<false, true, 64>(), x > 0);
+            }
           mma_commit(done_a);
         }
-        wait(has_w, parity);
-        if (*s_fail) break;
+        __syncwarp();
+      }
+      wait(has_w, parity);
+      if (*s_fail) break;
+      if (leader) {
 #pragma unroll
         for (int q = 2; q >= 0; --q)  // smallest first
 #pragma unroll
           for (int x = 0; x < kC / 16; ++x)
-            // the second 64 rows of a 64-wide b are its first ones again
-            mma_bf16(tmem + kLCol, smem_desc(base + F::kB + x * 2048, na == 2 ? kBlock : 0, 1024),
-                     smem_desc(base + F::plane(q) + x * 2048, 8192, 1024), idesc<true, true, 64>(), q < 2 || x > 0);
+            mma_bf16(tmem + kLCol, dbt + (x * 2048 >> 4), dp[q] + (x * 2048 >> 4), idesc<true, true, 64>(), q < 2 || x > 0);
         mma_commit(done_l);
-        if (kOut) {
-          wait(has_p, parity);
-          if (*s_fail) break;
-          for (int q = weak ? 1 : 0; q >= 0; --q) {
-            const uint32_t b = base + (weak ? F::plane(q) : F::kCc);
+      }
+      __syncwarp();
+      if (kOut) {
+        wait(has_p, parity);
+        if (*s_fail) break;
+        if (leader) {
+          if (weak) {
+#pragma unroll
+            for (int q = 1; q >= 0; --q)
+#pragma unroll
+              for (int x = 0; x < kC / 16; ++x)
+                mma_bf16_ts(tmem + kOCol, tmem + (x >> 2) * 64 + (x & 3) * 8, dp[q] + (x * 2048 >> 4),
+                            idesc<false, true, 64>(), 1);
+          } else {
 #pragma unroll
             for (int x = 0; x < kC / 16; ++x)
-              mma_bf16_ts(tmem + kOCol, tmem + (x >> 2) * 64 + (x & 3) * 8, smem_desc(b + x * 2048, 8192, 1024), idesc<false, true, 64>(), 1);
+              mma_bf16_ts(tmem + kOCol, tmem + (x >> 2) * 64 + (x & 3) * 8, dc + (x * 2048 >> 4),
+                          idesc<false, true, 64>(), 1);
           }
           mma_commit(done_o);
-          wait(done_o, parity);
         }
-        wait(done_l, parity);
-        if (*s_fail) break;
-        if (i0 + kC < end) load(i0 + kC);
+        __syncwarp();
+        wait(done_o, parity);
       }
-      if (*s_fail) {
-        // let copies and MMAs in flight end before the block's memory goes
-        mbar_wait_bounded(full, parity);
-        mbar_wait_bounded(done_a, parity);
-        mbar_wait_bounded(done_l, parity);
-        mbar_wait_bounded(done_o, parity);
-      }
+      wait(done_l, parity);
+      if (*s_fail) break;
+      if (leader && i0 + kC < end) load(i0 + kC);
+      __syncwarp();
+    }
+    if (*s_fail) {
+      // let copies and MMAs in flight end before the block's memory goes
+      mbar_wait_bounded(full, parity);
+      mbar_wait_bounded(done_a, parity);
+      mbar_wait_bounded(done_l, parity);
+      mbar_wait_bounded(done_o, parity);
     }
   } else {
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
