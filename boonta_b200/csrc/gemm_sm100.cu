@@ -50,7 +50,7 @@ int encode_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t oute
 }
 
 int encode_map_4d(CUtensorMap* map, const void* base, const uint64_t dims[4], const uint64_t strides[3],
-                  const uint32_t box[4]) {
+                  const uint32_t box[4], int swizzle_bytes) {
   BT_TRY(resolve_encode());
   cuuint64_t d[4], st[3];
   cuuint32_t b[4], estr[4] = {1, 1, 1, 1};
@@ -58,7 +58,8 @@ int encode_map_4d(CUtensorMap* map, const void* base, const uint64_t dims[4], co
   // a dimension of one element is never stepped along, so any stride does
   for (int i = 0; i < 3; ++i) st[i] = dims[i + 1] > 1 ? strides[i] : 16;
   const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, st, b, estr,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed (%d): dims %llu x %llu x %llu x %llu, strides %llu %llu %llu", (int)r,

@@ -919,9 +919,9 @@ struct EpiDw {
 int encode_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
                uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer);
 
-// 4-D bf16 tensor map with 128-byte swizzle (strides in bytes, of dimensions 1 to 3).
+// 4-D bf16 tensor map with 128- or 64-byte swizzle (strides in bytes, of dimensions 1 to 3).
 int encode_map_4d(CUtensorMap* map, const void* base, const uint64_t dims[4], const uint64_t strides[3],
-                  const uint32_t box[4]);
+                  const uint32_t box[4], int swizzle_bytes);
 
 // Epilogue tile map: 32 x 32 box over a row-major [outer, inner] fp32 (128-byte swizzle) or
 // bf16 (64-byte swizzle) tensor with row stride `row_bytes`.

@@ -341,18 +341,24 @@ int run_ops(Ops& ops, cudaStream_t stream) {
   return go(std::integral_constant<int, 128>{});
 }
 
-// Splits of the steps: the number whose launches fill the GPU best, a walk over all splits counted
-// as two blocks an SM, and the sums of the splits (two of the four streams of a full walk, and a launch)
-// as two fifths more. At least four of the tensor cores' chunks each.
+// Splits of the steps: the number whose launches are the shortest, in units of the walk over 128 steps. Two
+// blocks share an SM (one alone is faster by about a third); a sequence costs a third of a unit to begin,
+// the sums of the splits half of a full walk, and the two more launches about two units.
 void choose_splits(const bt_linear_attention_shape* s, int ops, int* nsplit, int* len) {
   const int64_t blocks = (int64_t)s->batch * s->heads * ceil_div(max(s->key_dim, s->value_dim), kDS) * ops;
-  int best = 1;
+  const int chunks = max(1, ceil_div(s->steps, 128));
+  int best = chunks;
   double least = 1e300;
-  for (int n = 1; n <= 32 && n <= max(1, s->steps / 512); ++n) {
-    const double t = (double)ceil_div64(blocks * n, 2 * kNumSMs) / n * (n > 1 ? 1.4 : 1.0);
-    if (t < least) least = t, best = n;
+  for (int n = 1; n <= 64 && n <= chunks; ++n) {
+    const int each = ceil_div(chunks, n), have = ceil_div(chunks, each);
+    auto walk = [&](int64_t items, double unit) {
+      const double shared = items <= kNumSMs ? 0.65 : 1.0;
+      return (double)ceil_div64(items, 2 * kNumSMs) * (each * unit + 0.33) * shared;
+    };
+    const double t = walk(blocks * have, 1.0) + (have > 1 ? walk(blocks * (have - 1), 0.5) + 2.0 : 0.0);
+    if (t < least) least = t, best = each;
   }
-  *len = max(128, ceil_div(ceil_div(s->steps, best), 128) * 128);
+  *len = best * 128;
   *nsplit = max(1, ceil_div(s->steps, *len));
 }
 

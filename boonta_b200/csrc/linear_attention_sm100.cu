@@ -1,8 +1,8 @@
 // Linear attention with a decay per head on the tensor cores (tcgen05), bf16 inputs (the operation:
 // linear_attention.cuh).
 //
-// A block owns one (batch row, head), 64 columns of c and of the state, and walks its positions 128 at
-// a time. In a chunk, with p the position of a row, w_j = in_scale e^{(n - 1 - p_j) g}, and everything
+// A block takes one (batch row, head) and 64 columns of c and of the state after the other, and walks its
+// positions 128 at a time. In a chunk, with p the position of a row, w_j = in_scale e^{(n - 1 - p_j) g}, and everything
 // accumulated in fp32:
 //   P0 = a b^T                                     [128 x 128]  tensor memory
 //   O  = a S                                       [128 x 64]   S: bf16 copy of the state in shared memory
@@ -70,7 +70,7 @@ struct Cfg {
 static_assert(2 * (Cfg<128>::kBytes + 1024) <= 228 * 1024, "two blocks on an SM");
 
 struct Maps {
-  CUtensorMap a[3], b[3], c[3];
+  CUtensorMap a[3], b[3], c[3], out[3];
 };
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int t, int h, int b,
@@ -81,6 +81,20 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(t), "r"(h), "r"(b), "r"(smem_u32(bar))
       : "memory");
 }
+
+__device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* map, int x, int t, int h, int b) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(t), "r"(h), "r"(b)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int x, int t, int h, int b) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(t), "r"(h), "r"(b), "r"(smem_u32(src))
+               : "memory");
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // D (tensor memory) += A (tensor memory, two K elements a column) B (shared memory).
 __device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
@@ -135,8 +149,20 @@ __device__ __forceinline__ constexpr uint32_t idesc() {
   return umma::instr_desc<N, A_MN, B_MN>();
 }
 
-// The eight worker warps (named barrier 1).
+// The eight worker warps (named barrier 1), and the two of them that share 32 rows (2 to 5).
 __device__ __forceinline__ void sync_workers() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void sync_pair(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory"); }
+
+// A sequence of the launch: one (batch row, head) and 64 columns of c.
+struct Seq {
+  int batch, head, d0;
+  __device__ Seq(const Op& o, int w) {
+    const int slices = ceil_div(o.Dc, kDS), per = o.heads * slices;
+    batch = w / per;
+    head = w % per / slices;
+    d0 = w % slices * kDS;
+  }
+};
 
 // kOut: outputs, from the state that enters the split; else the split's own sum.
 template <int DA, bool kOut>
@@ -156,28 +182,46 @@ __global__ void __launch_bounds__(kThreads, 2)
   unsigned* s_cut = reinterpret_cast<unsigned*>(pl + 4);  // [2][4] the cuts of a chunk, a bit a position
 
   const Op& o = ops.op[blockIdx.z];
-  const int slices = ceil_div(o.Dc, kDS);
-  if ((int)blockIdx.x >= o.batch * o.heads * slices) return;
+  const int total = o.batch * o.heads * ceil_div(o.Dc, kDS), stride = gridDim.x;
+  if ((int)blockIdx.x >= total) return;
   if (smem_u32(smem) & 1023) {  // the swizzled tiles count on it
     if (threadIdx.x == 0) atomicExch(err, kErrAlignment);
     return;
   }
-  const int bh = blockIdx.x / slices, d0 = blockIdx.x % slices * kDS;
-  const int batch = bh / o.heads, head = bh % o.heads;
   const int split = blockIdx.y;
   const int begin = split * o.split_len, end = min(o.steps, begin + o.split_len);
   const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
   const int na = min(F::kNA, ceil_div(o.Da, 64));
   const uint32_t base = smem_u32(smem);
+  const bool reverse = o.reverse;
 
-  auto load = [&](int i0) {
-    const int t0 = o.reverse ? o.steps - i0 - kC : i0;
+  auto time_of = [&](int i0) { return reverse ? o.steps - i0 - kC : i0; };
+  auto load = [&](const Seq& q, int i0) {
+    const int t0 = time_of(i0);
     mbar_arrive_expect_tx(full, ((kOut ? 2 : 1) * na + 1) * kBlock);
-    tma_load_4d(smem + F::kCc, &maps.c[blockIdx.z], d0, t0, head, batch, full);
+    tma_load_4d(smem + F::kCc, &maps.c[blockIdx.z], q.d0, t0, q.head, q.batch, full);
     for (int x = 0; x < na; ++x) {
-      if (kOut) tma_load_4d(smem + F::kA + x * kBlock, &maps.a[blockIdx.z], 64 * x, t0, head, batch, full);
-      tma_load_4d(smem + F::kB + x * kBlock, &maps.b[blockIdx.z], 64 * x, t0, head, batch, full);
+      if (kOut) tma_load_4d(smem + F::kA + x * kBlock, &maps.a[blockIdx.z], 64 * x, t0, q.head, q.batch, full);
+      tma_load_4d(smem + F::kB + x * kBlock, &maps.b[blockIdx.z], 64 * x, t0, q.head, q.batch, full);
     }
+  };
+  // towards L2, a chunk ahead of its load
+  auto prefetch = [&](const Seq& q, int i0) {
+    const int t0 = time_of(i0);
+    tma_prefetch_4d(&maps.c[blockIdx.z], q.d0, t0, q.head, q.batch);
+    for (int x = 0; x < na; ++x) {
+      if (kOut) tma_prefetch_4d(&maps.a[blockIdx.z], 64 * x, t0, q.head, q.batch);
+      tma_prefetch_4d(&maps.b[blockIdx.z], 64 * x, t0, q.head, q.batch);
+    }
+  };
+  // the chunk after (w, i0) in this block's walk
+  auto advance = [&](int& w, int& i0) {
+    i0 += kC;
+    if (i0 >= end) {
+      i0 = begin;
+      w += stride;
+    }
+    return w < total;
   };
   if (warp == 8) {
     if (lane == 0) {
@@ -185,71 +229,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int i = 0; i < 4; ++i) mbar_init(bars + i, 1);
       for (int i = 4; i < 7; ++i) mbar_init(bars + i, kWorkers / 32);
       fence_mbar_init();
-      if (begin < end) load(begin);
+      int w = blockIdx.x, i0 = begin;
+      load(Seq(o, w), i0);
+      if (advance(w, i0)) prefetch(Seq(o, w), i0);
     }
     __syncwarp();
     umma::tmem_alloc(tmem_slot, kCols);
   }
-  const float g = fmaxf(o.log_decay[head], kMinLogDecay);
-  const bool weak = g >= kWeakDecay;
-  if (tid <= kC) pw[tid] = (float)exp((double)tid * (double)g);
-  if (tid >= kWorkers && tid < kWorkers + 4) {
-    const int last = max(1, end - begin) - (max(1, end - begin) - 1) / kC * kC;
-    const int x = tid - kWorkers;
-    const double e = exp((double)(x == 0 ? kC - 1 : x == 1 ? kC : x == 2 ? last : last - 1) * (double)g);
-    pl[x] = (float)(e - (double)(float)e);
-  }
-
-  const int row = (warp & 3) * 32 + lane, half = warp >> 2;  // tensor memory lane, column half
-  const size_t elems = (size_t)o.Da * o.Dc;
-  // A worker's piece of the state: row k, columns y0 .. (the rows of L repeat where Da <= 64, and the
-  // second copy takes the other half of the columns).
-  constexpr int kSC = DA == 128 ? 32 : 16;
-  const int k = DA == 128 ? row : row & 63;
-  const int y0 = DA == 128 ? half * 32 : (row >> 6) * 32 + half * 16;
-  float s[kSC];
-  auto put_state = [&]() {
-#pragma unroll
-    for (int i = 0; i < kSC; i += 8) {
-      uint32_t w[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) w[u] = pack_bf16(s[i + 2 * u], s[i + 2 * u + 1]);
-      *reinterpret_cast<uint4*>(smem + F::kS + k * 128 + ((((y0 + i) >> 3) ^ (k & 7)) << 4)) =
-          make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  };
-  bool cut = false;  // of position tid of the coming chunk
-  if (warp < 8) {
-    if (tid < kC && begin + tid < end) cut = op_cut(o, batch, begin + tid);
-    const float* from = nullptr;
-    int64_t sx = o.sx, sy = o.sy;
-    if (kOut) {
-      if (split > 0) {
-        from = o.local + ((size_t)(split - 1) * o.batch * o.heads + bh) * elems;
-        sx = o.Dc;
-        sy = 1;
-      } else if (o.init) {
-        from = o.init + bh * elems;
-      }
-    }
-    const bool whole = from && sy == 1 && o.Dc % 4 == 0 && ((uintptr_t)from & 15) == 0;
-#pragma unroll
-    for (int i = 0; i < kSC; i += 4) {
-      const int y = d0 + y0 + i;
-      if (whole) {
-        const float4 f = k < o.Da && y < o.Dc ? *reinterpret_cast<const float4*>(from + k * sx + y)
-                                              : make_float4(0.f, 0.f, 0.f, 0.f);
-        s[i] = f.x, s[i + 1] = f.y, s[i + 2] = f.z, s[i + 3] = f.w;
-      } else {
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          s[i + u] = from && k < o.Da && y + u < o.Dc ? from[k * sx + (y + u) * sy] : 0.f;
-      }
-    }
-    if (kOut && !weak) put_state();
-  }
-  fence_proxy_async_smem();
-  fence_before_sync();
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = *tmem_slot;
@@ -259,6 +245,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (!mbar_wait_bounded(bar, parity)) *s_fail = 1;
     fence_after_sync();
   };
+  auto decay_of = [&](int head) { return fmaxf(o.log_decay[head], kMinLogDecay); };
 
   if (warp == 8) {
     // Descriptors of the tiles; a step along the contraction adds to the address field (16-byte units).
@@ -270,7 +257,9 @@ __global__ void __launch_bounds__(kThreads, 2)
                             smem_desc(base + F::plane(2), 8192, 1024)};
     const bool leader = elect_one();
     uint32_t parity = 0;
-    for (int i0 = begin; i0 < end; i0 += kC, parity ^= 1) {
+    int w = blockIdx.x, i0 = begin, head = Seq(o, w).head;
+    bool weak = decay_of(head) >= kWeakDecay;
+    for (bool more = true; more; parity ^= 1) {
       wait(full, parity);
       if (kOut) {
         wait(has_s, parity);
@@ -327,8 +316,19 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       wait(done_l, parity);
       if (*s_fail) break;
-      if (leader && i0 + kC < end) load(i0 + kC);
+      more = advance(w, i0);
+      if (!more) break;
+      const Seq q(o, w);
+      if (leader) {
+        load(q, i0);
+        int w2 = w, i2 = i0;
+        if (advance(w2, i2)) prefetch(Seq(o, w2), i2);
+      }
       __syncwarp();
+      if (q.head != head) {
+        head = q.head;
+        weak = decay_of(head) >= kWeakDecay;
+      }
     }
     if (*s_fail) {
       // let copies and MMAs in flight end before the block's memory goes
@@ -338,214 +338,309 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_wait_bounded(done_o, parity);
     }
   } else {
+    const int row = (warp & 3) * 32 + lane, half = warp >> 2;  // tensor memory lane, column half
+    const size_t elems = (size_t)o.Da * o.Dc;
+    // A worker's piece of the state: row k, columns y0 .. (the rows of L repeat where Da <= 64, and the
+    // second copy takes the other half of the columns).
+    constexpr int kSC = DA == 128 ? 32 : 16;
+    const int k = DA == 128 ? row : row & 63;
+    const int y0 = DA == 128 ? half * 32 : (row >> 6) * 32 + half * 16;
+    float s[kSC];
+    auto put_state = [&]() {
+#pragma unroll
+      for (int i = 0; i < kSC; i += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u] = pack_bf16(s[i + 2 * u], s[i + 2 * u + 1]);
+        *reinterpret_cast<uint4*>(smem + F::kS + k * 128 + ((((y0 + i) >> 3) ^ (k & 7)) << 4)) =
+            make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    };
+    // where a sequence's entering state lies (null: zeros), and by which strides
+    const bool local = kOut && split > 0;
+    const int64_t sx = local ? o.Dc : o.sx, sy = local ? 1 : o.sy;
+    auto state_in = [&](const Seq& q) -> const float* {
+      if (!kOut) return nullptr;
+      const int bh = q.batch * o.heads + q.head;
+      if (local) return o.local + ((size_t)(split - 1) * o.batch * o.heads + bh) * elems;
+      return o.init ? o.init + bh * elems : nullptr;
+    };
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const int p = o.reverse ? kC - 1 - row : row;  // the position of this thread's row
+    uint8_t* stage = smem + F::kP2 + (warp & 3) * 4096 + half * 2048;  // in plane rows of this warp pair
+    const int p = reverse ? kC - 1 - row : row;  // the position of this thread's row
     const float in_scale = o.in_scale;
-    const bool reverse = o.reverse, resets = o.reset != nullptr;
-    bool any_cut = false;
-    int e0 = (reverse && split == 0) ? 0 : 1;
+    const bool resets = o.reset != nullptr;
     uint32_t parity = 0;
+    int head = -1;
+    bool weak = true;
+    bool cut = resets && tid < kC && begin + tid < end && op_cut(o, Seq(o, blockIdx.x).batch, begin + tid);
     auto arrive = [&](uint64_t* bar) {
+      fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    // s takes its decay over the n positions to come, and its copy goes where O's product reads it. The
-    // factor in two parts: its rounding, met once a chunk, would add up over a long memory.
-    auto hand_state = [&](int n) {
-      if (kOut && !weak) put_state();
-      const float keep = pw[n - 1 + e0], keep_lo = pl[n == kC ? e0 : 3 - e0];
-#pragma unroll
-      for (int i = 0; i < kSC; ++i) s[i] = fmaf(keep, s[i], keep_lo * s[i]);
-      if (kOut && weak) put_state();
-      fence_proxy_async_smem();
-    };
-    if (begin < end) hand_state(min(kC, end - begin));
-    if (kOut) arrive(has_s);
 
-    for (int i0 = begin; i0 < end; i0 += kC, parity ^= 1) {
-      const int n = min(kC, end - i0);
-      // the last cut of the chunk, and the last one at or before p (-1: none)
-      int last = -1, lo = -1;
-      if (resets) {
-        unsigned* cuts = s_cut + 4 * parity;
-        if (tid < kC) {
-          const unsigned m = __ballot_sync(~0u, cut);
-          if (lane == 0) cuts[warp] = m;
-          cut = i0 + kC + tid < end && op_cut(o, batch, i0 + kC + tid);
-        }
-        sync_workers();
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const unsigned m = cuts[w], own = m & bits(0, p - 32 * w);
-          if (m) last = 32 * w + 31 - __clz(m);
-          if (own) lo = 32 * w + 31 - __clz(own);
-        }
-        any_cut |= last >= 0;
-      }
-
-      wait(full, parity);
-      {  // w c: this thread's row, half of the columns; the planes that go into a's place wait for it
-        const float wf = p < n ? in_scale * pw[n - 1 - p] : 0.f;
-        const uint64_t w = pair(wf, wf);
-        uint4 held[F::kNA][4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int off = row * 128 + (((half * 4 + u) ^ (row & 7)) << 4);
-          const uint4 x = *reinterpret_cast<const uint4*>(smem + F::kCc + off);
-          const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-          uint32_t y[3][4];
-          // 24 bits cut into 8 + 8 + 8: each plane takes the leading bits, the rest is exact
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint64_t v = mul2(w, pair_of_bf16(xs[i]));
-#pragma unroll
-            for (int q = 0; q < 3; ++q) {
-              y[q][i] = __byte_perm((uint32_t)v, (uint32_t)(v >> 32), 0x7632);
-              if (q < 2) v = sub2(v, v & 0xffff0000ffff0000ull);
-            }
-          }
-#pragma unroll
-          for (int q = 0; q < 3; ++q) {
-            const uint4 z = make_uint4(y[q][0], y[q][1], y[q][2], y[q][3]);
-            if (q < F::kNA) held[q < F::kNA ? q : 0][u] = z;
-            else *reinterpret_cast<uint4*>(smem + F::plane(q) + off) = z;
-          }
-        }
-        if (kOut) wait(done_a, parity);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int off = row * 128 + (((half * 4 + u) ^ (row & 7)) << 4);
-#pragma unroll
-          for (int q = 0; q < F::kNA; ++q) *reinterpret_cast<uint4*>(smem + F::plane(q) + off) = held[q][u];
-        }
-        if (last > p) {  // what a cut hides has no part in L; P0 is done with its row of b
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int x = 0; x < F::kNA; ++x)
-              *reinterpret_cast<uint4*>(smem + F::kB + x * kBlock + row * 128 + (half * 4 + u) * 16) =
-                  make_uint4(0, 0, 0, 0);
-        }
-      }
-      fence_proxy_async_smem();
-      fence_before_sync();
-      arrive(has_w);
-      if (kOut) {
-        if (!weak || last >= 0) {
-          // the rows of a S by the decay since the state; a cut drops it whatever it holds
-          const float reach = lo >= 0 || p >= n ? 0.f : weak ? 1.f : pw[p + e0];
-          float v[32];
-          tmem_ld32(lanes + kOCol + 32 * half, v);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = reach != 0.f ? __float_as_uint(reach * v[16 * j + i]) : 0u;
-            tmem_st16(lanes + kOCol + 32 * half + 16 * j, w);
-          }
-        }
-        // P: this warp's 32 rows against the column blocks 2 half and 2 half + 1. It takes the place of
-        // the first of the two, which is read by then.
-        const int from = max(lo, 0);  // columns of positions from .. p count
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int blk = 2 * half + u;
-          const unsigned m = reverse ? bits(kC - 1 - 32 * blk - p, kC - 1 - 32 * blk - from)
-                                     : bits(from - 32 * blk, p - 32 * blk);
-          uint32_t pk[16];
-          if (__all_sync(~0u, m == 0)) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) pk[i] = 0;
-          } else {
-            float v[32];
-            tmem_ld32(lanes + 32 * blk, v);
-            if (!weak) {
-              // e^{(p_i - p_j) g}: only where the column comes no later than the row
-              const int gap0 = reverse ? 32 * blk - row : row - 32 * blk, dir = reverse ? 1 : -1;
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] *= in_scale * pw[max(0, gap0 + dir * i)];
-            }
-            if (!__all_sync(~0u, m == ~0u)) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = m >> i & 1 ? v[i] : 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) pk[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-          }
-          tmem_st16(lanes + 64 * half + 16 * u, pk);
-        }
-        tmem_wait_st();
-        fence_before_sync();
-        arrive(has_p);
-      }
-      wait(done_l, parity);
-      {
-        float l[kSC];
-        if constexpr (kSC == 32) tmem_ld32(lanes + kLCol + y0, l);
-        else tmem_ld16(lanes + kLCol + y0, l);
-#pragma unroll
-        for (int i = 0; i < kSC; ++i) s[i] = (last < 0 ? s[i] : 0.f) + l[i];
-      }
-      e0 = 1;
-      if (i0 + kC < end) hand_state(min(kC, end - i0 - kC));
-      if (kOut) {
-        wait(done_o, parity);
-        float v[32];
-        tmem_ld32(lanes + kOCol + 32 * half, v);
-        fence_before_sync();
-        arrive(has_s);
-        if (p < n) {
-          const int t = reverse ? o.steps - 1 - i0 - p : i0 + p;
-          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(o.out) + batch * o.out_batch +
-                               (int64_t)t * o.out_step + head * o.out_head + d0 + 32 * half;
-          const int left = o.Dc - d0 - 32 * half;
-          const float f = weak ? o.out_scale / pw[n - 1 - p] : o.out_scale;
-#pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            // Dc is a multiple of 8, as the rows' strides are
-            if (i < left)
-              *reinterpret_cast<uint4*>(out + i) =
-                  make_uint4(pack_bf16(f * v[i], f * v[i + 1]), pack_bf16(f * v[i + 2], f * v[i + 3]),
-                             pack_bf16(f * v[i + 4], f * v[i + 5]), pack_bf16(f * v[i + 6], f * v[i + 7]));
-        }
-      } else {
-        fence_before_sync();
-      }
-    }
-    float* to = nullptr;
-    int64_t sx = o.sx, sy = o.sy;
-    float way_out = 1.f;
-    if (kOut) {
-      if (o.fin && split == o.nsplit - 1) {
-        to = o.fin + bh * elems;
-        if (o.reverse && o.steps > 0) {
-          way_out = pw[1];
-          if (o.reset && o.reset[batch * o.reset_batch]) way_out = 0.f;
-        }
-      }
-    } else {
-      to = o.local + ((size_t)split * o.batch * o.heads + bh) * elems;
-      sx = o.Dc;
-      sy = 1;
-      if (tid == 0 && d0 == 0 && head == 0) o.cut[split * o.batch + batch] = any_cut;
-    }
-    if (to && k < o.Da) {
-      const bool whole = sy == 1 && o.Dc % 4 == 0 && ((uintptr_t)to & 15) == 0;
+    for (int w = blockIdx.x; w < total; w += stride) {
+      const Seq q(o, w);
+      const float* from = state_in(q);
+      const bool whole = sy == 1 && o.Dc % 4 == 0 && ((uintptr_t)from & 15) == 0;
 #pragma unroll
       for (int i = 0; i < kSC; i += 4) {
-        const int y = d0 + y0 + i;
-        float f[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) f[u] = way_out == 0.f ? 0.f : way_out * s[i + u];
-        if (whole) {
-          if (y < o.Dc) *reinterpret_cast<float4*>(to + k * sx + y) = make_float4(f[0], f[1], f[2], f[3]);
+        const int y = q.d0 + y0 + i;
+        if (from && whole) {
+          const float4 f = k < o.Da && y < o.Dc ? *reinterpret_cast<const float4*>(from + k * sx + y)
+                                                : make_float4(0.f, 0.f, 0.f, 0.f);
+          s[i] = f.x, s[i + 1] = f.y, s[i + 2] = f.z, s[i + 3] = f.w;
         } else {
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            if (y + u < o.Dc) to[k * sx + (y + u) * sy] = f[u];
+            s[i + u] = from && k < o.Da && y + u < o.Dc ? from[k * sx + (y + u) * sy] : 0.f;
+        }
+      }
+      if (q.head != head) {
+        head = q.head;
+        const float g = decay_of(head);
+        weak = g >= kWeakDecay;
+        sync_workers();  // nobody reads the last head's powers any more
+        if (tid <= kC) {
+          pw[tid] = (float)exp((double)tid * (double)g);
+        } else if (tid >= kWorkers - 4) {
+          const int last = end - begin - (end - begin - 1) / kC * kC;
+          const int x = tid - (kWorkers - 4);
+          const double e = exp((double)(x == 0 ? kC - 1 : x == 1 ? kC : x == 2 ? last : last - 1) * (double)g);
+          pl[x] = (float)(e - (double)(float)e);
+        }
+        sync_workers();
+      }
+      // the next sequence's state on its way to L2
+      if (kOut && w + stride < total) {
+        const Seq nq(o, w + stride);
+        const float* next = state_in(nq);
+        if (next && k < o.Da && nq.d0 + y0 < o.Dc) {
+          if (sy == 1) {
+#pragma unroll
+            for (int i = 0; i < kSC; i += 8) prefetch_l2(next + k * sx + nq.d0 + min(y0 + i, o.Dc - 1 - nq.d0));
+          } else if ((k & 7) == 0) {
+#pragma unroll
+            for (int i = 0; i < kSC; ++i) prefetch_l2(next + k * sx + min(nq.d0 + y0 + i, o.Dc - 1) * sy);
+          }
+        }
+      }
+      bool any_cut = false;
+      int e0 = (reverse && split == 0) ? 0 : 1;
+      // s takes its decay over the n positions to come, and its copy goes where O's product reads it. The
+      // factor in two parts: its rounding, met once a chunk, would add up over a long memory.
+      auto hand_state = [&](int n) {
+        if (kOut && !weak) put_state();
+        const float keep = pw[n - 1 + e0], keep_lo = pl[n == kC ? e0 : 3 - e0];
+#pragma unroll
+        for (int i = 0; i < kSC; ++i) s[i] = fmaf(keep, s[i], keep_lo * s[i]);
+        if (kOut && weak) put_state();
+        fence_proxy_async_smem();
+      };
+      hand_state(min(kC, end - begin));
+      if (kOut) arrive(has_s);
+
+      for (int i0 = begin; i0 < end; i0 += kC, parity ^= 1) {
+        const int n = min(kC, end - i0);
+        const bool ends = i0 + kC >= end;
+        // the last cut of the chunk, and the last one at or before p (-1: none)
+        int last = -1, lo = -1;
+        if (resets) {
+          unsigned* cuts = s_cut + 4 * parity;
+          if (tid < kC) {
+            const unsigned m = __ballot_sync(~0u, cut);
+            if (lane == 0) cuts[warp] = m;
+            const int nw = ends ? w + stride : w, ni = (ends ? begin : i0 + kC) + tid;
+            cut = nw < total && ni < end && op_cut(o, Seq(o, nw).batch, ni);
+          }
+          sync_workers();
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const unsigned m = cuts[x], own = m & bits(0, p - 32 * x);
+            if (m) last = 32 * x + 31 - __clz(m);
+            if (own) lo = 32 * x + 31 - __clz(own);
+          }
+          any_cut |= last >= 0;
+        }
+
+        wait(full, parity);
+        if (kOut) {
+          // the pair's last outputs have left their staging rows
+          if (lane == 0) umma::bulk_wait_read_all();
+          sync_pair(warp & 3);
+        }
+        {  // w c: this thread's row, half of the columns; the planes that go into a's place wait for it
+          const float wf = p < n ? in_scale * pw[n - 1 - p] : 0.f;
+          const uint64_t wp = pair(wf, wf);
+          uint4 held[F::kNA][4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int off = row * 128 + (((half * 4 + u) ^ (row & 7)) << 4);
+            const uint4 x = *reinterpret_cast<const uint4*>(smem + F::kCc + off);
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+            uint32_t y[3][4];
+            // 24 bits cut into 8 + 8 + 8: each plane takes the leading bits, the rest is exact
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint64_t v = mul2(wp, pair_of_bf16(xs[i]));
+#pragma unroll
+              for (int z = 0; z < 3; ++z) {
+                y[z][i] = __byte_perm((uint32_t)v, (uint32_t)(v >> 32), 0x7632);
+                if (z < 2) v = sub2(v, v & 0xffff0000ffff0000ull);
+              }
+            }
+#pragma unroll
+            for (int z = 0; z < 3; ++z) {
+              const uint4 t = make_uint4(y[z][0], y[z][1], y[z][2], y[z][3]);
+              if (z < F::kNA) held[z < F::kNA ? z : 0][u] = t;
+              else *reinterpret_cast<uint4*>(smem + F::plane(z) + off) = t;
+            }
+          }
+          if (kOut) wait(done_a, parity);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int off = row * 128 + (((half * 4 + u) ^ (row & 7)) << 4);
+#pragma unroll
+            for (int z = 0; z < F::kNA; ++z) *reinterpret_cast<uint4*>(smem + F::plane(z) + off) = held[z][u];
+          }
+          if (last > p) {  // what a cut hides has no part in L; P0 is done with its row of b
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+              for (int x = 0; x < F::kNA; ++x)
+                *reinterpret_cast<uint4*>(smem + F::kB + x * kBlock + row * 128 + (half * 4 + u) * 16) =
+                    make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async_smem();
+        arrive(has_w);
+        if (kOut) {
+          if (!weak || last >= 0) {
+            // the rows of a S by the decay since the state; a cut drops it whatever it holds
+            const float reach = lo >= 0 || p >= n ? 0.f : weak ? 1.f : pw[p + e0];
+            float v[32];
+            tmem_ld32(lanes + kOCol + 32 * half, v);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t x[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) x[i] = reach != 0.f ? __float_as_uint(reach * v[16 * j + i]) : 0u;
+              tmem_st16(lanes + kOCol + 32 * half + 16 * j, x);
+            }
+          }
+          // P: this warp's 32 rows against the column blocks 2 half and 2 half + 1. It takes the place of
+          // the first of the two, which is read by then.
+          const int first = max(lo, 0);  // columns of positions first .. p count
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int blk = 2 * half + u;
+            const unsigned m = reverse ? bits(kC - 1 - 32 * blk - p, kC - 1 - 32 * blk - first)
+                                       : bits(first - 32 * blk, p - 32 * blk);
+            uint32_t pk[16];
+            if (__all_sync(~0u, m == 0)) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pk[i] = 0;
+            } else {
+              float v[32];
+              tmem_ld32(lanes + 32 * blk, v);
+              if (!weak) {
+                // e^{(p_i - p_j) g}: only where the column comes no later than the row
+                const int gap0 = reverse ? 32 * blk - row : row - 32 * blk, dir = reverse ? 1 : -1;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] *= in_scale * pw[max(0, gap0 + dir * i)];
+              }
+              if (!__all_sync(~0u, m == ~0u)) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = m >> i & 1 ? v[i] : 0.f;
+              }
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pk[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+            }
+            tmem_st16(lanes + 64 * half + 16 * u, pk);
+          }
+          tmem_wait_st();
+          arrive(has_p);
+        }
+        wait(done_l, parity);
+        {
+          float l[kSC];
+          if constexpr (kSC == 32) tmem_ld32(lanes + kLCol + y0, l);
+          else tmem_ld16(lanes + kLCol + y0, l);
+#pragma unroll
+          for (int i = 0; i < kSC; ++i) s[i] = (last < 0 ? s[i] : 0.f) + l[i];
+        }
+        e0 = 1;
+        if (!ends) hand_state(min(kC, end - i0 - kC));
+        if (kOut) {
+          wait(done_o, parity);
+          float v[32];
+          tmem_ld32(lanes + kOCol + 32 * half, v);
+          if (!ends) arrive(has_s);
+          const float f = weak && p < n ? o.out_scale / pw[n - 1 - p] : o.out_scale;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] *= f;
+          const int t0 = time_of(i0), x0 = q.d0 + 32 * half;
+          if (t0 >= 0) {
+            // rows behind the last step and columns behind Dc fall away in the store
+            umma::stage_row_bf16(stage, nullptr, lane, v);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && x0 < o.Dc) {
+              tma_store_4d(&maps.out[blockIdx.z], stage, x0, t0 + 32 * (warp & 3), q.head, q.batch);
+              umma::bulk_commit();
+            }
+          } else if (p < n) {  // a first chunk in time that begins before step 0
+            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(o.out) + q.batch * o.out_batch +
+                                 (int64_t)(t0 + row) * o.out_step + q.head * o.out_head + x0;
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              // Dc is a multiple of 8, as the rows' strides are
+              if (x0 + i < o.Dc)
+                *reinterpret_cast<uint4*>(out + i) =
+                    make_uint4(pack_bf16(v[i], v[i + 1]), pack_bf16(v[i + 2], v[i + 3]),
+                               pack_bf16(v[i + 4], v[i + 5]), pack_bf16(v[i + 6], v[i + 7]));
+          }
+        }
+      }
+      const int bh = q.batch * o.heads + q.head;
+      float* to = nullptr;
+      int64_t tx = o.sx, ty = o.sy;
+      float way_out = 1.f;
+      if (kOut) {
+        if (o.fin && split == o.nsplit - 1) {
+          to = o.fin + bh * elems;
+          if (reverse) {
+            way_out = pw[1];
+            if (resets && o.reset[q.batch * o.reset_batch]) way_out = 0.f;
+          }
+        }
+      } else {
+        to = o.local + ((size_t)split * o.batch * o.heads + bh) * elems;
+        tx = o.Dc;
+        ty = 1;
+        if (tid == 0 && q.d0 == 0 && q.head == 0) o.cut[split * o.batch + q.batch] = any_cut;
+      }
+      if (to && k < o.Da) {
+        const bool vec = ty == 1 && o.Dc % 4 == 0 && ((uintptr_t)to & 15) == 0;
+#pragma unroll
+        for (int i = 0; i < kSC; i += 4) {
+          const int y = q.d0 + y0 + i;
+          float f[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) f[u] = way_out == 0.f ? 0.f : way_out * s[i + u];
+          if (vec) {
+            if (y < o.Dc) *reinterpret_cast<float4*>(to + k * tx + y) = make_float4(f[0], f[1], f[2], f[3]);
+          } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (y + u < o.Dc) to[k * tx + (y + u) * ty] = f[u];
+          }
         }
       }
     }
+    if (lane == 0) umma::bulk_wait_all();
+    __syncwarp();
   }
   fence_before_sync();
   __syncthreads();
@@ -560,7 +655,14 @@ int map_rows(CUtensorMap* m, const Op& o, const Rows& r, int d) {
   const uint64_t dims[4] = {(uint64_t)d, (uint64_t)o.steps, (uint64_t)o.heads, (uint64_t)o.batch};
   const uint64_t strides[3] = {(uint64_t)r.step * 2, (uint64_t)r.head * 2, (uint64_t)r.batch * 2};
   const uint32_t box[4] = {64, kC, 1, 1};
-  return umma::encode_map_4d(m, r.p, dims, strides, box);
+  return umma::encode_map_4d(m, r.p, dims, strides, box, 128);
+}
+
+int map_out(CUtensorMap* m, const Op& o) {
+  const uint64_t dims[4] = {(uint64_t)o.Dc, (uint64_t)o.steps, (uint64_t)o.heads, (uint64_t)o.batch};
+  const uint64_t strides[3] = {(uint64_t)o.out_step * 2, (uint64_t)o.out_head * 2, (uint64_t)o.out_batch * 2};
+  const uint32_t box[4] = {32, 32, 1, 1};
+  return umma::encode_map_4d(m, o.out, dims, strides, box, 64);
 }
 
 }  // namespace
@@ -576,14 +678,17 @@ bool suits_tensor_cores(const Op& o) {
 
 int run_tensor_cores(Ops& ops, cudaStream_t stream) {
   Maps maps;
-  int da = 0, blocks = 0;
+  int da = 0, blocks = 0, per = 1;
   for (int i = 0; i < ops.n; ++i) {
     const Op& o = ops.op[i];
+    const int slices = ceil_div(o.Dc, kDS);
     da = max(da, o.Da);
-    blocks = max(blocks, o.batch * o.heads * ceil_div(o.Dc, kDS));
+    blocks = max(blocks, o.batch * o.heads * slices);
+    per = max(per, o.heads * slices);
     BT_TRY(map_rows(&maps.a[i], o, o.a, o.Da));
     BT_TRY(map_rows(&maps.b[i], o, o.b, o.Da));
     BT_TRY(map_rows(&maps.c[i], o, o.c, o.Dc));
+    BT_TRY(map_out(&maps.out[i], o));
   }
   int* err = nullptr;
   BT_TRY(operator_error_word(&err));
@@ -594,13 +699,19 @@ int run_tensor_cores(Ops& ops, cudaStream_t stream) {
     auto outs = chunk_tc_kernel<DA, true>;
     constexpr int kSmem = Cfg<DA>::kBytes;
     BT_CUDA(cudaFuncSetAttribute(outs, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    // Two blocks an SM in all, each with every so many-th sequence: the same head again and again where the
+    // heads allow it (its powers are kept).
+    auto wide = [&](int splits) {
+      const int room = max(1, 2 * kNumSMs / (splits * ops.n));
+      return min(blocks, room > per ? room / per * per : room);
+    };
     if (o.nsplit > 1) {
       BT_CUDA(cudaFuncSetAttribute(sums, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-      sums<<<dim3(blocks, o.nsplit - 1, ops.n), kThreads, kSmem, stream>>>(ops, maps, err);
+      sums<<<dim3(wide(o.nsplit - 1), o.nsplit - 1, ops.n), kThreads, kSmem, stream>>>(ops, maps, err);
       BT_LAUNCH_CHECK("linear attention split sums");
       BT_TRY(launch_join(ops, stream));
     }
-    outs<<<dim3(blocks, o.nsplit, ops.n), kThreads, kSmem, stream>>>(ops, maps, err);
+    outs<<<dim3(wide(o.nsplit), o.nsplit, ops.n), kThreads, kSmem, stream>>>(ops, maps, err);
     BT_LAUNCH_CHECK("linear attention");
     return BT_OK;
   };
