@@ -153,15 +153,29 @@ __device__ __forceinline__ constexpr uint32_t idesc() {
 __device__ __forceinline__ void sync_workers() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ void sync_pair(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory"); }
 
-// A sequence of the launch: one (batch row, head) and 64 columns of c.
+// A sequence of the launch: one (batch row, head) and 64 columns of c (one or two slices of them). A block
+// takes every gridDim.x-th; the heads and slices of a batch row follow one another.
 struct Seq {
-  int batch, head, d0;
-  __device__ Seq(const Op& o, int w) {
-    const int slices = ceil_div(o.Dc, kDS), per = o.heads * slices;
+  int batch, at;  // at: head * slices + slice
+  int per, slices, by_batch, by_at;
+  __device__ Seq(const Op& o, int w, int stride) {
+    slices = o.Dc > kDS ? 2 : 1;
+    per = o.heads * slices;
     batch = w / per;
-    head = w % per / slices;
-    d0 = w % slices * kDS;
+    at = w - batch * per;
+    by_batch = stride / per;
+    by_at = stride - by_batch * per;
   }
+  __device__ __forceinline__ void advance() {
+    batch += by_batch;
+    at += by_at;
+    if (at >= per) {
+      at -= per;
+      ++batch;
+    }
+  }
+  __device__ __forceinline__ int head() const { return slices == 2 ? at >> 1 : at; }
+  __device__ __forceinline__ int d0() const { return slices == 2 ? (at & 1) * kDS : 0; }
 };
 
 // kOut: outputs, from the state that enters the split; else the split's own sum.
@@ -182,8 +196,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   unsigned* s_cut = reinterpret_cast<unsigned*>(pl + 4);  // [2][4] the cuts of a chunk, a bit a position
 
   const Op& o = ops.op[blockIdx.z];
-  const int total = o.batch * o.heads * ceil_div(o.Dc, kDS), stride = gridDim.x;
-  if ((int)blockIdx.x >= total) return;
+  if ((int)blockIdx.x >= o.batch * o.heads * ceil_div(o.Dc, kDS)) return;
   if (smem_u32(smem) & 1023) {  // the swizzled tiles count on it
     if (threadIdx.x == 0) atomicExch(err, kErrAlignment);
     return;
@@ -199,29 +212,29 @@ __global__ void __launch_bounds__(kThreads, 2)
   auto load = [&](const Seq& q, int i0) {
     const int t0 = time_of(i0);
     mbar_arrive_expect_tx(full, ((kOut ? 2 : 1) * na + 1) * kBlock);
-    tma_load_4d(smem + F::kCc, &maps.c[blockIdx.z], q.d0, t0, q.head, q.batch, full);
+    tma_load_4d(smem + F::kCc, &maps.c[blockIdx.z], q.d0(), t0, q.head(), q.batch, full);
     for (int x = 0; x < na; ++x) {
-      if (kOut) tma_load_4d(smem + F::kA + x * kBlock, &maps.a[blockIdx.z], 64 * x, t0, q.head, q.batch, full);
-      tma_load_4d(smem + F::kB + x * kBlock, &maps.b[blockIdx.z], 64 * x, t0, q.head, q.batch, full);
+      if (kOut) tma_load_4d(smem + F::kA + x * kBlock, &maps.a[blockIdx.z], 64 * x, t0, q.head(), q.batch, full);
+      tma_load_4d(smem + F::kB + x * kBlock, &maps.b[blockIdx.z], 64 * x, t0, q.head(), q.batch, full);
     }
   };
   // towards L2, a chunk ahead of its load
   auto prefetch = [&](const Seq& q, int i0) {
     const int t0 = time_of(i0);
-    tma_prefetch_4d(&maps.c[blockIdx.z], q.d0, t0, q.head, q.batch);
+    tma_prefetch_4d(&maps.c[blockIdx.z], q.d0(), t0, q.head(), q.batch);
     for (int x = 0; x < na; ++x) {
-      if (kOut) tma_prefetch_4d(&maps.a[blockIdx.z], 64 * x, t0, q.head, q.batch);
-      tma_prefetch_4d(&maps.b[blockIdx.z], 64 * x, t0, q.head, q.batch);
+      if (kOut) tma_prefetch_4d(&maps.a[blockIdx.z], 64 * x, t0, q.head(), q.batch);
+      tma_prefetch_4d(&maps.b[blockIdx.z], 64 * x, t0, q.head(), q.batch);
     }
   };
-  // the chunk after (w, i0) in this block's walk
-  auto advance = [&](int& w, int& i0) {
+  // the chunk after (q, i0) in this block's walk
+  auto advance = [&](Seq& q, int& i0) {
     i0 += kC;
     if (i0 >= end) {
       i0 = begin;
-      w += stride;
+      q.advance();
     }
-    return w < total;
+    return q.batch < o.batch;
   };
   if (warp == 8) {
     if (lane == 0) {
@@ -229,9 +242,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int i = 0; i < 4; ++i) mbar_init(bars + i, 1);
       for (int i = 4; i < 7; ++i) mbar_init(bars + i, kWorkers / 32);
       fence_mbar_init();
-      int w = blockIdx.x, i0 = begin;
-      load(Seq(o, w), i0);
-      if (advance(w, i0)) prefetch(Seq(o, w), i0);
+      Seq q(o, blockIdx.x, gridDim.x);
+      int i0 = begin;
+      load(q, i0);
+      if (advance(q, i0)) prefetch(q, i0);
     }
     __syncwarp();
     umma::tmem_alloc(tmem_slot, kCols);
@@ -257,7 +271,8 @@ __global__ void __launch_bounds__(kThreads, 2)
                             smem_desc(base + F::plane(2), 8192, 1024)};
     const bool leader = elect_one();
     uint32_t parity = 0;
-    int w = blockIdx.x, i0 = begin, head = Seq(o, w).head;
+    Seq q(o, blockIdx.x, gridDim.x);
+    int i0 = begin, head = q.head();
     bool weak = decay_of(head) >= kWeakDecay;
     for (bool more = true; more; parity ^= 1) {
       wait(full, parity);
@@ -316,17 +331,17 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       wait(done_l, parity);
       if (*s_fail) break;
-      more = advance(w, i0);
+      more = advance(q, i0);
       if (!more) break;
-      const Seq q(o, w);
       if (leader) {
         load(q, i0);
-        int w2 = w, i2 = i0;
-        if (advance(w2, i2)) prefetch(Seq(o, w2), i2);
+        Seq q2 = q;
+        int i2 = i0;
+        if (advance(q2, i2)) prefetch(q2, i2);
       }
       __syncwarp();
-      if (q.head != head) {
-        head = q.head;
+      if (q.head() != head) {
+        head = q.head();
         weak = decay_of(head) >= kWeakDecay;
       }
     }
@@ -359,11 +374,63 @@ __global__ void __launch_bounds__(kThreads, 2)
     // where a sequence's entering state lies (null: zeros), and by which strides
     const bool local = kOut && split > 0;
     const int64_t sx = local ? o.Dc : o.sx, sy = local ? 1 : o.sy;
-    auto state_in = [&](const Seq& q) -> const float* {
-      if (!kOut) return nullptr;
-      const int bh = q.batch * o.heads + q.head;
-      if (local) return o.local + ((size_t)(split - 1) * o.batch * o.heads + bh) * elems;
-      return o.init ? o.init + bh * elems : nullptr;
+    const float* states = !kOut ? nullptr : local ? o.local + (size_t)(split - 1) * o.batch * o.heads * elems : o.init;
+    const bool whole_in = sy == 1 && o.Dc % 4 == 0 && ((uintptr_t)states & 15) == 0;
+    auto state_in = [&](const Seq& q) { return states + (q.batch * o.heads + q.head()) * elems + k * sx + (q.d0() + y0) * sy; };
+    auto load_state = [&](const Seq& q) {
+      const int left = states && k < o.Da ? o.Dc - q.d0() - y0 : 0;  // columns of this piece that there are
+      const float* from = state_in(q);
+#pragma unroll
+      for (int i = 0; i < kSC; i += 4) {
+        if (whole_in) {
+          const float4 f = i < left ? *reinterpret_cast<const float4*>(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+          s[i] = f.x, s[i + 1] = f.y, s[i + 2] = f.z, s[i + 3] = f.w;
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) s[i + u] = i + u < left ? from[(i + u) * sy] : 0.f;
+        }
+      }
+    };
+    // a coming sequence's state on its way to L2
+    auto prefetch_state = [&](const Seq& q) {
+      const int left = states && k < o.Da ? o.Dc - q.d0() - y0 : 0;
+      const float* from = state_in(q);
+      if (sy == 1) {
+#pragma unroll
+        for (int i = 0; i < kSC; i += 8)
+          if (i < left) prefetch_l2(from + i);
+      } else if ((k & 7) == 0) {
+#pragma unroll
+        for (int i = 0; i < kSC; ++i)
+          if (i < left) prefetch_l2(from + i * sy);
+      }
+    };
+    // what the walk leaves of s: the final state, or the split's own sum
+    const bool last_split = split == o.nsplit - 1;
+    float* const finals = !kOut ? o.local + (size_t)split * o.batch * o.heads * elems : last_split ? o.fin : nullptr;
+    const int64_t tx = kOut ? o.sx : o.Dc, ty = kOut ? o.sy : 1;
+    const bool whole_out = ty == 1 && o.Dc % 4 == 0 && ((uintptr_t)finals & 15) == 0;
+    auto store_state = [&](const Seq& q) {
+      if (!finals || k >= o.Da) return;
+      // backwards the way out of the last position passes reset[0] and one decay more
+      const bool out = kOut && reverse;
+      const bool dropped = out && o.reset && o.reset[q.batch * o.reset_batch];
+      const float f = out ? pw[1] : 1.f;
+      float* to = finals + (q.batch * o.heads + q.head()) * elems + k * tx + (q.d0() + y0) * ty;
+      const int left = o.Dc - q.d0() - y0;
+#pragma unroll
+      for (int i = 0; i < kSC; i += 4) {
+        float v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = dropped ? 0.f : f * s[i + u];
+        if (whole_out) {
+          if (i < left) *reinterpret_cast<float4*>(to + i) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (i + u < left) to[(i + u) * ty] = v[u];
+        }
+      }
     };
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     uint8_t* stage = smem + F::kP2 + (warp & 3) * 4096 + half * 2048;  // in plane rows of this warp pair
@@ -373,32 +440,26 @@ __global__ void __launch_bounds__(kThreads, 2)
     uint32_t parity = 0;
     int head = -1;
     bool weak = true;
-    bool cut = resets && tid < kC && begin + tid < end && op_cut(o, Seq(o, blockIdx.x).batch, begin + tid);
+    Seq q(o, blockIdx.x, gridDim.x);
+    // the reset flag that cuts before position `begin + tid`, of batch row 0 (there is none before the start)
+    const int t_cut = reverse ? o.steps - begin - tid : begin + tid;
+    const uint8_t* cut0 = resets ? o.reset + t_cut * o.reset_step : nullptr;
+    const int64_t cut_chunk = reverse ? -kC * o.reset_step : kC * o.reset_step;
+    auto cut_at = [&](int batch, int i0) {  // position i0 + tid, i0 = begin + chunk * kC
+      return tid < kC && i0 + tid < end && (!reverse || i0 + tid > 0) &&
+             cut0[batch * o.reset_batch + (i0 - begin) / kC * cut_chunk] != 0;
+    };
+    bool cut = resets && cut_at(q.batch, begin);
+    load_state(q);
     auto arrive = [&](uint64_t* bar) {
       fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
 
-    for (int w = blockIdx.x; w < total; w += stride) {
-      const Seq q(o, w);
-      const float* from = state_in(q);
-      const bool whole = sy == 1 && o.Dc % 4 == 0 && ((uintptr_t)from & 15) == 0;
-#pragma unroll
-      for (int i = 0; i < kSC; i += 4) {
-        const int y = q.d0 + y0 + i;
-        if (from && whole) {
-          const float4 f = k < o.Da && y < o.Dc ? *reinterpret_cast<const float4*>(from + k * sx + y)
-                                                : make_float4(0.f, 0.f, 0.f, 0.f);
-          s[i] = f.x, s[i + 1] = f.y, s[i + 2] = f.z, s[i + 3] = f.w;
-        } else {
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            s[i + u] = from && k < o.Da && y + u < o.Dc ? from[k * sx + (y + u) * sy] : 0.f;
-        }
-      }
-      if (q.head != head) {
-        head = q.head;
+    for (bool more = true; more;) {
+      if (q.head() != head) {
+        head = q.head();
         const float g = decay_of(head);
         weak = g >= kWeakDecay;
         sync_workers();  // nobody reads the last head's powers any more
@@ -412,20 +473,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         sync_workers();
       }
-      // the next sequence's state on its way to L2
-      if (kOut && w + stride < total) {
-        const Seq nq(o, w + stride);
-        const float* next = state_in(nq);
-        if (next && k < o.Da && nq.d0 + y0 < o.Dc) {
-          if (sy == 1) {
-#pragma unroll
-            for (int i = 0; i < kSC; i += 8) prefetch_l2(next + k * sx + nq.d0 + min(y0 + i, o.Dc - 1 - nq.d0));
-          } else if ((k & 7) == 0) {
-#pragma unroll
-            for (int i = 0; i < kSC; ++i) prefetch_l2(next + k * sx + min(nq.d0 + y0 + i, o.Dc - 1) * sy);
-          }
-        }
-      }
+      Seq next = q;
+      next.advance();
+      more = next.batch < o.batch;
+      if (kOut && more) prefetch_state(next);
       bool any_cut = false;
       int e0 = (reverse && split == 0) ? 0 : 1;
       // s takes its decay over the n positions to come, and its copy goes where O's product reads it. The
@@ -451,8 +502,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (tid < kC) {
             const unsigned m = __ballot_sync(~0u, cut);
             if (lane == 0) cuts[warp] = m;
-            const int nw = ends ? w + stride : w, ni = (ends ? begin : i0 + kC) + tid;
-            cut = nw < total && ni < end && op_cut(o, Seq(o, nw).batch, ni);
+            cut = (!ends || more) && cut_at(ends ? next.batch : q.batch, ends ? begin : i0 + kC);
           }
           sync_workers();
 #pragma unroll
@@ -571,7 +621,13 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int i = 0; i < kSC; ++i) s[i] = (last < 0 ? s[i] : 0.f) + l[i];
         }
         e0 = 1;
-        if (!ends) hand_state(min(kC, end - i0 - kC));
+        if (!ends) {
+          hand_state(min(kC, end - i0 - kC));
+        } else {
+          store_state(q);
+          if (!kOut && tid == 0 && q.at == 0) o.cut[split * o.batch + q.batch] = any_cut;
+          if (more) load_state(next);  // comes in while the outputs go out
+        }
         if (kOut) {
           wait(done_o, parity);
           float v[32];
@@ -580,19 +636,19 @@ __global__ void __launch_bounds__(kThreads, 2)
           const float f = weak && p < n ? o.out_scale / pw[n - 1 - p] : o.out_scale;
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] *= f;
-          const int t0 = time_of(i0), x0 = q.d0 + 32 * half;
+          const int t0 = time_of(i0), x0 = q.d0() + 32 * half;
           if (t0 >= 0) {
             // rows behind the last step and columns behind Dc fall away in the store
             umma::stage_row_bf16(stage, nullptr, lane, v);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0 && x0 < o.Dc) {
-              tma_store_4d(&maps.out[blockIdx.z], stage, x0, t0 + 32 * (warp & 3), q.head, q.batch);
+              tma_store_4d(&maps.out[blockIdx.z], stage, x0, t0 + 32 * (warp & 3), q.head(), q.batch);
               umma::bulk_commit();
             }
           } else if (p < n) {  // a first chunk in time that begins before step 0
             __nv_bfloat16* out = static_cast<__nv_bfloat16*>(o.out) + q.batch * o.out_batch +
-                                 (int64_t)(t0 + row) * o.out_step + q.head * o.out_head + x0;
+                                 (int64_t)(t0 + row) * o.out_step + q.head() * o.out_head + x0;
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
               // Dc is a multiple of 8, as the rows' strides are
@@ -603,41 +659,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
         }
       }
-      const int bh = q.batch * o.heads + q.head;
-      float* to = nullptr;
-      int64_t tx = o.sx, ty = o.sy;
-      float way_out = 1.f;
-      if (kOut) {
-        if (o.fin && split == o.nsplit - 1) {
-          to = o.fin + bh * elems;
-          if (reverse) {
-            way_out = pw[1];
-            if (resets && o.reset[q.batch * o.reset_batch]) way_out = 0.f;
-          }
-        }
-      } else {
-        to = o.local + ((size_t)split * o.batch * o.heads + bh) * elems;
-        tx = o.Dc;
-        ty = 1;
-        if (tid == 0 && q.d0 == 0 && q.head == 0) o.cut[split * o.batch + q.batch] = any_cut;
-      }
-      if (to && k < o.Da) {
-        const bool vec = ty == 1 && o.Dc % 4 == 0 && ((uintptr_t)to & 15) == 0;
-#pragma unroll
-        for (int i = 0; i < kSC; i += 4) {
-          const int y = q.d0 + y0 + i;
-          float f[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) f[u] = way_out == 0.f ? 0.f : way_out * s[i + u];
-          if (vec) {
-            if (y < o.Dc) *reinterpret_cast<float4*>(to + k * tx + y) = make_float4(f[0], f[1], f[2], f[3]);
-          } else {
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (y + u < o.Dc) to[k * tx + (y + u) * ty] = f[u];
-          }
-        }
-      }
+      q = next;
     }
     if (lane == 0) umma::bulk_wait_all();
     __syncwarp();
