@@ -64,7 +64,8 @@ struct Cfg {
   static constexpr int kP2 = kS + DA * 128;  // planes that do not fit into a's buffer
   static constexpr int kPlanes = kP2 + (3 - kNA) * kBlock;
   static constexpr int kBar = kPlanes;
-  static constexpr int kBytes = kBar + 80 + 4 * (kC + 4) + 16 + 32;
+  static constexpr int kOp = kBar + 80 + 4 * (kC + 4) + 16 + 32;
+  static constexpr int kBytes = kOp + (sizeof(Op) + 15) / 16 * 16;
   __device__ static int plane(int k) { return k < kNA ? kA + k * kBlock : kP2 + (k - kNA) * kBlock; }
 };
 static_assert(2 * (Cfg<128>::kBytes + 1024) <= 228 * 1024, "two blocks on an SM");
@@ -115,6 +116,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
@@ -152,6 +158,31 @@ __device__ __forceinline__ constexpr uint32_t idesc() {
 // The eight worker warps (named barrier 1), and the two of them that share 32 rows (2 to 5).
 __device__ __forceinline__ void sync_workers() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ void sync_pair(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory"); }
+
+// A value whose descendants the compiler does not take out of a loop.
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+r"(x));
+  return x;
+}
+
+// Four lanes' rows of 16 values, four at a time, turned about: lane l's piece j becomes lane j's piece l.
+// A row's 64 bytes are then read or written by four neighbouring lanes at once.
+__device__ __forceinline__ void turn_quads(float* s, int lane) {
+#pragma unroll
+  for (int bit = 1; bit <= 2; bit <<= 1) {
+    const bool up = lane & bit;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j & bit) continue;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float &a = s[4 * j + u], &b = s[4 * (j + bit) + u];
+        const float y = __shfl_xor_sync(~0u, up ? a : b, bit);
+        if (up) a = y; else b = y;
+      }
+    }
+  }
+}
 
 // A sequence of the launch: one (batch row, head) and 64 columns of c (one or two slices of them). A block
 // takes every gridDim.x-th; the heads and slices of a batch row follow one another.
@@ -195,7 +226,11 @@ __global__ void __launch_bounds__(kThreads, 2)
   float* pl = pw + kC + 4;  // what the rounding left of e^{i g}, i = 127, 128, n and n - 1 of the last chunk
   unsigned* s_cut = reinterpret_cast<unsigned*>(pl + 4);  // [2][4] the cuts of a chunk, a bit a position
 
-  const Op& o = ops.op[blockIdx.z];
+  // a copy in shared memory, so that what is rarely needed holds no registers
+  Op& o = *reinterpret_cast<Op*>(smem + F::kOp);
+  if (threadIdx.x < sizeof(Op) / 4)
+    reinterpret_cast<uint32_t*>(&o)[threadIdx.x] = reinterpret_cast<const uint32_t*>(&ops.op[blockIdx.z])[threadIdx.x];
+  __syncthreads();
   if ((int)blockIdx.x >= o.batch * o.heads * ceil_div(o.Dc, kDS)) return;
   if (smem_u32(smem) & 1023) {  // the swizzled tiles count on it
     if (threadIdx.x == 0) atomicExch(err, kErrAlignment);
@@ -353,15 +388,16 @@ __global__ void __launch_bounds__(kThreads, 2)
       mbar_wait_bounded(done_o, parity);
     }
   } else {
-    const int row = (warp & 3) * 32 + lane, half = warp >> 2;  // tensor memory lane, column half
-    const size_t elems = (size_t)o.Da * o.Dc;
+    const int row0 = (warp & 3) * 32 + lane, half0 = warp >> 2, lane0 = lane;  // tensor memory lane, column half
+    uint8_t* const smem0 = smem;
     // A worker's piece of the state: row k, columns y0 .. (the rows of L repeat where Da <= 64, and the
     // second copy takes the other half of the columns).
     constexpr int kSC = DA == 128 ? 32 : 16;
-    const int k = DA == 128 ? row : row & 63;
-    const int y0 = DA == 128 ? half * 32 : (row >> 6) * 32 + half * 16;
+    auto row_of_state = [&]() { return DA == 128 ? opaque(row0) : opaque(row0) & 63; };
+    auto column_of_state = [&]() { return DA == 128 ? opaque(half0) * 32 : (opaque(row0) >> 6) * 32 + half0 * 16; };
     float s[kSC];
     auto put_state = [&]() {
+      const int k = row_of_state(), y0 = column_of_state();
 #pragma unroll
       for (int i = 0; i < kSC; i += 8) {
         uint32_t w[4];
@@ -373,28 +409,46 @@ __global__ void __launch_bounds__(kThreads, 2)
     };
     // where a sequence's entering state lies (null: zeros), and by which strides
     const bool local = kOut && split > 0;
-    const int64_t sx = local ? o.Dc : o.sx, sy = local ? 1 : o.sy;
-    const float* states = !kOut ? nullptr : local ? o.local + (size_t)(split - 1) * o.batch * o.heads * elems : o.init;
-    const bool whole_in = sy == 1 && o.Dc % 4 == 0 && ((uintptr_t)states & 15) == 0;
-    auto state_in = [&](const Seq& q) { return states + (q.batch * o.heads + q.head()) * elems + k * sx + (q.d0() + y0) * sy; };
+    auto state_in = [&](const Seq& q, int k, int y0, int& sx, int& sy) -> const float* {
+      const float* all = !kOut ? nullptr : local ? o.local + (size_t)(split - 1) * o.batch * o.heads * (o.Da * o.Dc) : o.init;
+      if (!all) return nullptr;
+      sx = local ? o.Dc : o.sx;
+      sy = local ? 1 : o.sy;
+      return all + (size_t)(q.batch * o.heads + q.head()) * (o.Da * o.Dc) + k * sx + (q.d0() + y0) * sy;
+    };
+    // (a state's rows start on 16-byte boundaries where its columns lie together and Dc is a multiple of 4)
+    const bool whole_in = (local || o.sy == 1) && o.Dc % 4 == 0 && ((uintptr_t)(local ? o.local : o.init) & 15) == 0;
     auto load_state = [&](const Seq& q) {
-      const int left = states && k < o.Da ? o.Dc - q.d0() - y0 : 0;  // columns of this piece that there are
-      const float* from = state_in(q);
+      int sx = 0, sy = 0;
+      const int k = row_of_state(), y0 = column_of_state();
+      const float* from = state_in(q, k, y0, sx, sy);
+      const int left = from ? o.Dc - q.d0() - y0 : 0;  // columns of this piece that there are
+      if (whole_in) {
+        const int l = lane & 3;
 #pragma unroll
-      for (int i = 0; i < kSC; i += 4) {
-        if (whole_in) {
-          const float4 f = i < left ? *reinterpret_cast<const float4*>(from + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < kSC; i += 4) {
+          const int r = (i >> 2 & 3) - l, c = (i & ~15) + 4 * l;  // the row's neighbour, and its columns
+          const float4 f = k + r < o.Da && c < left ? *reinterpret_cast<const float4*>(from + r * sx + c)
+                                                    : make_float4(0.f, 0.f, 0.f, 0.f);
           s[i] = f.x, s[i + 1] = f.y, s[i + 2] = f.z, s[i + 3] = f.w;
-        } else {
-#pragma unroll
-          for (int u = 0; u < 4; ++u) s[i + u] = i + u < left ? from[(i + u) * sy] : 0.f;
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kSC; ++i) s[i] = k < o.Da && i < left ? from[i * sy] : 0.f;
       }
+    };
+    // after load_state, before the state is used
+    auto settle_state = [&]() {
+      if (whole_in)
+#pragma unroll
+        for (int i = 0; i < kSC; i += 16) turn_quads(s + i, lane);
     };
     // a coming sequence's state on its way to L2
     auto prefetch_state = [&](const Seq& q) {
-      const int left = states && k < o.Da ? o.Dc - q.d0() - y0 : 0;
-      const float* from = state_in(q);
+      int sx = 0, sy = 0;
+      const int k = row_of_state(), y0 = column_of_state();
+      const float* from = state_in(q, k, y0, sx, sy);
+      const int left = from && k < o.Da ? o.Dc - q.d0() - y0 : 0;
       if (sy == 1) {
 #pragma unroll
         for (int i = 0; i < kSC; i += 8)
@@ -406,49 +460,44 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     };
     // what the walk leaves of s: the final state, or the split's own sum
-    const bool last_split = split == o.nsplit - 1;
-    float* const finals = !kOut ? o.local + (size_t)split * o.batch * o.heads * elems : last_split ? o.fin : nullptr;
-    const int64_t tx = kOut ? o.sx : o.Dc, ty = kOut ? o.sy : 1;
-    const bool whole_out = ty == 1 && o.Dc % 4 == 0 && ((uintptr_t)finals & 15) == 0;
     auto store_state = [&](const Seq& q) {
-      if (!finals || k >= o.Da) return;
+      float* const all = !kOut ? o.local + (size_t)split * o.batch * o.heads * (o.Da * o.Dc)
+                               : split == o.nsplit - 1 ? o.fin : nullptr;
+      if (!all) return;
+      const int k = row_of_state(), y0 = column_of_state();
+      const int tx = kOut ? o.sx : o.Dc, ty = kOut ? o.sy : 1;
+      const bool whole_out = ty == 1 && o.Dc % 4 == 0 && ((uintptr_t)all & 15) == 0;
       // backwards the way out of the last position passes reset[0] and one decay more
       const bool out = kOut && reverse;
       const bool dropped = out && o.reset && o.reset[q.batch * o.reset_batch];
       const float f = out ? pw[1] : 1.f;
-      float* to = finals + (q.batch * o.heads + q.head()) * elems + k * tx + (q.d0() + y0) * ty;
+      float* to = all + (size_t)(q.batch * o.heads + q.head()) * (o.Da * o.Dc) + k * tx + (q.d0() + y0) * ty;
       const int left = o.Dc - q.d0() - y0;
+      // s is not read again
 #pragma unroll
-      for (int i = 0; i < kSC; i += 4) {
-        float v[4];
+      for (int i = 0; i < kSC; ++i) s[i] = dropped ? 0.f : f * s[i];
+      if (whole_out) {
+        const int l = lane & 3;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = dropped ? 0.f : f * s[i + u];
-        if (whole_out) {
-          if (i < left) *reinterpret_cast<float4*>(to + i) = make_float4(v[0], v[1], v[2], v[3]);
-        } else {
+        for (int i = 0; i < kSC; i += 16) turn_quads(s + i, lane);
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (i + u < left) to[(i + u) * ty] = v[u];
+        for (int i = 0; i < kSC; i += 4) {
+          const int r = (i >> 2 & 3) - l, c = (i & ~15) + 4 * l;
+          if (k + r < o.Da && c < left)
+            *reinterpret_cast<float4*>(to + r * tx + c) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kSC; ++i)
+          if (k < o.Da && i < left) to[i * ty] = s[i];
       }
     };
-    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    uint8_t* stage = smem + F::kP2 + (warp & 3) * 4096 + half * 2048;  // in plane rows of this warp pair
-    const int p = reverse ? kC - 1 - row : row;  // the position of this thread's row
-    const float in_scale = o.in_scale;
     const bool resets = o.reset != nullptr;
     uint32_t parity = 0;
     int head = -1;
     bool weak = true;
     Seq q(o, blockIdx.x, gridDim.x);
-    // the reset flag that cuts before position `begin + tid`, of batch row 0 (there is none before the start)
-    const int t_cut = reverse ? o.steps - begin - tid : begin + tid;
-    const uint8_t* cut0 = resets ? o.reset + t_cut * o.reset_step : nullptr;
-    const int64_t cut_chunk = reverse ? -kC * o.reset_step : kC * o.reset_step;
-    auto cut_at = [&](int batch, int i0) {  // position i0 + tid, i0 = begin + chunk * kC
-      return tid < kC && i0 + tid < end && (!reverse || i0 + tid > 0) &&
-             cut0[batch * o.reset_batch + (i0 - begin) / kC * cut_chunk] != 0;
-    };
+    auto cut_at = [&](int batch, int i0) { return tid < kC && i0 + tid < end && op_cut(o, batch, i0 + tid); };
     bool cut = resets && cut_at(q.batch, begin);
     load_state(q);
     auto arrive = [&](uint64_t* bar) {
@@ -477,6 +526,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       next.advance();
       more = next.batch < o.batch;
       if (kOut && more) prefetch_state(next);
+      settle_state();
       bool any_cut = false;
       int e0 = (reverse && split == 0) ? 0 : 1;
       // s takes its decay over the n positions to come, and its copy goes where O's product reads it. The
@@ -495,6 +545,14 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int i0 = begin; i0 < end; i0 += kC, parity ^= 1) {
         const int n = min(kC, end - i0);
         const bool ends = i0 + kC >= end;
+        // what follows from a thread's place is formed anew in every chunk: kept, it would crowd the registers out
+        // into local memory, for which shared memory leaves next to no L1
+        const int row = opaque(row0), half = opaque(half0), lane = opaque(lane0);
+        const int p = reverse ? kC - 1 - row : row;
+        uint8_t* const smem = smem0 + opaque(0);
+        uint8_t* const stage = smem + F::kP2 + (row >> 5) * 4096 + half * 2048;  // in plane rows of this warp pair
+        const uint32_t lanes = tmem + ((uint32_t)(row & 96) << 16);
+        const int y0 = DA == 128 ? half * 32 : (row >> 6) * 32 + half * 16;
         // the last cut of the chunk, and the last one at or before p (-1: none)
         int last = -1, lo = -1;
         if (resets) {
@@ -518,41 +576,47 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (kOut) {
           // the pair's last outputs have left their staging rows
           if (lane == 0) umma::bulk_wait_read_all();
-          sync_pair(warp & 3);
+          sync_pair(row >> 5);
         }
         {  // w c: this thread's row, half of the columns; the planes that go into a's place wait for it
-          const float wf = p < n ? in_scale * pw[n - 1 - p] : 0.f;
+          const float wf = p < n ? o.in_scale * pw[n - 1 - p] : 0.f;
           const uint64_t wp = pair(wf, wf);
-          uint4 held[F::kNA][4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int off = row * 128 + (((half * 4 + u) ^ (row & 7)) << 4);
+          // 24 bits cut into 8 + 8 + 8: each plane takes the leading bits, the rest is exact
+          auto cut_up = [&](int off, uint4 (&y)[3]) {
             const uint4 x = *reinterpret_cast<const uint4*>(smem + F::kCc + off);
             const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-            uint32_t y[3][4];
-            // 24 bits cut into 8 + 8 + 8: each plane takes the leading bits, the rest is exact
+            uint32_t t[3][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint64_t v = mul2(wp, pair_of_bf16(xs[i]));
 #pragma unroll
               for (int z = 0; z < 3; ++z) {
-                y[z][i] = __byte_perm((uint32_t)v, (uint32_t)(v >> 32), 0x7632);
+                t[z][i] = __byte_perm((uint32_t)v, (uint32_t)(v >> 32), 0x7632);
                 if (z < 2) v = sub2(v, v & 0xffff0000ffff0000ull);
               }
             }
 #pragma unroll
-            for (int z = 0; z < 3; ++z) {
-              const uint4 t = make_uint4(y[z][0], y[z][1], y[z][2], y[z][3]);
-              if (z < F::kNA) held[z < F::kNA ? z : 0][u] = t;
-              else *reinterpret_cast<uint4*>(smem + F::plane(z) + off) = t;
-            }
+            for (int z = 0; z < 3; ++z) y[z] = make_uint4(t[z][0], t[z][1], t[z][2], t[z][3]);
+          };
+          auto place = [&](int u) { return row * 128 + (((half * 4 + u) ^ (row & 7)) << 4); };
+          uint4 held[4], y[3];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            cut_up(place(u), y);
+            if (F::kNA == 1) held[u] = y[0];
+#pragma unroll
+            for (int z = F::kNA; z < 3; ++z) *reinterpret_cast<uint4*>(smem + F::plane(z) + place(u)) = y[z];
           }
           if (kOut) wait(done_a, parity);
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const int off = row * 128 + (((half * 4 + u) ^ (row & 7)) << 4);
+            if (F::kNA == 1) {
+              y[0] = held[u];
+            } else {
+              cut_up(place(u), y);  // once more: two planes held would not fit in the registers
+            }
 #pragma unroll
-            for (int z = 0; z < F::kNA; ++z) *reinterpret_cast<uint4*>(smem + F::plane(z) + off) = held[z][u];
+            for (int z = 0; z < F::kNA; ++z) *reinterpret_cast<uint4*>(smem + F::plane(z) + place(u)) = y[z];
           }
           if (last > p) {  // what a cut hides has no part in L; P0 is done with its row of b
 #pragma unroll
@@ -569,45 +633,44 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (!weak || last >= 0) {
             // the rows of a S by the decay since the state; a cut drops it whatever it holds
             const float reach = lo >= 0 || p >= n ? 0.f : weak ? 1.f : pw[p + e0];
-            float v[32];
-            tmem_ld32(lanes + kOCol + 32 * half, v);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
+              float v[16];
               uint32_t x[16];
+              tmem_ld16(lanes + kOCol + 32 * half + 16 * j, v);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) x[i] = reach != 0.f ? __float_as_uint(reach * v[16 * j + i]) : 0u;
+              for (int i = 0; i < 16; ++i) x[i] = reach != 0.f ? __float_as_uint(reach * v[i]) : 0u;
               tmem_st16(lanes + kOCol + 32 * half + 16 * j, x);
             }
           }
-          // P: this warp's 32 rows against the column blocks 2 half and 2 half + 1. It takes the place of
-          // the first of the two, which is read by then.
+          // P: this warp's 32 rows against the columns 64 half .. 64 half + 63, 16 at a time. It takes the place
+          // of the first half of them: what it replaces is read by then.
           const int first = max(lo, 0);  // columns of positions first .. p count
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int blk = 2 * half + u;
-            const unsigned m = reverse ? bits(kC - 1 - 32 * blk - p, kC - 1 - 32 * blk - first)
-                                       : bits(first - 32 * blk, p - 32 * blk);
-            uint32_t pk[16];
+          for (int u = 0; u < 4; ++u) {
+            const int c0 = 64 * half + 16 * u;
+            const unsigned m = (reverse ? bits(kC - 1 - c0 - p, kC - 1 - c0 - first) : bits(first - c0, p - c0)) & 0xffffu;
+            uint32_t pk[8];
             if (__all_sync(~0u, m == 0)) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) pk[i] = 0;
+              for (int i = 0; i < 8; ++i) pk[i] = 0;
             } else {
-              float v[32];
-              tmem_ld32(lanes + 32 * blk, v);
+              float v[16];
+              tmem_ld16(lanes + c0, v);
               if (!weak) {
                 // e^{(p_i - p_j) g}: only where the column comes no later than the row
-                const int gap0 = reverse ? 32 * blk - row : row - 32 * blk, dir = reverse ? 1 : -1;
+                const int gap0 = reverse ? c0 - row : row - c0, dir = reverse ? 1 : -1;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] *= in_scale * pw[max(0, gap0 + dir * i)];
+                for (int i = 0; i < 16; ++i) v[i] *= o.in_scale * pw[max(0, gap0 + dir * i)];
               }
-              if (!__all_sync(~0u, m == ~0u)) {
+              if (!__all_sync(~0u, m == 0xffffu)) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = m >> i & 1 ? v[i] : 0.f;
+                for (int i = 0; i < 16; ++i) v[i] = m >> i & 1 ? v[i] : 0.f;
               }
 #pragma unroll
-              for (int i = 0; i < 16; ++i) pk[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+              for (int i = 0; i < 8; ++i) pk[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
             }
-            tmem_st16(lanes + 64 * half + 16 * u, pk);
+            tmem_st8(lanes + 64 * half + 8 * u, pk);
           }
           tmem_wait_st();
           arrive(has_p);
@@ -630,32 +693,38 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         if (kOut) {
           wait(done_o, parity);
-          float v[32];
-          tmem_ld32(lanes + kOCol + 32 * half, v);
-          if (!ends) arrive(has_s);
           const float f = weak && p < n ? o.out_scale / pw[n - 1 - p] : o.out_scale;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] *= f;
           const int t0 = time_of(i0), x0 = q.d0() + 32 * half;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float v[16];
+            tmem_ld16(lanes + kOCol + 32 * half + 16 * j, v);
+            if (j == 1 && !ends) arrive(has_s);
+            uint4 y[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              y[i] = make_uint4(pack_bf16(f * v[8 * i], f * v[8 * i + 1]), pack_bf16(f * v[8 * i + 2], f * v[8 * i + 3]),
+                                pack_bf16(f * v[8 * i + 4], f * v[8 * i + 5]), pack_bf16(f * v[8 * i + 6], f * v[8 * i + 7]));
+            if (t0 >= 0) {  // (the 64-byte swizzle of a row of 32)
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<uint4*>(stage + lane * 64 + (((2 * j + i) ^ (lane >> 1 & 3)) << 4)) = y[i];
+            } else if (p < n) {  // a first chunk in time that begins before step 0
+              __nv_bfloat16* out = static_cast<__nv_bfloat16*>(o.out) + q.batch * o.out_batch +
+                                   (int64_t)(t0 + row) * o.out_step + q.head() * o.out_head + x0 + 16 * j;
+#pragma unroll
+              for (int i = 0; i < 2; ++i)  // Dc is a multiple of 8, as the rows' strides are
+                if (x0 + 16 * j + 8 * i < o.Dc) *reinterpret_cast<uint4*>(out + 8 * i) = y[i];
+            }
+          }
           if (t0 >= 0) {
             // rows behind the last step and columns behind Dc fall away in the store
-            umma::stage_row_bf16(stage, nullptr, lane, v);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0 && x0 < o.Dc) {
               tma_store_4d(&maps.out[blockIdx.z], stage, x0, t0 + 32 * (warp & 3), q.head(), q.batch);
               umma::bulk_commit();
             }
-          } else if (p < n) {  // a first chunk in time that begins before step 0
-            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(o.out) + q.batch * o.out_batch +
-                                 (int64_t)(t0 + row) * o.out_step + q.head() * o.out_head + x0;
-#pragma unroll
-            for (int i = 0; i < 32; i += 8)
-              // Dc is a multiple of 8, as the rows' strides are
-              if (x0 + i < o.Dc)
-                *reinterpret_cast<uint4*>(out + i) =
-                    make_uint4(pack_bf16(v[i], v[i + 1]), pack_bf16(v[i + 2], v[i + 3]),
-                               pack_bf16(v[i + 4], v[i + 5]), pack_bf16(v[i + 6], v[i + 7]));
           }
         }
       }
