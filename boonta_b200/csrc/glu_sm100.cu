@@ -7,7 +7,7 @@
 //             K <= 800 reading two fp32 values per element back costs more than 4 K flops do)
 //   kInput    dx = dG Wg^T + dU Wu^T         the two products in one accumulator
 //   kWeights  dWg = x^T dG, dWu = x^T dU     both from one load of x, split over the rows
-// A CTA per SM walks the output tiles. Warp 0 loads 64-deep blocks of A and B by TMA into a ring of
+// A CTA per SM walks the output tiles (of half the width where there are fewer tiles than SMs). Warp 0 loads 64-deep blocks of A and B by TMA into a ring of
 // four 48 KB stages, warp 1 issues the MMAs into one of two 256-column accumulators in tensor
 // memory, and eight epilogue warps drain the other: activation and product in registers, the
 // result through 4 KB of shared memory per warp to TMA stores.
@@ -35,10 +35,15 @@ using namespace umma;
 
 enum Mode { kForward, kGrads, kInput, kWeights };
 
-constexpr int kStages = 4, kBN = 256;
-constexpr int kAB = BM * BK * 2, kBB = kBN * BK * 2, kStageBytes = kAB + kBB;
-constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * kEpiWarpBytes + 1024 + 256;
-static_assert(kSmemBytes <= kMaxSmem, "stage ring");
+constexpr int kAB = BM * BK * 2;
+// N columns of the MMA: 256, or 128 where that many would leave SMs without a tile.
+template <int N>
+struct Ring {
+  static constexpr int kStages = N == 256 ? 4 : 6;
+  static constexpr int kStageBytes = kAB + N * BK * 2;
+  static constexpr int kSmem = kStages * kStageBytes + kEpiWarps * kEpiWarpBytes + 1024 + 256;
+  static_assert(kSmem <= kMaxSmem, "stage ring");
+};
 
 struct Seg {
   uint8_t a, b0, b1;  // maps of a product's A and of its B (kInput: b0 alone)
@@ -166,12 +171,14 @@ __device__ __forceinline__ void put_planes(const CUtensorMap* maps, int row0, in
 
 // T: the layer's type. An fp32 layer's operands are planes and its accumulator is handed over after
 // every 64-deep block.
-template <class T, Mode kMode>
+template <class T, Mode kMode, int kN>
 __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant__ Params p) {
+  constexpr int kStages = Ring<kN>::kStages, kStageBytes = Ring<kN>::kStageBytes;
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr bool kDual = kMode != kInput;
   constexpr bool A_MN = kMode == kWeights, B_MN = kMode != kInput;
-  constexpr int kTileN = kDual ? kBN / 2 : kBN;
+  constexpr int kTileN = kDual ? kN / 2 : kN;
+  constexpr int kGroups = kN / 64;  // groups of 32 accumulator columns of an epilogue warp
   // 64-deep blocks between two hand-overs of the accumulator: bf16 results keep 2^-8, far above what
   // the truncation of a whole product leaves
   constexpr int kHand = kF32 ? 1 : 1 << 30;
@@ -200,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
     for (int w = 0; w < kEpiWarps; ++w) mbar_init(&epi_in[w], 1);
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, 2 * kBN);
+  if (warp == 1) tmem_alloc(tmem_slot, 2 * kN);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
@@ -246,8 +253,8 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
             }
             if (kDual) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                tma_load_2d(sb + j * 8192, &p.map[j < 2 ? sg.b0 : sg.b1], n0 + 64 * (j & 1), k, &full[s]);
+              for (int j = 0; j < kN / 64; ++j)
+                tma_load_2d(sb + j * 8192, &p.map[j < kN / 128 ? sg.b0 : sg.b1], n0 + 64 * (j % (kN / 128)), k, &full[s]);
             } else {
               tma_load_2d(sb, &p.map[sg.b0], k, n0, &full[s]);
             }
@@ -260,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t idesc = instr_desc<kBN, A_MN, B_MN>();
+      constexpr uint32_t idesc = instr_desc<kN, A_MN, B_MN>();
       int g = 0, c = 0;
       bool ok = true;
       for (int t = blockIdx.x; t < tiles && ok && !failed(); t += gridDim.x) {
@@ -276,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
             }
             fence_after_sync();
           }
-          const uint32_t acc = tmem + (uint32_t)((c & 1) * kBN);
+          const uint32_t acc = tmem + (uint32_t)((c & 1) * kN);
           for (int e = 0; e < p.nseg; ++e, ++g) {
             const int s = g % kStages;
             if (!mbar_wait_bounded(&full[s], (g / kStages) & 1)) {
@@ -305,11 +312,10 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
     uint8_t* buf = epi_smem + (warp - 2) * kEpiWarpBytes;
     uint64_t* ibar = &epi_in[warp - 2];
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
-    // TMEM column of this warp's group j: two groups of each projection, or four of the one product
-    auto column = [&](int j) {
-      return kDual ? (j >> 1) * (kBN / 2) + half * 64 + (j & 1) * 32 : half * 128 + j * 32;
-    };
-    float run[kF32 ? 4 : 1][32];
+    // TMEM column of this warp's group j: half of the groups of each projection, or all of the one product
+    constexpr int kEach = kDual ? kGroups / 2 : kGroups;
+    auto column = [&](int j) { return j / kEach * (kN / 2) + half * (kEach * 32) + j % kEach * 32; };
+    float run[kF32 ? kGroups : 1][32];
     int c = 0, loads = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok && !failed(); t += gridDim.x) {
@@ -318,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
       const int row0 = m0 + q * 32;
       if constexpr (kF32) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < kGroups; ++j)
 #pragma unroll
           for (int i = 0; i < 32; ++i) run[j][i] = 0.f;
         for (int kb = k0; kb < k1; ++kb, ++c) {
@@ -326,9 +332,9 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
           if (!ok) break;
           fence_after_sync();
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < kGroups; ++j) {
             float v[32];
-            tmem_ld32(lanes + (uint32_t)((c & 1) * kBN + column(j)), v);
+            tmem_ld32(lanes + (uint32_t)((c & 1) * kN + column(j)), v);
 #pragma unroll
             for (int i = 0; i < 32; ++i) run[j][i] += v[i];
           }
@@ -344,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
         if (lane == 0) atomicExch(&s_fail, kErrTimeoutAcc);
         break;
       }
-      const uint32_t acc = lanes + (uint32_t)((c & 1) * kBN);
+      const uint32_t acc = lanes + (uint32_t)((c & 1) * kN);
       auto group = [&](int j, float (&v)[32]) {
         if constexpr (kF32) {
 #pragma unroll
@@ -363,8 +369,8 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
       };
       if constexpr (kMode == kForward || kMode == kGrads) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int col0 = n0 + half * 64 + 32 * j;
+        for (int j = 0; j < kEach; ++j) {
+          const int col0 = n0 + half * (kEach * 32) + 32 * j;
           const bool in = col0 < p.N && row0 < p.M;
           if (kMode == kGrads && in) {
             staging_free(lane);
@@ -377,8 +383,8 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
           }
           float g[32], u[32];
           group(j, g);
-          group(2 + j, u);
-          if (j == 1) release();
+          group(kEach + j, u);
+          if (j == kEach - 1) release();
           if constexpr (kMode == kForward) {
             if (!in) continue;
             with_act(p.act, [&](auto tag) {
@@ -428,20 +434,20 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
         }
       } else if constexpr (kMode == kInput) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int col0 = n0 + half * 128 + 32 * j;
+        for (int j = 0; j < kGroups; ++j) {
+          const int col0 = n0 + half * (kN / 2) + 32 * j;
           float v[32];
           group(j, v);
-          if (j == 3) release();
+          if (j == kGroups - 1) release();
           if (col0 < p.N && row0 < p.M) put<T>(&p.out[0], p.o0, p, row0, col0, buf, lane, v);
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int which = j >> 1, col0 = n0 + half * 64 + 32 * (j & 1);
+        for (int j = 0; j < kGroups; ++j) {
+          const int which = j / kEach, col0 = n0 + half * (kEach * 32) + 32 * (j % kEach);
           float v[32];
           group(j, v);
-          if (j == 3) release();
+          if (j == kGroups - 1) release();
           if (col0 >= p.N || row0 >= p.M) continue;
           if (p.splits > 1) {  // one partial plane for each split and weight
             put<float>(&p.out[0], nullptr, p, (2 * split + which) * p.plane_rows + row0, col0, buf, lane, v);
@@ -458,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
   __syncthreads();
   if (warp == 1) {
     fence_after_sync();
-    tmem_dealloc(tmem, 2 * kBN);
+    tmem_dealloc(tmem, 2 * kN);
   }
   if (threadIdx.x == 0 && s_fail) atomicExch(p.err, s_fail);
 }
@@ -523,7 +529,7 @@ int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 // through memory (written and read once at about 5 TB/s); a 64-deep block of a tile takes 0.33 us
 // (fp32: six times that).
 int choose_splits(int M, int K, int N, int planes) {
-  const int tiles = ceil_div(K, BM) * ceil_div(N, kBN / 2), nk = ceil_div(M, BK);
+  const int tiles = ceil_div(K, BM) * ceil_div(N, 128), nk = ceil_div(M, BK);
   const double block = planes == 3 ? 2.0 : 0.33;
   int best = 1;
   double least = 1e30;
@@ -618,14 +624,22 @@ struct Run {
       }
     return n;
   }
+  // Whether a product's tiles of 256 accumulator columns would leave SMs without one.
+  static bool narrow(int M, int N, int splits, bool dual) {
+    return ceil_div(M, BM) * ceil_div(N, dual ? 128 : 256) * splits < kNumSMs;
+  }
+  template <Mode kMode, int kN>
+  int launch_n(Params& p) {
+    auto kernel = glu_kernel<T, kMode, kN>;
+    BT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<kN>::kSmem));
+    BT_TRY(operator_error_word(&p.err));
+    const int tiles = ceil_div(p.M, BM) * ceil_div(p.N, kMode == kInput ? kN : kN / 2) * p.splits;
+    BT_CUDA(launch_pdl(kernel, dim3(min(tiles, kNumSMs)), dim3(kThreads), Ring<kN>::kSmem, s, p));
+    return BT_OK;
+  }
   template <Mode kMode>
   int launch(Params& p) {
-    auto kernel = glu_kernel<T, kMode>;
-    BT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
-    BT_TRY(operator_error_word(&p.err));
-    const int tiles = ceil_div(p.M, BM) * ceil_div(p.N, kMode == kInput ? kBN : kBN / 2) * p.splits;
-    BT_CUDA(launch_pdl(kernel, dim3(min(tiles, kNumSMs)), dim3(kThreads), kSmemBytes, s, p));
-    return BT_OK;
+    return narrow(p.M, p.N, p.splits, kMode != kInput) ? launch_n<kMode, 128>(p) : launch_n<kMode, 256>(p);
   }
   // A row-major T output (or dh) of `cols` columns: by TMA where its rows suit it.
   static bool suits(int cols) { return cols % (16 / (int)sizeof(T)) == 0; }
@@ -661,8 +675,9 @@ struct Run {
     p.M = l.M, p.N = l.K, p.K = l.N, p.splits = 1, p.depth = ceil_div(l.N, BK);
     BT_TRY(maps(&p.map[0], reinterpret_cast<const __nv_bfloat16*>(ws + w.dg), l.M, l.N, w.ldn, BM));
     BT_TRY(maps(&p.map[kP], reinterpret_cast<const __nv_bfloat16*>(ws + w.du), l.M, l.N, w.ldn, BM));
-    BT_TRY(maps(&p.map[2 * kP], wg, l.K, l.N, ldw, kBN));
-    BT_TRY(maps(&p.map[3 * kP], wu, l.K, l.N, ldw, kBN));
+    const int box = narrow(p.M, p.N, 1, false) ? 128 : 256;
+    BT_TRY(maps(&p.map[2 * kP], wg, l.K, l.N, ldw, box));
+    BT_TRY(maps(&p.map[3 * kP], wu, l.K, l.N, ldw, box));
     p.nseg = segments(p.seg, 2, false);
     p.ldo = l.K;
     if (suits(l.K)) BT_TRY(tile_map(&p.out[0], dx, l.M, l.K));

@@ -5,8 +5,12 @@
 //   P = (a b^T) * e^{(i - j) g} on and below the diagonal, 0 across a cut
 //   out = out_scale (in_scale P c + e^{(i + e0) g} a S)      rows before the chunk's first cut
 //   S = e^{(n - 1 + e0) g} S + in_scale sum_j e^{(n - 1 - j) g} b_j c_j^T
-// A block owns one (batch row, head) and 64 columns of c; the state stays in shared memory for
-// the block's whole walk. Sequences too few to fill the GPU are split along the steps: a first
+// A block owns one (batch row, head) and DS columns of c; the state stays in shared memory for the
+// block's whole walk. It serves float32, and bf16 whose rows do not start on 16-byte boundaries. A row
+// takes only the columns from its last cut to itself, so what a cut or the future hides is not read, whatever
+// it holds. Bound by the latency of the walk where sequences are few: blocks of 16 columns then, four times
+// as many, each a third as long (48 x 100 x 3 x 48 float32: 83 us with 64 columns, 41 with 16).
+// Sequences too few to fill the GPU are split along the steps: a first
 // launch sums each split from an empty state, a second joins the sums into the states that enter
 // the splits (S_{s+1} = e^{len g} S_s + local_s), a third runs the splits from those.
 #include <type_traits>
@@ -18,50 +22,56 @@ namespace la {
 namespace {
 
 constexpr int kC = 32;       // positions of a chunk
-constexpr int kDS = 64;      // columns of c (and of the state) of a block
 constexpr int kThreads = 256;
+constexpr int kWide = 64, kNarrow = 16;  // columns of c (and of the state) of a block
 
-template <int DA>
+template <int DA, int DS>
 struct Smem {
-  float a[kC][DA + 4], b[kC][DA + 4], c[kC][kDS + 4], s[DA][kDS + 4], p[kC][kC + 1];
+  float a[kC][DA + 4], b[kC][DA + 4], c[kC][DS + 4], s[DA][DS + 4], p[kC][kC + 1];
   float pw[kC + 2], pl[kC + 2];  // e^{i g} and what its rounding left
-  int seg[kC];
+  int first[kC];                 // of a row: the first position of its own stretch between cuts
 };
 
-template <class T>
-__device__ __forceinline__ void load_rows(const Op& o, const Rows& r, int batch, int head, int i0,
-                                          int n, int d0, int d, int width, float* dst, int ld) {
-  const T* p = static_cast<const T*>(r.p) + batch * r.batch + head * r.head;
-  for (int e = threadIdx.x; e < kC * width; e += kThreads) {
-    const int i = e / width, x = e % width;
+template <class T, int W>
+__device__ __forceinline__ void load_rows(const Op& o, const Rows& r, int batch, int head, int i0, int n, int d0, int d,
+                                          float* dst, int ld, bool vec) {
+  const T* p = static_cast<const T*>(r.p) + batch * r.batch + head * r.head + d0;
+  if (sizeof(T) == 4 && vec) {  // rows on 16-byte boundaries, a multiple of 4 columns
+#pragma unroll
+    for (int e = threadIdx.x; e < kC * W / 4; e += kThreads) {
+      const int i = e / (W / 4), x = e % (W / 4) * 4;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < n && d0 + x < d) v = *reinterpret_cast<const float4*>(p + (int64_t)op_time(o, i0 + i) * r.step + x);
+      *reinterpret_cast<float4*>(dst + i * ld + x) = v;
+    }
+    return;
+  }
+#pragma unroll 8
+  for (int e = threadIdx.x; e < kC * W; e += kThreads) {
+    const int i = e / W, x = e % W;
     float v = 0.f;
-    if (i < n && d0 + x < d) v = to_float(p[(int64_t)op_time(o, i0 + i) * r.step + d0 + x]);
+    if (i < n && d0 + x < d) v = to_float(p[(int64_t)op_time(o, i0 + i) * r.step + x]);
     dst[i * ld + x] = v;
   }
 }
 
 // kOut: outputs and (split s) from the state that enters the split; else the split's own sum.
-template <class T, int DA, bool kOut>
-__global__ void __launch_bounds__(kThreads) chunk_kernel(const __grid_constant__ Ops ops) {
+template <class T, int DA, int DS, bool kOut>
+__global__ void __launch_bounds__(kThreads) chunk_kernel(const __grid_constant__ Ops ops, bool vec) {
   const Op& o = ops.op[blockIdx.z];
   extern __shared__ __align__(16) uint8_t raw[];
-  Smem<DA>& sm = *reinterpret_cast<Smem<DA>*>(raw);
-  const int slices = ceil_div(o.Dc, kDS);
+  Smem<DA, DS>& sm = *reinterpret_cast<Smem<DA, DS>*>(raw);
+  const int slices = ceil_div(o.Dc, DS);
   if ((int)blockIdx.x >= o.batch * o.heads * slices) return;
-  const int bh = blockIdx.x / slices, d0 = blockIdx.x % slices * kDS;
+  const int bh = blockIdx.x / slices, d0 = blockIdx.x % slices * DS;
   const int batch = bh / o.heads, head = bh % o.heads;
   const int split = blockIdx.y;
   const int begin = split * o.split_len, end = min(o.steps, begin + o.split_len);
   const int tid = threadIdx.x;
   const float g = fmaxf(o.log_decay[head], kMinLogDecay);
-  const int DcV = min(kDS, o.Dc - d0);
+  const int DcV = min(DS, o.Dc - d0);
   const size_t elems = (size_t)o.Da * o.Dc;
 
-  if (tid < kC + 2) {
-    const double e = exp((double)tid * (double)g);
-    sm.pw[tid] = (float)e;
-    sm.pl[tid] = (float)(e - (double)(float)e);
-  }
   const float* from = nullptr;
   int sx = o.sx, sy = o.sy;
   if (kOut) {
@@ -73,9 +83,16 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(const __grid_constant__
       from = o.init + bh * elems;
     }
   }
-  for (int e = tid; e < DA * kDS; e += kThreads) {
-    const int x = e / kDS, y = e % kDS;
+#pragma unroll 4
+  for (int e = tid; e < DA * DS; e += kThreads) {
+    // neighbouring threads along the state's own rows
+    const int x = sy == 1 ? e / DS : e % DA, y = sy == 1 ? e % DS : e / DA;
     sm.s[x][y] = from && x < o.Da && y < DcV ? from[(size_t)x * sx + (size_t)(d0 + y) * sy] : 0.f;
+  }
+  if (tid < kC + 2) {
+    const double e = exp((double)tid * (double)g);
+    sm.pw[tid] = (float)e;
+    sm.pl[tid] = (float)(e - (double)(float)e);
   }
   bool any_cut = false;
   // decays that the entering state meets before position `begin`
@@ -84,21 +101,23 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(const __grid_constant__
   for (int i0 = begin; i0 < end; i0 += kC) {
     const int n = min(kC, end - i0);
     __syncthreads();
-    if (kOut) load_rows<T>(o, o.a, batch, head, i0, n, 0, o.Da, DA, &sm.a[0][0], DA + 4);
-    load_rows<T>(o, o.b, batch, head, i0, n, 0, o.Da, DA, &sm.b[0][0], DA + 4);
-    load_rows<T>(o, o.c, batch, head, i0, n, d0, o.Dc, kDS, &sm.c[0][0], kDS + 4);
+    if (kOut) load_rows<T, DA>(o, o.a, batch, head, i0, n, 0, o.Da, &sm.a[0][0], DA + 4, vec);
+    load_rows<T, DA>(o, o.b, batch, head, i0, n, 0, o.Da, &sm.b[0][0], DA + 4, vec);
+    load_rows<T, DS>(o, o.c, batch, head, i0, n, d0, o.Dc, &sm.c[0][0], DS + 4, vec);
     if (tid < kC) {
       const unsigned m = __ballot_sync(~0u, tid < n && op_cut(o, batch, i0 + tid));
-      sm.seg[tid] = __popc(m & (~0u >> (31 - tid)));
+      const unsigned own = m & (~0u >> (31 - tid));
+      sm.first[tid] = own ? 31 - __clz(own) : -1;
     }
     __syncthreads();
-    const int seg_end = sm.seg[kC - 1];
-    any_cut |= seg_end > 0;
+    const int last = sm.first[kC - 1];  // the chunk's last cut; what comes before it leaves nothing
+    any_cut |= last >= 0;
 
     if (kOut) {
       {  // P: row i = tid / 8, columns tid % 8 + 8 m
         const int i = tid >> 3, j0 = tid & 7;
         float acc[4] = {};
+#pragma unroll 4
         for (int k = 0; k < DA; k += 4) {
           const float4 x = *reinterpret_cast<const float4*>(&sm.a[i][k]);
 #pragma unroll
@@ -110,63 +129,46 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(const __grid_constant__
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           const int j = j0 + 8 * m;
-          const bool on = j <= i && sm.seg[i] == sm.seg[j];
-          sm.p[i][j] = on ? acc[m] * sm.pw[i - j] * o.in_scale : 0.f;
+          sm.p[i][j] = j <= i && j >= sm.first[i] ? acc[m] * sm.pw[i - j] * o.in_scale : 0.f;
         }
       }
       __syncthreads();
-      // out: rows 2 r, 2 r + 1, columns 4 q .. 4 q + 3
-      const int r = tid >> 4, y = (tid & 15) * 4;
-      float acc[2][4] = {}, st[2][4] = {};
-      for (int j = 0; j <= 2 * r + 1; ++j) {
-        const float4 c = *reinterpret_cast<const float4*>(&sm.c[j][y]);
+      // out: row i = tid / 8, columns DS / 8 of them
+      constexpr int kW = DS / 8;
+      const int i = tid >> 3, y = (tid & 7) * kW;
+      float acc[kW] = {}, st[kW] = {};
+      const int first = sm.first[i];
+      for (int j = max(first, 0); j <= i; ++j) {
+        const float p = sm.p[i][j];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (j > 2 * r + u || sm.seg[2 * r + u] != sm.seg[j]) continue;
-          const float p = sm.p[2 * r + u][j];
-          acc[u][0] += p * c.x;
-          acc[u][1] += p * c.y;
-          acc[u][2] += p * c.z;
-          acc[u][3] += p * c.w;
-        }
+        for (int w = 0; w < kW; ++w) acc[w] += p * sm.c[j][y + w];
       }
-      for (int k = 0; k < DA; k += 4) {
-        float4 x[2];
+      if (first < 0) {
+#pragma unroll 4
+        for (int k = 0; k < DA; k += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(&sm.a[i][k]);
+          const float xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int u = 0; u < 2; ++u) x[u] = *reinterpret_cast<const float4*>(&sm.a[2 * r + u][k]);
+          for (int v = 0; v < 4; ++v)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float4 s = *reinterpret_cast<const float4*>(&sm.s[k + w][y]);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float xv = w == 0 ? x[u].x : w == 1 ? x[u].y : w == 2 ? x[u].z : x[u].w;
-            st[u][0] += xv * s.x;
-            st[u][1] += xv * s.y;
-            st[u][2] += xv * s.z;
-            st[u][3] += xv * s.w;
-          }
+            for (int w = 0; w < kW; ++w) st[w] += xs[v] * sm.s[k + v][y + w];
         }
+        const float reach = sm.pw[i + e0];
+#pragma unroll
+        for (int w = 0; w < kW; ++w) acc[w] += reach != 0.f ? reach * st[w] : 0.f;
       }
+      if (i < n) {
+        T* out = static_cast<T*>(o.out) + batch * o.out_batch + (int64_t)op_time(o, i0 + i) * o.out_step +
+                 head * o.out_head + d0 + y;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int i = 2 * r + u;
-        if (i >= n) continue;
-        const float reach = sm.seg[i] == 0 ? sm.pw[i + e0] : 0.f;
-        T* out = static_cast<T*>(o.out) + batch * o.out_batch +
-                 (int64_t)op_time(o, i0 + i) * o.out_step + head * o.out_head + d0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          if (y + w >= DcV) continue;
-          // a cut drops the state whatever it holds, not 0 times it
-          const float v = reach != 0.f ? acc[u][w] + reach * st[u][w] : acc[u][w];
-          out[y + w] = from_float<T>(v * o.out_scale);
-        }
+        for (int w = 0; w < kW; ++w)
+          if (y + w < DcV) out[w] = from_float<T>(acc[w] * o.out_scale);
       }
       __syncthreads();
     }
-    {  // state: rows DA / 16 * r .., columns 4 q ..
-      constexpr int kR = DA / 16;
-      const int x0 = (tid >> 4) * kR, y = (tid & 15) * 4;
+    {  // state: kR rows, four columns
+      constexpr int kCols = DS / 4, kR = DA * kCols / kThreads;
+      const int x0 = tid / kCols * kR, y = tid % kCols * 4;
       // the same factor meets the state once a chunk, so its rounding would add up over a long
       // memory: two parts leave only the roundings of the sums, which do not lean one way
       const float keep = sm.pw[n - 1 + e0], keep_lo = sm.pl[n - 1 + e0];
@@ -175,18 +177,19 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(const __grid_constant__
       for (int u = 0; u < kR; ++u)
 #pragma unroll
         for (int w = 0; w < 4; ++w)
-          acc[u][w] = seg_end == 0 ? fmaf(keep, sm.s[x0 + u][y + w], keep_lo * sm.s[x0 + u][y + w]) : 0.f;
-      for (int j = 0; j < n; ++j) {
-        if (sm.seg[j] != seg_end) continue;
+          acc[u][w] = last < 0 ? fmaf(keep, sm.s[x0 + u][y + w], keep_lo * sm.s[x0 + u][y + w]) : 0.f;
+#pragma unroll 4
+      for (int j = max(last, 0); j < n; ++j) {
         const float wj = sm.pw[n - 1 - j] * o.in_scale;
         const float4 c = *reinterpret_cast<const float4*>(&sm.c[j][y]);
+        const float4 wc = make_float4(c.x * wj, c.y * wj, c.z * wj, c.w * wj);
 #pragma unroll
         for (int u = 0; u < kR; ++u) {
-          const float b = sm.b[j][x0 + u] * wj;
-          acc[u][0] += b * c.x;
-          acc[u][1] += b * c.y;
-          acc[u][2] += b * c.z;
-          acc[u][3] += b * c.w;
+          const float b = sm.b[j][x0 + u];
+          acc[u][0] += b * wc.x;
+          acc[u][1] += b * wc.y;
+          acc[u][2] += b * wc.z;
+          acc[u][3] += b * wc.w;
         }
       }
 #pragma unroll
@@ -198,7 +201,7 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(const __grid_constant__
   }
   __syncthreads();
   float* to = nullptr;
-  float last = 1.f;
+  float way_out = 1.f;
   if (kOut) {
     if (o.fin && split == o.nsplit - 1) {
       to = o.fin + bh * elems;
@@ -206,8 +209,8 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(const __grid_constant__
       sy = o.sy;
       // backwards: the way out of position steps - 1 passes reset[0] and one decay
       if (o.reverse && o.steps > 0) {
-        last = sm.pw[1];
-        if (o.reset && o.reset[batch * o.reset_batch]) last = 0.f;
+        way_out = sm.pw[1];
+        if (o.reset && o.reset[batch * o.reset_batch]) way_out = 0.f;
       }
     }
   } else {
@@ -217,10 +220,11 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(const __grid_constant__
     if (tid == 0 && d0 == 0 && head == 0) o.cut[split * o.batch + batch] = any_cut;
   }
   if (to) {
-    for (int e = tid; e < DA * kDS; e += kThreads) {
-      const int x = e / kDS, y = e % kDS;
+#pragma unroll 4
+    for (int e = tid; e < DA * DS; e += kThreads) {
+      const int x = sy == 1 ? e / DS : e % DA, y = sy == 1 ? e % DS : e / DA;
       if (x < o.Da && y < DcV)
-        to[(size_t)x * sx + (size_t)(d0 + y) * sy] = last == 0.f ? 0.f : last * sm.s[x][y];
+        to[(size_t)x * sx + (size_t)(d0 + y) * sy] = way_out == 0.f ? 0.f : way_out * sm.s[x][y];
     }
   }
 }
@@ -237,13 +241,24 @@ __global__ void join_kernel(const __grid_constant__ Ops ops) {
   float s = o.init ? o.init[bh * elems + (int64_t)x * o.sx + (int64_t)y * o.sy] : 0.f;
   const double full = exp((double)o.split_len * (double)g);
   const double first = o.reverse ? exp((double)(o.split_len - 1) * (double)g) : full;
-  for (int k = 0; k + 1 < o.nsplit; ++k) {
-    const float own = o.local[(int64_t)k * total + e];
-    s = o.cut[k * o.batch + batch] ? own : (float)((k == 0 ? first : full) * (double)s + (double)own);
-    o.local[(int64_t)k * total + e] = s;
+  // the sums come eight at a time: only the states follow from one another
+  for (int k0 = 0; k0 + 1 < o.nsplit; k0 += 8) {
+    float own[8];
+    bool cut[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const bool in = k0 + u + 1 < o.nsplit;
+      own[u] = in ? o.local[(int64_t)(k0 + u) * total + e] : 0.f;
+      cut[u] = in && o.cut[(k0 + u) * o.batch + batch];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (k0 + u + 1 >= o.nsplit) break;
+      s = cut[u] ? own[u] : (float)((k0 + u == 0 ? first : full) * (double)s + (double)own[u]);
+      o.local[(int64_t)(k0 + u) * total + e] = s;
+    }
   }
 }
-
 
 // One position of every (batch row, head): S' = [not reset] e^g S + k v^T, out = scale S'^T q.
 // A block takes one (batch row, head); thread (r, y) holds the columns V y .. V y + V - 1 of the
@@ -312,40 +327,51 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+template <class T, int DA, int DS>
+int run_chunks(const Ops& ops, bool vec, cudaStream_t stream) {
+  const Op& o = ops.op[0];
+  constexpr int kSmem = sizeof(Smem<DA, DS>);
+  int blocks = 0;
+  for (int i = 0; i < ops.n; ++i) blocks = max(blocks, o.batch * o.heads * ceil_div(ops.op[i].Dc, DS));
+  if (o.nsplit > 1) {
+    BT_CUDA(cudaFuncSetAttribute(chunk_kernel<T, DA, DS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    chunk_kernel<T, DA, DS, false><<<dim3(blocks, o.nsplit - 1, ops.n), kThreads, kSmem, stream>>>(ops, vec);
+    BT_LAUNCH_CHECK("linear attention split sums");
+    BT_TRY(launch_join(ops, stream));
+  }
+  BT_CUDA(cudaFuncSetAttribute(chunk_kernel<T, DA, DS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  chunk_kernel<T, DA, DS, true><<<dim3(blocks, o.nsplit, ops.n), kThreads, kSmem, stream>>>(ops, vec);
+  BT_LAUNCH_CHECK("linear attention");
+  return BT_OK;
+}
+
 template <class T>
-int run_ops(Ops& ops, cudaStream_t stream) {
-  int da = 0, blocks = 0;
+int run_ops(const Ops& ops, cudaStream_t stream) {
+  int da = 0, dc = 0;
+  bool vec = sizeof(T) == 4;
   for (int i = 0; i < ops.n; ++i) {
     const Op& o = ops.op[i];
     da = max(da, o.Da);
-    blocks = max(blocks, o.batch * o.heads * ceil_div(o.Dc, kDS));
+    dc = max(dc, o.Dc);
+    auto rows = [&](const Rows& r) {
+      auto ok = [](int64_t s, int n) { return n <= 1 || s % 4 == 0; };
+      return ((uintptr_t)r.p & 15) == 0 && ok(r.step, o.steps) && ok(r.head, o.heads) && ok(r.batch, o.batch);
+    };
+    vec = vec && o.Da % 4 == 0 && o.Dc % 4 == 0 && rows(o.a) && rows(o.b) && rows(o.c);
   }
+  // narrow blocks while wide ones would leave SMs with less than two
   const Op& o = ops.op[0];
-  auto go = [&](auto size) -> int {
-    constexpr int DA = decltype(size)::value;
-    constexpr int kSmem = sizeof(Smem<DA>);
-    BT_CUDA(cudaFuncSetAttribute(chunk_kernel<T, DA, false>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-    BT_CUDA(cudaFuncSetAttribute(chunk_kernel<T, DA, true>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-    if (o.nsplit > 1) {
-      chunk_kernel<T, DA, false><<<dim3(blocks, o.nsplit - 1, ops.n), kThreads, kSmem, stream>>>(ops);
-      BT_LAUNCH_CHECK("linear attention split sums");
-      BT_TRY(launch_join(ops, stream));
-    }
-    chunk_kernel<T, DA, true><<<dim3(blocks, o.nsplit, ops.n), kThreads, kSmem, stream>>>(ops);
-    BT_LAUNCH_CHECK("linear attention");
-    return BT_OK;
-  };
-  if (da <= 64) return go(std::integral_constant<int, 64>{});
-  return go(std::integral_constant<int, 128>{});
+  const bool narrow = (int64_t)o.batch * o.heads * ceil_div(dc, kWide) * o.nsplit * ops.n < 4 * kNumSMs;
+  if (da <= 64)
+    return narrow ? run_chunks<T, 64, kNarrow>(ops, vec, stream) : run_chunks<T, 64, kWide>(ops, vec, stream);
+  return narrow ? run_chunks<T, 128, kNarrow>(ops, vec, stream) : run_chunks<T, 128, kWide>(ops, vec, stream);
 }
 
 // Splits of the steps: the number whose launches are the shortest, in units of the walk over 128 steps. Two
 // blocks share an SM (one alone is faster by about a third); a sequence costs a third of a unit to begin,
 // the sums of the splits half of a full walk, and the two more launches about two units.
 void choose_splits(const bt_linear_attention_shape* s, int ops, int* nsplit, int* len) {
-  const int64_t blocks = (int64_t)s->batch * s->heads * ceil_div(max(s->key_dim, s->value_dim), kDS) * ops;
+  const int64_t blocks = (int64_t)s->batch * s->heads * ceil_div(max(s->key_dim, s->value_dim), kWide) * ops;
   const int chunks = max(1, ceil_div(s->steps, 128));
   int best = chunks;
   double least = 1e300;
