@@ -7,18 +7,22 @@
 //             K <= 800 reading two fp32 values per element back costs more than 4 K flops do)
 //   kInput    dx = dG Wg^T + dU Wu^T         the two products in one accumulator
 //   kWeights  dWg = x^T dG, dWu = x^T dU     both from one load of x, split over the rows
-// A CTA per SM walks the output tiles (of half the width where there are fewer tiles than SMs). Warp 0 loads 64-deep blocks of A and B by TMA into a ring of
-// four 48 KB stages, warp 1 issues the MMAs into one of two 256-column accumulators in tensor
-// memory, and eight epilogue warps drain the other: activation and product in registers, the
-// result through 4 KB of shared memory per warp to TMA stores.
+// A tile belongs to a cluster of two CTAs on neighbouring SMs (cta_group::2): each holds 128 of its 256 rows
+// and one half of the columns of B (of the projections: one of them each), the leader issues one MMA of M =
+// 256 over both, and each has its own rows of the accumulator. So a CTA loads 32 KB for 512 cycles of MMA;
+// alone it would load 48 KB, and 148 SMs doing that stood at what L2 gives, 12 TB/s (measured: 1.06
+// PFLOP/s). Pairs walk the tiles (of half the width where that fills more SMs). Warp 0 loads 64-deep blocks
+// by TMA into a ring of six stages, signalling the leader; the leader's warp 1 issues the MMAs into one of
+// two 256-column accumulators in tensor memory, and eight epilogue warps drain the other: activation and
+// product in registers, the result through 4 KB of shared memory per warp to TMA stores.
 //
 // fp32 operands are three bf16 planes each, x = x0 + x1 + x2 (24 bits), and a product is the six
-// plane products whose size reaches 2^-24 of it: (0,2) (1,1) (2,0) (0,1) (1,0) (0,0), added in that
-// order, smallest first. The accumulator truncates, so for fp32 it is handed to fp32 registers after
-// every 64-deep block (24 MMAs); 270 of the 1622 bf16 TFLOP/s remain, about four times what the
-// CUDA cores' fp32 FMA does.
+// plane products whose size reaches 2^-24 of it: (2,0) (0,2) (1,1) (0,1) (1,0) (0,0), added in that
+// order, smallest first, from one load of each plane. The accumulator truncates, so for fp32 it is handed to
+// fp32 registers after every 64-deep block (24 MMAs); a sixth of the bf16 rate remains, which is
+// four times what the CUDA cores' fp32 FMA does.
 //
-// Bound by the tensor cores: 128 x 256 x 64 per 48 KB of operands, 512 cycles of MMA a block.
+// Bound by the tensor cores.
 #include <type_traits>
 
 #include "gemm_sm100.cuh"
@@ -36,24 +40,19 @@ using namespace umma;
 enum Mode { kForward, kGrads, kInput, kWeights };
 
 constexpr int kAB = BM * BK * 2;
+constexpr int kPairs = kNumSMs / 2;
 // N columns of the MMA: 256, or 128 where that many would leave SMs without a tile.
 template <int N>
 struct Ring {
-  static constexpr int kStages = N == 256 ? 4 : 6;
-  static constexpr int kStageBytes = kAB + N * BK * 2;
+  static constexpr int kStages = 6;
+  static constexpr int kStageBytes = kAB + N / 2 * BK * 2;  // of one CTA of the pair
   static constexpr int kSmem = kStages * kStageBytes + kEpiWarps * kEpiWarpBytes + 1024 + 256;
   static_assert(kSmem <= kMaxSmem, "stage ring");
-};
-
-struct Seg {
-  uint8_t a, b0, b1;  // maps of a product's A and of its B (kInput: b0 alone)
 };
 
 struct Params {
   CUtensorMap map[12];
   CUtensorMap out[6], in;
-  Seg seg[12];
-  int nseg;
   int M, N, K;        // of the product: rows and columns of the output, depth
   int act;
   int splits, depth;  // kWeights: 64-deep blocks of a split
@@ -63,6 +62,55 @@ struct Params {
   int plane_rows;     // kWeights with splits: rows of one partial plane
   int* err;
 };
+
+// ---- the two CTAs of a pair ----
+__device__ __forceinline__ uint32_t pair_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A load into this CTA's shared memory that reports to the leader's barrier.
+__device__ __forceinline__ void pair_load_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar) & 0xFEFFFFFFu)
+      : "memory");
+}
+__device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives at the barrier of both CTAs when the MMAs issued so far are done.
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void leader_arrive(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %0, 0;\n\t"
+      "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t* slot, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
 
 template <class T>
 __device__ __forceinline__ T from_f32(float x) {
@@ -172,11 +220,12 @@ __device__ __forceinline__ void put_planes(const CUtensorMap* maps, int row0, in
 // T: the layer's type. An fp32 layer's operands are planes and its accumulator is handed over after
 // every 64-deep block.
 template <class T, Mode kMode, int kN>
-__global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant__ Params p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant__ Params p) {
   constexpr int kStages = Ring<kN>::kStages, kStageBytes = Ring<kN>::kStageBytes;
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr bool kDual = kMode != kInput;
   constexpr bool A_MN = kMode == kWeights, B_MN = kMode != kInput;
+  constexpr int kP = kF32 ? 3 : 1, kSums = kDual ? 1 : 2;  // planes of an operand, products in a sum
   constexpr int kTileN = kDual ? kN / 2 : kN;
   constexpr int kGroups = kN / 64;  // groups of 32 accumulator columns of an epilogue warp
   // 64-deep blocks between two hand-overs of the accumulator: bf16 results keep 2^-8, far above what
@@ -202,26 +251,28 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], kEpiWarps);
+      mbar_init(&acc_empty[b], 2 * kEpiWarps);  // (the leader's) both CTAs' epilogue warps
     }
     for (int w = 0; w < kEpiWarps; ++w) mbar_init(&epi_in[w], 1);
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, 2 * kN);
+  if (warp == 1) pair_tmem_alloc(tmem_slot, 2 * kN);
   fence_before_sync();
-  __syncthreads();
+  __syncwarp();
+  pair_sync();
   fence_after_sync();
+  const int rank = (int)pair_rank();
   const uint32_t tmem = *tmem_slot;
   auto failed = [&]() { return *(volatile int*)&s_fail != 0; };
   pdl_wait();
-  const int ntn = ceil_div(p.N, kTileN), ntm = ceil_div(p.M, BM);
+  const int ntn = ceil_div(p.N, kTileN), ntm = ceil_div(p.M, 2 * BM);
   const int nk = ceil_div(p.K, BK);
   const int tiles = ntm * ntn * p.splits;
   // the splits of one tile lie far apart, the column tiles of one row block together
   auto where = [&](int t, int& m0, int& n0, int& k0, int& k1, int& split) {
     split = t / (ntm * ntn);
     const int u = t % (ntm * ntn);
-    m0 = u / ntn * BM;
+    m0 = u / ntn * (2 * BM) + rank * BM;
     n0 = u % ntn * kTileN;
     k0 = split * p.depth;
     k1 = min(nk, k0 + p.depth);
@@ -230,12 +281,12 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
   if (warp == 0) {
     if (lane == 0) {
       int g = 0;
-      for (int t = blockIdx.x; t < tiles && !failed(); t += gridDim.x) {
+      for (int t = blockIdx.x >> 1; t < tiles && !failed(); t += gridDim.x >> 1) {
         int m0, n0, k0, k1, split;
         where(t, m0, n0, k0, k1, split);
         for (int kb = k0; kb < k1 && !failed(); ++kb) {
           const int k = kb * BK;
-          for (int e = 0; e < p.nseg; ++e, ++g) {
+          for (int e = 0; e < kSums * kP; ++e, ++g) {
             const int s = g % kStages;
             if (g >= kStages && !mbar_wait_bounded(&empty[s], ((g / kStages) - 1) & 1)) {
               atomicExch(&s_fail, kErrTimeoutEmpty);
@@ -243,39 +294,42 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
             }
             uint8_t* sa = smem + s * kStageBytes;
             uint8_t* sb = sa + kAB;
-            mbar_arrive_expect_tx(&full[s], kStageBytes);
-            const Seg sg = p.seg[e];
+            // both CTAs' bytes
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStageBytes);
+            const int q = e / kP, z = kP - 1 - e % kP;  // the smallest plane first
+            const CUtensorMap* ma = &p.map[kDual ? z : q * kP + z];
+            const CUtensorMap* mb = &p.map[kDual ? (1 + rank) * kP + z : (2 + q) * kP + z];
             if (A_MN) {
-              tma_load_2d(sa, &p.map[sg.a], m0, k, &full[s]);
-              tma_load_2d(sa + 8192, &p.map[sg.a], m0 + 64, k, &full[s]);
+              pair_load_2d(sa, ma, m0, k, &full[s]);
+              pair_load_2d(sa + 8192, ma, m0 + 64, k, &full[s]);
             } else {
-              tma_load_2d(sa, &p.map[sg.a], k, m0, &full[s]);
+              pair_load_2d(sa, ma, k, m0, &full[s]);
             }
             if (kDual) {
 #pragma unroll
-              for (int j = 0; j < kN / 64; ++j)
-                tma_load_2d(sb + j * 8192, &p.map[j < kN / 128 ? sg.b0 : sg.b1], n0 + 64 * (j % (kN / 128)), k, &full[s]);
+              for (int j = 0; j < kN / 128; ++j) pair_load_2d(sb + j * 8192, mb, n0 + 64 * j, k, &full[s]);
             } else {
-              tma_load_2d(sb, &p.map[sg.b0], k, n0, &full[s]);
+              pair_load_2d(sb, mb, k, n0 + rank * (kN / 2), &full[s]);
             }
           }
         }
       }
-      // every copy lands before the CTA may leave
+      // every stage is consumed (and so loaded) before the pair may leave
       for (int i = max(0, g - kStages); i < g; ++i)
-        if (!mbar_wait_bounded(&full[i % kStages], (i / kStages) & 1)) atomicExch(&s_fail, kErrTimeoutFull);
+        if (!mbar_wait_bounded(&empty[i % kStages], (i / kStages) & 1)) atomicExch(&s_fail, kErrTimeoutEmpty);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = instr_desc<kN, A_MN, B_MN>();
+    if (lane == 0 && rank == 0) {
+      // M = 256 over the pair
+      constexpr uint32_t idesc = instr_desc<kN, A_MN, B_MN>() + ((uint32_t)(BM >> 4) << 24);
       int g = 0, c = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok && !failed(); t += gridDim.x) {
+      for (int t = blockIdx.x >> 1; t < tiles && ok && !failed(); t += gridDim.x >> 1) {
         int m0, n0, k0, k1, split;
         where(t, m0, n0, k0, k1, split);
         for (int kb = k0; kb < k1 && ok; ++kb) {
-          const bool fresh = (kb - k0) % kHand == 0;
-          if (fresh && c >= 2) {
+          bool keep = (kb - k0) % kHand != 0;
+          if (!keep && c >= 2) {
             if (!mbar_wait_bounded(&acc_empty[c & 1], ((c >> 1) - 1) & 1)) {
               atomicExch(&s_fail, kErrTimeoutAcc);
               ok = false;
@@ -284,23 +338,42 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
             fence_after_sync();
           }
           const uint32_t acc = tmem + (uint32_t)((c & 1) * kN);
-          for (int e = 0; e < p.nseg; ++e, ++g) {
-            const int s = g % kStages;
-            if (!mbar_wait_bounded(&full[s], (g / kStages) & 1)) {
-              atomicExch(&s_fail, kErrTimeoutFull);
-              ok = false;
-              break;
-            }
-            fence_after_sync();
-            const uint32_t sa = smem_u32(smem + s * kStageBytes), sb = sa + kAB;
+          for (int q = 0; q < kSums && ok; ++q, g += kP) {
+            uint32_t at[kP];  // the planes' stages, by plane
+            uint64_t* done[kP];
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k)
-              mma_bf16(acc, operand_desc<A_MN>(sa, k), operand_desc<B_MN>(sb, k), idesc,
-                       (!fresh || e > 0 || k > 0) ? 1u : 0u);
-            mma_commit(&empty[s]);
+            for (int e = 0; e < kP; ++e) {
+              const int s = (g + e) % kStages;
+              if (!mbar_wait_bounded(&full[s], ((g + e) / kStages) & 1)) {
+                atomicExch(&s_fail, kErrTimeoutFull);
+                ok = false;
+              }
+              at[kP - 1 - e] = smem_u32(smem + s * kStageBytes);
+              done[kP - 1 - e] = &empty[s];
+            }
+            if (!ok) break;
+            fence_after_sync();
+            auto product = [&](int x, int y) {
+#pragma unroll
+              for (int k = 0; k < BK / 16; ++k) {
+                pair_mma(acc, operand_desc<A_MN>(at[x], k), operand_desc<B_MN>(at[y] + kAB, k), idesc, keep ? 1u : 0u);
+                keep = true;
+              }
+            };
+            if constexpr (kP == 3) {
+              product(2, 0);
+              product(0, 2);
+              pair_commit(done[2]);
+              product(1, 1);
+              product(0, 1);
+              product(1, 0);
+              pair_commit(done[1]);
+            }
+            product(0, 0);
+            pair_commit(done[0]);
           }
           if (ok && ((kb - k0) % kHand == kHand - 1 || kb == k1 - 1)) {
-            mma_commit(&acc_full[c & 1]);
+            pair_commit(&acc_full[c & 1]);
             ++c;
           }
         }
@@ -318,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
     float run[kF32 ? kGroups : 1][32];
     int c = 0, loads = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok && !failed(); t += gridDim.x) {
+    for (int t = blockIdx.x >> 1; t < tiles && ok && !failed(); t += gridDim.x >> 1) {
       int m0, n0, k0, k1, split;
       where(t, m0, n0, k0, k1, split);
       const int row0 = m0 + q * 32;
@@ -340,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
           }
           fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[c & 1]);
+          if (lane == 0) leader_arrive(&acc_empty[c & 1]);
         }
       } else {
         ok = mbar_wait_bounded(&acc_full[c & 1], (c >> 1) & 1);
@@ -363,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
         if constexpr (!kF32) {
           fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[c & 1]);
+          if (lane == 0) leader_arrive(&acc_empty[c & 1]);
           ++c;
         }
       };
@@ -461,10 +534,11 @@ __global__ void __launch_bounds__(kThreads, 1) glu_kernel(const __grid_constant_
     __syncwarp();
   }
   fence_before_sync();
-  __syncthreads();
+  __syncwarp();
+  pair_sync();
   if (warp == 1) {
     fence_after_sync();
-    tmem_dealloc(tmem, 2 * kN);
+    pair_tmem_dealloc(tmem, 2 * kN);
   }
   if (threadIdx.x == 0 && s_fail) atomicExch(p.err, s_fail);
 }
@@ -526,15 +600,15 @@ int round_up(int x, int m) { return (x + m - 1) / m * m; }
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 // Splits of the rows for the weight gradients: whole waves of tiles against the partial planes' way
-// through memory (written and read once at about 5 TB/s); a 64-deep block of a tile takes 0.33 us
+// through memory (written and read once at about 5 TB/s); a 64-deep block of a tile takes 0.3 us
 // (fp32: six times that).
 int choose_splits(int M, int K, int N, int planes) {
-  const int tiles = ceil_div(K, BM) * ceil_div(N, 128), nk = ceil_div(M, BK);
-  const double block = planes == 3 ? 2.0 : 0.33;
+  const int tiles = ceil_div(K, 2 * BM) * ceil_div(N, 128), nk = ceil_div(M, BK);
+  const double block = planes == 3 ? 1.8 : 0.3;
   int best = 1;
   double least = 1e30;
   for (int s = 1; s <= 32 && s <= nk; ++s) {
-    const double us = ceil_div(tiles * s, kNumSMs) * ceil_div(nk, s) * block +
+    const double us = ceil_div(tiles * s, kPairs) * ceil_div(nk, s) * block +
                       (s > 1 ? 2.0 + s * 2.0 * K * N * 8 / 5e6 : 0.0);
     if (us < least) least = us, best = s;
   }
@@ -568,7 +642,7 @@ Plan plan_of(const Layer& l, bool f32, bool backward) {
     w.dg = take((int64_t)w.planes * l.M * w.ldn, 2);
     w.du = take((int64_t)w.planes * l.M * w.ldn, 2);
     w.splits = choose_splits(l.M, l.K, l.N, w.planes);
-    w.plane_rows = round_up(l.K, BM);
+    w.plane_rows = round_up(l.K, 2 * BM);
     w.ldp = round_up(l.N, 4);
     if (w.splits > 1) w.part = take((int64_t)2 * w.splits * w.plane_rows * w.ldp, 4);
   }
@@ -612,29 +686,18 @@ struct Run {
       BT_TRY(encode_map(&m[k], base + k * rows * ld, cols, rows, (uint64_t)ld * 2, 64, box));
     return BT_OK;
   }
-  // The products of planes i and j with i + j <= 2, smallest first; `pairs` operand pairs each.
-  static int segments(Seg* seg, int pairs, bool dual) {
-    static const uint8_t ij[6][2] = {{0, 2}, {1, 1}, {2, 0}, {0, 1}, {1, 0}, {0, 0}};
-    int n = 0;
-    for (int k = kF32 ? 0 : 5; k < 6; ++k)
-      for (int q = 0; q < pairs; ++q) {
-        // dual: A planes, then those of both Bs. Otherwise: A0, A1, B0, B1
-        const int a = dual ? 0 : q * kP, b = dual ? kP : (2 + q) * kP;
-        seg[n++] = {(uint8_t)(a + ij[k][0]), (uint8_t)(b + ij[k][1]), (uint8_t)(b + kP + ij[k][1])};
-      }
-    return n;
-  }
-  // Whether a product's tiles of 256 accumulator columns would leave SMs without one.
+  // Whether tiles of half the width finish sooner: they take six tenths of the time each.
   static bool narrow(int M, int N, int splits, bool dual) {
-    return ceil_div(M, BM) * ceil_div(N, dual ? 128 : 256) * splits < kNumSMs;
+    const int rows = ceil_div(M, 2 * BM) * splits, w = dual ? 128 : 256;
+    return 0.6 * ceil_div(rows * ceil_div(N, w / 2), kPairs) < ceil_div(rows * ceil_div(N, w), kPairs);
   }
   template <Mode kMode, int kN>
   int launch_n(Params& p) {
     auto kernel = glu_kernel<T, kMode, kN>;
     BT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<kN>::kSmem));
     BT_TRY(operator_error_word(&p.err));
-    const int tiles = ceil_div(p.M, BM) * ceil_div(p.N, kMode == kInput ? kN : kN / 2) * p.splits;
-    BT_CUDA(launch_pdl(kernel, dim3(min(tiles, kNumSMs)), dim3(kThreads), Ring<kN>::kSmem, s, p));
+    const int tiles = ceil_div(p.M, 2 * BM) * ceil_div(p.N, kMode == kInput ? kN : kN / 2) * p.splits;
+    BT_CUDA(launch_pdl(kernel, dim3(2 * min(tiles, kPairs)), dim3(kThreads), Ring<kN>::kSmem, s, p));
     return BT_OK;
   }
   template <Mode kMode>
@@ -655,7 +718,6 @@ struct Run {
     BT_TRY(maps(&p.map[0], x, l.M, l.K, ldx, BM));
     BT_TRY(maps(&p.map[kP], wg, l.K, l.N, ldw, 64));
     BT_TRY(maps(&p.map[2 * kP], wu, l.K, l.N, ldw, 64));
-    p.nseg = segments(p.seg, 1, true);
     p.ldo = l.N;
     if constexpr (kMode == kForward) {
       if (suits(l.N)) BT_TRY(tile_map(&p.out[0], h, l.M, l.N));
@@ -675,10 +737,9 @@ struct Run {
     p.M = l.M, p.N = l.K, p.K = l.N, p.splits = 1, p.depth = ceil_div(l.N, BK);
     BT_TRY(maps(&p.map[0], reinterpret_cast<const __nv_bfloat16*>(ws + w.dg), l.M, l.N, w.ldn, BM));
     BT_TRY(maps(&p.map[kP], reinterpret_cast<const __nv_bfloat16*>(ws + w.du), l.M, l.N, w.ldn, BM));
-    const int box = narrow(p.M, p.N, 1, false) ? 128 : 256;
+    const int box = narrow(p.M, p.N, 1, false) ? 64 : 128;  // one CTA's half
     BT_TRY(maps(&p.map[2 * kP], wg, l.K, l.N, ldw, box));
     BT_TRY(maps(&p.map[3 * kP], wu, l.K, l.N, ldw, box));
-    p.nseg = segments(p.seg, 2, false);
     p.ldo = l.K;
     if (suits(l.K)) BT_TRY(tile_map(&p.out[0], dx, l.M, l.K));
     else p.o0 = dx;
@@ -692,7 +753,6 @@ struct Run {
     BT_TRY(maps(&p.map[0], x, l.M, l.K, ldx, 64));
     BT_TRY(maps(&p.map[kP], reinterpret_cast<const __nv_bfloat16*>(ws + w.dg), l.M, l.N, w.ldn, 64));
     BT_TRY(maps(&p.map[2 * kP], reinterpret_cast<const __nv_bfloat16*>(ws + w.du), l.M, l.N, w.ldn, 64));
-    p.nseg = segments(p.seg, 1, true);
     p.ldo = l.N;
     p.plane_rows = w.plane_rows;
     float* part = reinterpret_cast<float*>(ws + w.part);
