@@ -226,6 +226,15 @@ def check(code: int) -> None:
         raise BoontaError(code, lib().bt_last_error().decode(errors="replace"))
 
 
+def check_operators(device=None) -> None:
+    """Waits for the device's current stream and raises if a bounded wait inside a kernel of the
+    stateless operators (linear attention, the gated layer) gave up since the last check."""
+    import torch
+
+    with on_device(torch.cuda.current_device() if device is None else torch.device(device).index or 0) as stream:
+        check(lib().bt_operators_check(stream))
+
+
 class on_device:
     """Makes a CUDA device (its index) the current one for a call, and gives its current stream's
     handle; nothing is switched where it is current already."""

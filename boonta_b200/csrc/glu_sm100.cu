@@ -27,6 +27,7 @@
 
 #include "gemm_sm100.cuh"
 #include "glu.cuh"
+#include "launch.cuh"
 
 namespace bt {
 
@@ -543,21 +544,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) glu_ker
   if (threadIdx.x == 0 && s_fail) atomicExch(p.err, s_fail);
 }
 
-// An operand as the kernel reads it: rows of ld (a multiple of 8) bf16, kPlanes planes of them.
-// Thread: eight columns of a row.
+// The operands that are not read in place, as the kernel reads them: rows of ld (a multiple of 8) bf16,
+// kPlanes planes of them. blockIdx.y: which one; thread: eight columns of a row.
+struct Copies {
+  struct {
+    const void* src;
+    __nv_bfloat16* dst;
+    int64_t rows;
+    int cols, ld;
+  } of[3];
+};
 template <class T, int kPlanes>
-__global__ void __launch_bounds__(256) planes_kernel(const T* src, int64_t rows, int cols, int ld, __nv_bfloat16* dst) {
-  const int per = ld / 8;
+__global__ void __launch_bounds__(256) planes_kernel(const __grid_constant__ Copies copies) {
+  const auto& o = copies.of[blockIdx.y];
+  const int per = o.ld / 8;
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= rows * per) return;
+  if (e >= o.rows * per) return;
   const int64_t r = e / per;
   const int c = (int)(e % per) * 8;
-  const T* s = src + r * cols + c;
+  const T* s = static_cast<const T*>(o.src) + r * o.cols + c;
   float v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     v[i] = 0.f;
-    if (c + i < cols) {
+    if (c + i < o.cols) {
       if constexpr (sizeof(T) == 2) v[i] = __bfloat162float(s[i]); else v[i] = s[i];
     }
   }
@@ -571,7 +581,7 @@ __global__ void __launch_bounds__(256) planes_kernel(const T* src, int64_t rows,
       v[2 * i] -= __low2float(h);
       v[2 * i + 1] -= __high2float(h);
     }
-    *reinterpret_cast<uint4*>(dst + (k * rows + r) * ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(o.dst + (k * o.rows + r) * o.ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -661,24 +671,27 @@ struct Run {
   const __nv_bfloat16 *x, *wg, *wu;
   int ldx, ldw;
 
-  int operand(const void* src, int64_t rows, int cols, int ld, int64_t at, const __nv_bfloat16** to) {
-    if (at < 0) {
-      *to = static_cast<const __nv_bfloat16*>(src);
-      return BT_OK;
-    }
-    __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(ws + at);
-    planes_kernel<T, kP><<<(unsigned)ceil_div64(rows * (ld / 8), 256), 256, 0, s>>>(static_cast<const T*>(src), rows,
-                                                                                    cols, ld, dst);
-    BT_LAUNCH_CHECK("gated layer operand planes");
-    *to = dst;
-    return BT_OK;
-  }
   int operands() {
     ldx = w.x < 0 ? l.K : w.ldk;
     ldw = w.wg < 0 ? l.N : w.ldn;
-    BT_TRY(operand(l.x, l.M, l.K, w.ldk, w.x, &x));
-    BT_TRY(operand(l.wg, l.K, l.N, w.ldn, w.wg, &wg));
-    return operand(l.wu, l.K, l.N, w.ldn, w.wu, &wu);
+    Copies c{};
+    int n = 0;
+    int64_t most = 0;
+    auto operand = [&](const void* src, int64_t rows, int cols, int ld, int64_t at) -> const __nv_bfloat16* {
+      if (at < 0) return static_cast<const __nv_bfloat16*>(src);
+      __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(ws + at);
+      c.of[n++] = {src, dst, rows, cols, ld};
+      most = max(most, rows * (ld / 8));
+      return dst;
+    };
+    x = operand(l.x, l.M, l.K, w.ldk, w.x);
+    wg = operand(l.wg, l.K, l.N, w.ldn, w.wg);
+    wu = operand(l.wu, l.K, l.N, w.ldn, w.wu);
+    if (n > 0) {
+      planes_kernel<T, kP><<<dim3((unsigned)ceil_div64(most, 256), n), 256, 0, s>>>(c);
+      BT_LAUNCH_CHECK("gated layer operand planes");
+    }
+    return BT_OK;
   }
   // Maps of an operand's planes, `box` rows of 64 columns at a time.
   int maps(CUtensorMap* m, const __nv_bfloat16* base, int64_t rows, int cols, int ld, int box) {
@@ -694,7 +707,8 @@ struct Run {
   template <Mode kMode, int kN>
   int launch_n(Params& p) {
     auto kernel = glu_kernel<T, kMode, kN>;
-    BT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<kN>::kSmem));
+    static std::atomic<uint64_t> allowed{0};
+    BT_TRY(allow_smem(kernel, Ring<kN>::kSmem, allowed));
     BT_TRY(operator_error_word(&p.err));
     const int tiles = ceil_div(p.M, 2 * BM) * ceil_div(p.N, kMode == kInput ? kN : kN / 2) * p.splits;
     BT_CUDA(launch_pdl(kernel, dim3(2 * min(tiles, kPairs)), dim3(kThreads), Ring<kN>::kSmem, s, p));

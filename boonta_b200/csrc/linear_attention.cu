@@ -15,6 +15,7 @@
 // the splits (S_{s+1} = e^{len g} S_s + local_s), a third runs the splits from those.
 #include <type_traits>
 
+#include "launch.cuh"
 #include "linear_attention.cuh"
 
 namespace bt {
@@ -331,15 +332,16 @@ template <class T, int DA, int DS>
 int run_chunks(const Ops& ops, bool vec, cudaStream_t stream) {
   const Op& o = ops.op[0];
   constexpr int kSmem = sizeof(Smem<DA, DS>);
+  static std::atomic<uint64_t> allowed[2];
   int blocks = 0;
   for (int i = 0; i < ops.n; ++i) blocks = max(blocks, o.batch * o.heads * ceil_div(ops.op[i].Dc, DS));
   if (o.nsplit > 1) {
-    BT_CUDA(cudaFuncSetAttribute(chunk_kernel<T, DA, DS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    BT_TRY(allow_smem(chunk_kernel<T, DA, DS, false>, kSmem, allowed[1]));
     chunk_kernel<T, DA, DS, false><<<dim3(blocks, o.nsplit - 1, ops.n), kThreads, kSmem, stream>>>(ops, vec);
     BT_LAUNCH_CHECK("linear attention split sums");
     BT_TRY(launch_join(ops, stream));
   }
-  BT_CUDA(cudaFuncSetAttribute(chunk_kernel<T, DA, DS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  BT_TRY(allow_smem(chunk_kernel<T, DA, DS, true>, kSmem, allowed[0]));
   chunk_kernel<T, DA, DS, true><<<dim3(blocks, o.nsplit, ops.n), kThreads, kSmem, stream>>>(ops, vec);
   BT_LAUNCH_CHECK("linear attention");
   return BT_OK;

@@ -32,6 +32,7 @@
 
 #include "f32x2.cuh"
 #include "gemm_sm100.cuh"
+#include "launch.cuh"
 #include "linear_attention.cuh"
 
 namespace bt {
@@ -789,7 +790,8 @@ int run_tensor_cores(Ops& ops, cudaStream_t stream) {
     auto sums = chunk_tc_kernel<DA, false>;
     auto outs = chunk_tc_kernel<DA, true>;
     constexpr int kSmem = Cfg<DA>::kBytes;
-    BT_CUDA(cudaFuncSetAttribute(outs, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    static std::atomic<uint64_t> allowed[2];
+    BT_TRY(allow_smem(outs, kSmem, allowed[0]));
     // Two blocks an SM in all, each with every so many-th sequence: the same head again and again where the
     // heads allow it (its powers are kept).
     auto wide = [&](int splits) {
@@ -797,7 +799,7 @@ int run_tensor_cores(Ops& ops, cudaStream_t stream) {
       return min(blocks, room > per ? room / per * per : room);
     };
     if (o.nsplit > 1) {
-      BT_CUDA(cudaFuncSetAttribute(sums, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+      BT_TRY(allow_smem(sums, kSmem, allowed[1]));
       sums<<<dim3(wide(o.nsplit - 1), o.nsplit - 1, ops.n), kThreads, kSmem, stream>>>(ops, maps, err);
       BT_LAUNCH_CHECK("linear attention split sums");
       BT_TRY(launch_join(ops, stream));
