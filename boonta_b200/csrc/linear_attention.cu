@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(const __grid_constant__
   const int split = blockIdx.y;
   const int begin = split * o.split_len, end = min(o.steps, begin + o.split_len);
   const int tid = threadIdx.x;
-  const float g = fmaxf(o.log_decay[head], kMinLogDecay);
+  const float g = clamped_decay(o.log_decay[head]);
   const int DcV = min(DS, o.Dc - d0);
   const size_t elems = (size_t)o.Da * o.Dc;
 
@@ -238,7 +238,7 @@ __global__ void join_kernel(const __grid_constant__ Ops ops) {
   if (e >= total) return;
   const int64_t bh = e / elems;
   const int batch = (int)(bh / o.heads), x = (int)(e % elems / o.Dc), y = (int)(e % o.Dc);
-  const float g = fmaxf(o.log_decay[bh % o.heads], kMinLogDecay);
+  const float g = clamped_decay(o.log_decay[bh % o.heads]);
   float s = o.init ? o.init[bh * elems + (int64_t)x * o.sx + (int64_t)y * o.sy] : 0.f;
   const double full = exp((double)o.split_len * (double)g);
   const double first = o.reverse ? exp((double)(o.split_len - 1) * (double)g) : full;
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kThreads)
     sk[i] = to_float(kp[i]);
   }
   const bool cut = reset && reset[batch * reset_batch];
-  const float decay = expf(fmaxf(log_decay[head], kMinLogDecay));
+  const float decay = expf(clamped_decay(log_decay[head]));
   const int r = threadIdx.x / cols, y = threadIdx.x % cols * V;
   const bool on = r < R;
   float val[V], acc[V];
@@ -295,14 +295,14 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   const int64_t base = (int64_t)bh * Dk * Dv;
   if (on) {
-#pragma unroll 4
+#pragma unroll 8
     for (int x = r; x < Dk; x += R) {
       float s[V];
       if (cut) {
 #pragma unroll
         for (int w = 0; w < V; ++w) s[w] = 0.f;
       } else if constexpr (V == 4) {
-        const float4 f = *reinterpret_cast<const float4*>(state + base + (int64_t)x * Dv + y);
+        const float4 f = __ldcs(reinterpret_cast<const float4*>(state + base + (int64_t)x * Dv + y));
         s[0] = f.x, s[1] = f.y, s[2] = f.z, s[3] = f.w;
       } else {
         s[0] = state[base + (int64_t)x * Dv + y];
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(kThreads)
         acc[w] += sq[x] * s[w];
       }
       if constexpr (V == 4)
-        *reinterpret_cast<float4*>(next + base + (int64_t)x * Dv + y) = make_float4(s[0], s[1], s[2], s[3]);
+        __stcs(reinterpret_cast<float4*>(next + base + (int64_t)x * Dv + y), make_float4(s[0], s[1], s[2], s[3]));
       else
         next[base + (int64_t)x * Dv + y] = s[0];
     }

@@ -60,6 +60,8 @@ int launch_join(const Ops& ops, cudaStream_t stream);
 // would give 0 * inf).
 constexpr float kMinLogDecay = -1e4f;
 
+__device__ __forceinline__ float clamped_decay(float g) { return g < kMinLogDecay ? kMinLogDecay : g; }
+
 __device__ __forceinline__ int op_time(const Op& o, int i) { return o.reverse ? o.steps - 1 - i : i; }
 
 // Whether the state is cleared before position i.

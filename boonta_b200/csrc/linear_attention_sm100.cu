@@ -96,7 +96,6 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void*
                "r"(x), "r"(t), "r"(h), "r"(b), "r"(smem_u32(src))
                : "memory");
 }
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // D (tensor memory) += A (tensor memory, two K elements a column) B (shared memory).
 __device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
@@ -295,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (!mbar_wait_bounded(bar, parity)) *s_fail = 1;
     fence_after_sync();
   };
-  auto decay_of = [&](int head) { return fmaxf(o.log_decay[head], kMinLogDecay); };
+  auto decay_of = [&](int head) { return clamped_decay(o.log_decay[head]); };
 
   if (warp == 8) {
     // Descriptors of the tiles; a step along the contraction adds to the address field (16-byte units).
@@ -444,22 +443,6 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int i = 0; i < kSC; i += 16) turn_quads(s + i, lane);
     };
-    // a coming sequence's state on its way to L2
-    auto prefetch_state = [&](const Seq& q) {
-      int sx = 0, sy = 0;
-      const int k = row_of_state(), y0 = column_of_state();
-      const float* from = state_in(q, k, y0, sx, sy);
-      const int left = from && k < o.Da ? o.Dc - q.d0() - y0 : 0;
-      if (sy == 1) {
-#pragma unroll
-        for (int i = 0; i < kSC; i += 8)
-          if (i < left) prefetch_l2(from + i);
-      } else if ((k & 7) == 0) {
-#pragma unroll
-        for (int i = 0; i < kSC; ++i)
-          if (i < left) prefetch_l2(from + i * sy);
-      }
-    };
     // what the walk leaves of s: the final state, or the split's own sum
     auto store_state = [&](const Seq& q) {
       float* const all = !kOut ? o.local + (size_t)split * o.batch * o.heads * (o.Da * o.Dc)
@@ -526,7 +509,6 @@ __global__ void __launch_bounds__(kThreads, 2)
       Seq next = q;
       next.advance();
       more = next.batch < o.batch;
-      if (kOut && more) prefetch_state(next);
       settle_state();
       bool any_cut = false;
       int e0 = (reverse && split == 0) ? 0 : 1;
@@ -634,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (!weak || last >= 0) {
             // the rows of a S by the decay since the state; a cut drops it whatever it holds
             const float reach = lo >= 0 || p >= n ? 0.f : weak ? 1.f : pw[p + e0];
-#pragma unroll
+#pragma unroll 1
             for (int j = 0; j < 2; ++j) {
               float v[16];
               uint32_t x[16];
@@ -647,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           // P: this warp's 32 rows against the columns 64 half .. 64 half + 63, 16 at a time. It takes the place
           // of the first half of them: what it replaces is read by then.
           const int first = max(lo, 0);  // columns of positions first .. p count
-#pragma unroll
+#pragma unroll 1
           for (int u = 0; u < 4; ++u) {
             const int c0 = 64 * half + 16 * u;
             const unsigned m = (reverse ? bits(kC - 1 - c0 - p, kC - 1 - c0 - first) : bits(first - c0, p - c0)) & 0xffffu;
@@ -696,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           wait(done_o, parity);
           const float f = weak && p < n ? o.out_scale / pw[n - 1 - p] : o.out_scale;
           const int t0 = time_of(i0), x0 = q.d0() + 32 * half;
-#pragma unroll
+#pragma unroll 1
           for (int j = 0; j < 2; ++j) {
             float v[16];
             tmem_ld16(lanes + kOCol + 32 * half + 16 * j, v);

@@ -33,6 +33,18 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _tiles(t: torch.Tensor) -> torch.Tensor:
+    """_rows(t), and for bfloat16 a copy without gaps where the rows of `t` do not start on the
+    16-byte boundaries that the tensor-core kernels read from but the copy's would (a shared head
+    expanded over the others, a slice off the boundary)."""
+    t = _rows(t)
+    if t.dtype != torch.bfloat16 or t.shape[-1] % 8:
+        return t
+    fits = t.data_ptr() % 16 == 0 and all(
+        n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()))
+    return t if fits else t.clone(memory_format=torch.contiguous_format)
+
+
 def _device(name, first, *others) -> int:
     """The CUDA device of all the tensors (those that are not None)."""
     index = first.get_device()
@@ -95,7 +107,7 @@ def _workspace(shape, backward, device):
 
 def _forward(q, k, v, log_decay, state, reset, scale):
     """(out, final state) and the tensors that the call read."""
-    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
+    q, k, v, log_decay = _tiles(q), _tiles(k), _tiles(v), log_decay.contiguous()
     state = None if state is None else state.contiguous()
     out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
     final = torch.empty((q.shape[0], q.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32,
@@ -124,7 +136,7 @@ class _LinearAttention(torch.autograd.Function):
         q, k, v, log_decay, state, reset = ctx.saved_tensors
         if dout is None and dfinal is None:
             return (None,) * 7
-        dout = torch.zeros_like(v) if dout is None else _rows(dout.to(v.dtype))
+        dout = torch.zeros_like(v) if dout is None else _tiles(dout.to(v.dtype))
         dfinal = None if dfinal is None else dfinal.contiguous()
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         dstate = torch.empty((q.shape[0], q.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32,
@@ -170,7 +182,8 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
           or new_state.get_device() != device or not new_state.is_contiguous()):
         raise ValueError(f"linear_attention_step: new_state {tuple(new_state.shape)} "
                          f"{new_state.dtype}: a contiguous {tuple(state.shape)} float32 tensor expected")
-    elif new_state.data_ptr() != state.data_ptr() and _overlap(new_state, state):
+    elif _overlap(new_state, state) and not (new_state.data_ptr() == state.data_ptr()
+                                             and state.is_contiguous()):
         raise ValueError("linear_attention_step: new_state overlaps state in part")
     state = state.contiguous()
     out = torch.empty(v.shape, dtype=v.dtype, device=v.device)

@@ -186,9 +186,12 @@ BT_API int bt_linear_scan_backward(const void* a, const void* h, const void* ini
  * before it, the given state included, has no part in that step or a later one. Heads of 1 to 128
  * features; log_decay [heads] float32, <= 0 (-inf forgets everything at once), taken as a
  * constant. Sums and states are float32 or better. The backward takes the gradients of out and
- * final_state (null: zeros) and writes those of q, k, v and state. The step form takes steps = 1
+ * final_state (null: zeros) and writes those of q, k, v and state; no output may be an input. The step form takes steps = 1
  * and the rows' batch and head strides; out [batch, heads, value_dim] is contiguous and new_state
- * may be state. Workspaces are device memory, 16-byte aligned, of the size that
+ * may be state. bf16 calls whose rows all start on 16-byte boundaries (strides above 0) run on the
+ * tensor cores: products of bf16 values, sums and states float32, out rounded once more on the way
+ * (weighted scores or the state). A value that is not finite may reach other steps of its own (batch
+ * row, head), never another's. Workspaces are device memory, 16-byte aligned, of the size that
  * bt_linear_attention_workspace gives (-1: bad shape), free again when the call's work is done. */
 typedef struct bt_heads {
   void* data;
@@ -248,7 +251,8 @@ BT_API int bt_qk_norm_rotary_backward(const bt_qk_norm_rotary_shape* shape, cons
  * [rows, out_features], all row-major in `dtype`; activation BT_ACT_*. Sums are float32. The
  * backward takes the gradient of out, forms both projections again and writes dx and (both or
  * neither) dw_gate and dw_up; a null one is not formed. Pointers are 16-byte aligned. Workspaces as
- * above (bt_glu_workspace). */
+ * above (bt_glu_workspace). float32 values enter as three bf16 parts each (24 bits): one that is not
+ * finite makes the sums it enters NaN. */
 typedef struct bt_glu_shape {
   int32_t rows, in_features, out_features, dtype, activation;
 } bt_glu_shape;

@@ -231,6 +231,17 @@ def test_steps(B, H, dk, dv, dtype):
     assert same is s and torch.equal(s, new) and torch.equal(again, out)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_nan_decay_is_not_hidden(dtype):
+    import torch
+
+    a = list(inputs(33, 1, 140, 2, 64, 64, dtype, resets="none"))
+    a[3] = torch.tensor([math.nan, -0.1], device="cuda")
+    out, final = run(a, grads=False)
+    assert out[:, :, 0].isnan().all() and final[:, 0].isnan().all()
+    assert out[:, :, 1].isfinite().all() and final[:, 1].isfinite().all()
+
+
 def test_steps_follow_the_unroll():
     """Acting step by step gives what the unroll gives, and the state between."""
     import torch
@@ -265,6 +276,8 @@ def test_refusals_on_the_gpu():
     room = torch.zeros(3, 2, 8, 8, device="cuda")
     with pytest.raises(ValueError, match="overlaps"):
         linear_attention_step(*step, ld, room[:2], new_state=room[1:])
+    with pytest.raises(ValueError, match="overlaps"):
+        linear_attention_step(*step, ld, room[0].transpose(2, 1).expand(2, 2, 8, 8), new_state=room[:2])
     with pytest.raises(ValueError, match="a state"):
         linear_attention_step(*step, ld, None)
 

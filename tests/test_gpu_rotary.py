@@ -117,6 +117,13 @@ def test_far_positions_keep_their_phase(interleaved):
     compare(inputs(5, 2, 50, 2, 2, 64, "f32", far=1_000_000), "f32", None, 32, interleaved)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_positions_before_zero(dtype):
+    a = list(inputs(6, 2, 40, 2, 1, 64, dtype))
+    a[4] = a[4] - 500
+    compare(a, dtype, None, 32, False)
+
+
 def test_missing_weights_count_as_ones_and_positions_may_be_shared():
     import torch
 
