@@ -9,7 +9,7 @@
 // block's whole walk. It serves float32, and bf16 whose rows do not start on 16-byte boundaries. A row
 // takes only the columns from its last cut to itself, so what a cut or the future hides is not read, whatever
 // it holds. Bound by the latency of the walk where sequences are few: blocks of 16 columns then, four times
-// as many, each a third as long (48 x 100 x 3 x 48 float32: 83 us with 64 columns, 41 with 16).
+// as many, each a third as long (48 x 100 x 3 x 48 float32, forward: 83 us with 64 columns, 47 with 16).
 // Sequences too few to fill the GPU are split along the steps: a first
 // launch sums each split from an empty state, a second joins the sums into the states that enter
 // the splits (S_{s+1} = e^{len g} S_s + local_s), a third runs the splits from those.
@@ -361,17 +361,18 @@ int run_ops(const Ops& ops, cudaStream_t stream) {
     };
     vec = vec && o.Da % 4 == 0 && o.Dc % 4 == 0 && rows(o.a) && rows(o.b) && rows(o.c);
   }
-  // narrow blocks while wide ones would leave SMs with less than two
+  // narrow blocks while wide ones would not fill the SMs twice (three operations of the case above:
+  // 103 us wide, 125 narrow)
   const Op& o = ops.op[0];
-  const bool narrow = (int64_t)o.batch * o.heads * ceil_div(dc, kWide) * o.nsplit * ops.n < 4 * kNumSMs;
+  const bool narrow = (int64_t)o.batch * o.heads * ceil_div(dc, kWide) * o.nsplit * ops.n < 2 * kNumSMs;
   if (da <= 64)
     return narrow ? run_chunks<T, 64, kNarrow>(ops, vec, stream) : run_chunks<T, 64, kWide>(ops, vec, stream);
   return narrow ? run_chunks<T, 128, kNarrow>(ops, vec, stream) : run_chunks<T, 128, kWide>(ops, vec, stream);
 }
 
 // Splits of the steps: the number whose launches are the shortest, in units of the walk over 128 steps. Two
-// blocks share an SM (one alone is faster by about a third); a sequence costs a third of a unit to begin,
-// the sums of the splits half of a full walk, and the two more launches about two units.
+// blocks share an SM (one alone is faster by about a third); a sequence costs a unit to begin and end, the
+// sums of the splits half of a full walk, and the two more launches about two units.
 void choose_splits(const bt_linear_attention_shape* s, int ops, int* nsplit, int* len) {
   const int64_t blocks = (int64_t)s->batch * s->heads * ceil_div(max(s->key_dim, s->value_dim), kWide) * ops;
   const int chunks = max(1, ceil_div(s->steps, 128));
@@ -381,7 +382,7 @@ void choose_splits(const bt_linear_attention_shape* s, int ops, int* nsplit, int
     const int each = ceil_div(chunks, n), have = ceil_div(chunks, each);
     auto walk = [&](int64_t items, double unit) {
       const double shared = items <= kNumSMs ? 0.65 : 1.0;
-      return (double)ceil_div64(items, 2 * kNumSMs) * (each * unit + 0.33) * shared;
+      return (double)ceil_div64(items, 2 * kNumSMs) * (each * unit + 1.0) * shared;
     };
     const double t = walk(blocks * have, 1.0) + (have > 1 ? walk(blocks * (have - 1), 0.5) + 2.0 : 0.0);
     if (t < least) least = t, best = each;

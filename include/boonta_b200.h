@@ -29,6 +29,10 @@
  *   bt_linear_scan /
  *   bt_linear_scan_backward boonta/networks/kernels/scan.py:13-89 (the SSM torso's linear
  *                           recurrence and its custom VJP; the Pallas Mosaic-GPU kernel)
+ *   bt_linear_attention*, bt_qk_norm_rotary*, bt_glu*
+ *                           operators of a linear-attention torso, beside the scan (the
+ *                           reference's torso blocks are flax modules; these have no
+ *                           counterpart of the same form)
  *   bt_random_*             jax.random's threefry key operations behind ppo.py:200, 230
  *                           (permutation, split) and distributions.py:21-23 (uniform draws)
  *   bt_learner_comm_init    the NCCL communicator behind jax.distributed / XLA's
