@@ -27,7 +27,13 @@
 // to a row. A chunk is a chain of dependent steps, so the chain is cut where it can be (w c is formed
 // while a b^T runs, L runs while P is formed, the outputs are written while the next tiles come), and two
 // blocks share an SM: 256 of the 512 columns of tensor memory each, and at most 113 KB of shared memory
-// (planes of w c in place of a, which P0 and O are done with).
+// (planes of w c in place of a, which P0 and O are done with). Nothing that can be formed again is kept in
+// registers across a chunk: what spills goes through an L1 that shared memory leaves next to nothing of.
+//
+// Measured: 16 x 2000 x 8 heads x 64/128 forward 82 us (2.5 TB/s of its 205 MB, tensor pipe 38 %); 512 x 128
+// x 4 x 64 forward 62 us, its three gradients 158 us; 2 x 8191 x 16 x 128 forward 105 us after 57 us for the
+// splits' sums, gradients 355 us. Bound by the chain: 0.4 instructions a cycle and scheduler, a quarter of a
+// warp's time in waits for tensor memory, barriers and tiles.
 #include <type_traits>
 
 #include "f32x2.cuh"
