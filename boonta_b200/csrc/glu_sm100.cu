@@ -243,7 +243,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) glu_ker
   uint64_t* epi_in = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(epi_in + kEpiWarps);
   __shared__ int s_fail;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   pdl_trigger();
   if (threadIdx.x == 0) {
     s_fail = 0;
@@ -321,10 +321,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) glu_ker
         if (!mbar_wait_bounded(&empty[i % kStages], (i / kStages) & 1)) atomicExch(&s_fail, kErrTimeoutEmpty);
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      // M = 256 over the pair
+    if (rank == 0) {
+      // M = 256 over the pair. The whole warp walks along and one lane issues, so that descriptors stay in
+      // uniform registers; a stage's and a step's are the first ones plus a constant (16-byte units).
       constexpr uint32_t idesc = instr_desc<kN, A_MN, B_MN>() + ((uint32_t)(BM >> 4) << 24);
-      int g = 0, c = 0;
+      const uint64_t desc_a = operand_desc<A_MN>(smem_u32(smem), 0), desc_b = operand_desc<B_MN>(smem_u32(smem) + kAB, 0);
+      constexpr uint64_t kStepA = (A_MN ? 2048 : 32) >> 4, kStepB = (B_MN ? 2048 : 32) >> 4;
+      const bool leader = elect_one();
+      int s = 0, c = 0;  // the ring's stage and (its parity) round, the accumulator
+      uint32_t round = 0;
       bool ok = true;
       for (int t = blockIdx.x >> 1; t < tiles && ok && !failed(); t += gridDim.x >> 1) {
         int m0, n0, k0, k1, split;
@@ -333,49 +338,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) glu_ker
           bool keep = (kb - k0) % kHand != 0;
           if (!keep && c >= 2) {
             if (!mbar_wait_bounded(&acc_empty[c & 1], ((c >> 1) - 1) & 1)) {
-              atomicExch(&s_fail, kErrTimeoutAcc);
+              if (lane == 0) atomicExch(&s_fail, kErrTimeoutAcc);
               ok = false;
               break;
             }
             fence_after_sync();
           }
           const uint32_t acc = tmem + (uint32_t)((c & 1) * kN);
-          for (int q = 0; q < kSums && ok; ++q, g += kP) {
-            uint32_t at[kP];  // the planes' stages, by plane
-            uint64_t* done[kP];
+          for (int q = 0; q < kSums && ok; ++q) {
+            int at[kP];  // the planes' stages, by plane
 #pragma unroll
             for (int e = 0; e < kP; ++e) {
-              const int s = (g + e) % kStages;
-              if (!mbar_wait_bounded(&full[s], ((g + e) / kStages) & 1)) {
-                atomicExch(&s_fail, kErrTimeoutFull);
+              if (!mbar_wait_bounded(&full[s], round)) {
+                if (lane == 0) atomicExch(&s_fail, kErrTimeoutFull);
                 ok = false;
               }
-              at[kP - 1 - e] = smem_u32(smem + s * kStageBytes);
-              done[kP - 1 - e] = &empty[s];
+              at[kP - 1 - e] = s;
+              if (++s == kStages) s = 0, round ^= 1;
             }
             if (!ok) break;
             fence_after_sync();
-            auto product = [&](int x, int y) {
+            if (leader) {
+              auto product = [&](int x, int y) {
+                const uint64_t a = desc_a + (uint64_t)(at[x] * (kStageBytes >> 4));
+                const uint64_t b = desc_b + (uint64_t)(at[y] * (kStageBytes >> 4));
 #pragma unroll
-              for (int k = 0; k < BK / 16; ++k) {
-                pair_mma(acc, operand_desc<A_MN>(at[x], k), operand_desc<B_MN>(at[y] + kAB, k), idesc, keep ? 1u : 0u);
-                keep = true;
+                for (int k = 0; k < BK / 16; ++k) {
+                  pair_mma(acc, a + k * kStepA, b + k * kStepB, idesc, keep ? 1u : 0u);
+                  keep = true;
+                }
+              };
+              if constexpr (kP == 3) {
+                product(2, 0);
+                product(0, 2);
+                pair_commit(&empty[at[2]]);
+                product(1, 1);
+                product(0, 1);
+                product(1, 0);
+                pair_commit(&empty[at[1]]);
               }
-            };
-            if constexpr (kP == 3) {
-              product(2, 0);
-              product(0, 2);
-              pair_commit(done[2]);
-              product(1, 1);
-              product(0, 1);
-              product(1, 0);
-              pair_commit(done[1]);
+              product(0, 0);
+              pair_commit(&empty[at[0]]);
             }
-            product(0, 0);
-            pair_commit(done[0]);
+            keep = true;
+            __syncwarp();
           }
           if (ok && ((kb - k0) % kHand == kHand - 1 || kb == k1 - 1)) {
-            pair_commit(&acc_full[c & 1]);
+            if (leader) pair_commit(&acc_full[c & 1]);
+            __syncwarp();
             ++c;
           }
         }

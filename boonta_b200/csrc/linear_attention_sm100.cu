@@ -142,13 +142,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// One lane of a converged warp, the same one every time.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
-  return p != 0;
-}
-
 // The bits lo .. hi of a word (positions outside 0 .. 31 allowed).
 __device__ __forceinline__ unsigned bits(int lo, int hi) {
   const unsigned from = lo <= 0 ? ~0u : lo > 31 ? 0u : ~0u << lo;
