@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (lane == 0) umma::bulk_wait_read_all();
           sync_pair(row >> 5);
         }
-        {  // w c: this thread's row, half of the columns; the planes that go into a's place wait for it
+        {  // w c: this thread's row, half of the columns
           const float wf = p < n ? o.in_scale * pw[n - 1 - p] : 0.f;
           const uint64_t wp = pair(wf, wf);
           // 24 bits cut into 8 + 8 + 8: each plane takes the leading bits, the rest is exact
@@ -581,24 +581,22 @@ __global__ void __launch_bounds__(kThreads, 2)
             for (int z = 0; z < 3; ++z) y[z] = make_uint4(t[z][0], t[z][1], t[z][2], t[z][3]);
           };
           auto place = [&](int u) { return row * 128 + (((half * 4 + u) ^ (row & 7)) << 4); };
+          // Planes 0 (and 1) take a's place and wait for O's product. One plane is held until then; two would not
+          // fit in the registers, and forming them twice cost more than waiting first (2 x 8191 x 16 x 128
+          // training pass: 503 us, 485 so).
           uint4 held[4], y[3];
+          if (F::kNA == 2 && kOut) wait(done_a, parity);
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             cut_up(place(u), y);
             if (F::kNA == 1) held[u] = y[0];
 #pragma unroll
-            for (int z = F::kNA; z < 3; ++z) *reinterpret_cast<uint4*>(smem + F::plane(z) + place(u)) = y[z];
+            for (int z = F::kNA == 1 ? 1 : 0; z < 3; ++z) *reinterpret_cast<uint4*>(smem + F::plane(z) + place(u)) = y[z];
           }
-          if (kOut) wait(done_a, parity);
+          if (F::kNA == 1) {
+            if (kOut) wait(done_a, parity);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if (F::kNA == 1) {
-              y[0] = held[u];
-            } else {
-              cut_up(place(u), y);  // once more: two planes held would not fit in the registers
-            }
-#pragma unroll
-            for (int z = 0; z < F::kNA; ++z) *reinterpret_cast<uint4*>(smem + F::plane(z) + place(u)) = y[z];
+            for (int u = 0; u < 4; ++u) *reinterpret_cast<uint4*>(smem + F::plane(0) + place(u)) = held[u];
           }
           if (last > p) {  // what a cut hides has no part in L; P0 is done with its row of b
 #pragma unroll

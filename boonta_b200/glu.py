@@ -87,9 +87,9 @@ def gated_linear_unit(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     sums in float32, the result [..., out] in x's dtype. A float32 value that is not finite makes the
     sums it enters NaN."""
     _check(x, w_gate, w_up, activation)
-    rows = x.reshape(-1, x.shape[-1])
+    rows = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
     if _wants_grad(x, w_gate, w_up):
         out = _Glu.apply(rows, w_gate, w_up, activation)
     else:
         out = _forward(rows, w_gate, w_up, activation)[0]
-    return out.reshape(*x.shape[:-1], w_gate.shape[1])
+    return out if x.ndim == 2 else out.reshape(*x.shape[:-1], w_gate.shape[1])
