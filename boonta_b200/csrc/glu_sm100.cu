@@ -10,7 +10,7 @@
 // A tile belongs to a cluster of two CTAs on neighbouring SMs (cta_group::2): each holds 128 of its 256 rows
 // and one half of the columns of B (of the projections: one of them each), the leader issues one MMA of M =
 // 256 over both, and each has its own rows of the accumulator. So a CTA loads 32 KB for 512 cycles of MMA;
-// alone it would load 48 KB, and 148 SMs doing that stood at what L2 gives, 12 TB/s (measured: 1.06
+// alone it would load 48 KB, and 148 SMs doing that draw 12 TB/s from L2 (measured: 178 us forward, 1.06
 // PFLOP/s). Pairs walk the tiles (of half the width where that fills more SMs). Warp 0 loads 64-deep blocks
 // by TMA into a ring of six stages, signalling the leader; the leader's warp 1 issues the MMAs into one of
 // two 256-column accumulators in tensor memory, and eight epilogue warps drain the other: activation and
@@ -22,8 +22,10 @@
 // fp32 registers after every 64-deep block (24 MMAs); a sixth of the bf16 rate remains, which is
 // four times what the CUDA cores' fp32 FMA does.
 //
-// Bound by the tensor cores: 16384 x 1024 -> 2816 bf16 takes 158 us forward (1.20 PFLOP/s, pipe 64 % active),
-// 172 us for dG and dU, 163 us for dx (256 tiles on 74 pairs, 3.5 waves in 4), 163 + 16 us for dW.
+// Bound by the tensor cores: 16384 x 1024 -> 2816 bf16 takes 126 us forward (1.50 PFLOP/s, pipe 88 % active),
+// 144 us for dG and dU (76 %), 130 us for dx (93 %; 256 tiles on 74 pairs, 3.5 waves in 4), 136 + 16 us for dW.
+// With the descriptors formed by the issuing lane instead of kept in uniform registers the issue of an MMA
+// cost about as much as its 128 cycles: 158, 172, 163 and 163 us.
 #include <type_traits>
 
 #include "gemm_sm100.cuh"

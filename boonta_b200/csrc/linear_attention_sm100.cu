@@ -31,9 +31,9 @@
 // registers across a chunk: what spills goes through an L1 that shared memory leaves next to nothing of.
 //
 // Measured: 16 x 2000 x 8 heads x 64/128 forward 82 us (2.5 TB/s of its 205 MB, tensor pipe 38 %); 512 x 128
-// x 4 x 64 forward 62 us, its three gradients 158 us; 2 x 8191 x 16 x 128 forward 105 us after 57 us for the
-// splits' sums, gradients 355 us. Bound by the chain: 0.4 instructions a cycle and scheduler, a quarter of a
-// warp's time in waits for tensor memory, barriers and tiles.
+// x 4 x 64 forward 63 us, its three gradients 159 us; 2 x 8191 x 16 x 128 forward 101 us after 63 us for the
+// splits' sums and their join, gradients 346 us. Bound by the chain: 0.4 instructions a cycle and scheduler, a
+// quarter of a warp's time in waits for tensor memory, barriers and tiles.
 #include <type_traits>
 
 #include "f32x2.cuh"
