@@ -24,6 +24,17 @@ static int resolve_encode() {
   return BT_OK;
 }
 
+// Encoding is a driver call, and a host thread whose first CUDA call it is (an autograd engine's, when its
+// memory came from a cache) has no current context yet: the runtime makes one current, and it is tried again.
+template <class... Args>
+static CUresult encode(Args... args) {
+  const CUresult r = g_encode(args...);
+  if (r != CUDA_ERROR_INVALID_CONTEXT && r != CUDA_ERROR_NOT_INITIALIZED) return r;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return r;
+  return g_encode(args...);
+}
+
 int encode_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
                uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer) {
   BT_TRY(resolve_encode());
@@ -36,7 +47,7 @@ int encode_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t oute
   cuuint64_t strides[1] = {row_bytes};
   cuuint32_t box[2] = {box_inner, box_outer};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
+  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
                         strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -57,7 +68,7 @@ int encode_map_4d(CUtensorMap* map, const void* base, const uint64_t dims[4], co
   for (int i = 0; i < 4; ++i) d[i] = dims[i], b[i] = box[i];
   // a dimension of one element is never stepped along, so any stride does
   for (int i = 0; i < 3; ++i) st[i] = dims[i + 1] > 1 ? strides[i] : 16;
-  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, st, b, estr,
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, st, b, estr,
                               CU_TENSOR_MAP_INTERLEAVE_NONE,
                               swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -83,7 +94,7 @@ int encode_tile_map(CUtensorMap* map, const void* base, bool f32, uint64_t inner
   cuuint64_t strides[1] = {row_bytes};
   cuuint32_t box[2] = {32, 32};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = g_encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+  CUresult r = encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                         2, const_cast<void*>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE,
                         swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,

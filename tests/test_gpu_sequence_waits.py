@@ -117,3 +117,37 @@ def test_rows_behind_the_outputs_are_left_as_they_were():
         assert torch.equal(out, want) and torch.equal(states[1:7], final.view(6, 64, 64))
         out.fill_(3.0)
         assert (wide == 3.0).all() and (states[0] == 5).all() and (states[7] == 5).all()
+
+
+def test_a_fresh_host_thread_may_call_first():
+    """A thread whose first CUDA call is an operator (its memory comes from torch's cache)."""
+    import threading
+
+    import torch
+
+    from boonta_b200.glu import gated_linear_unit
+    from boonta_b200.linear_attention import linear_attention
+
+    a = attention(4)
+    x, w = torch.randn(200, 64, device="cuda").bfloat16(), torch.randn(64, 64, device="cuda").bfloat16()
+    calls = (lambda: gated_linear_unit(x, w, w), lambda: linear_attention(*a)[0])
+    want = [f() for f in calls]
+    for f in calls:  # the cache now holds blocks of every size that the threads will ask for
+        del_me = [f() for _ in range(4)]
+    del del_me
+    got = [None, None]
+
+    def go(i):
+        try:
+            got[i] = calls[i]()
+        except Exception as e:  # noqa: BLE001
+            got[i] = e
+
+    for i in (0, 1):
+        t = threading.Thread(target=go, args=(i,))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    for g, b in zip(got, want):
+        assert torch.is_tensor(g), g
+        assert torch.equal(g, b)
