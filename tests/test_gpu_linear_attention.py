@@ -176,6 +176,18 @@ def test_extreme_decays(dtype):
     compare(run(a), want, scale, 200, 64, 64, dtype)
 
 
+@pytest.mark.parametrize("resets", ["none", "some"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_decays_on_both_sides_of_the_two_forms_of_the_scores(dtype, resets):
+    """Heads just above and just below the decay where the weights change their place; a negative scale."""
+    import torch
+
+    a = list(inputs(47, 2, 333, 5, 64, 128, dtype, resets=resets))
+    a[3] = torch.tensor([-0.2299, -0.2301, -0.1, -0.6, -5.0], device="cuda")
+    want, scale = oracle(*a, scale=-0.3)
+    compare(run(a, scale=-0.3), want, scale, 333, 64, 128, dtype)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_a_nan_stays_in_its_sequence(dtype):
     import torch
