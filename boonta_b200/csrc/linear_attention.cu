@@ -6,7 +6,7 @@
 //   out = out_scale (in_scale P c + e^{(i + e0) g} a S)      rows before the chunk's first cut
 //   S = e^{(n - 1 + e0) g} S + in_scale sum_j e^{(n - 1 - j) g} b_j c_j^T
 // A block owns one (batch row, head) and DS columns of c; the state stays in shared memory for the
-// block's whole walk. It serves float32, and bf16 whose rows do not start on 16-byte boundaries. A row
+// block's whole walk. It serves float32, and bf16 whose rows do not start (outputs: and end) on 16-byte boundaries. A row
 // takes only the columns from its last cut to itself, so what a cut or the future hides is not read, whatever
 // it holds. Bound by the latency of the walk where sequences are few: blocks of 16 columns then, four times
 // as many, each a third as long (48 x 100 x 3 x 48 float32, forward: 83 us with 64 columns, 47 with 16).

@@ -50,7 +50,8 @@ struct Ops {  // one launch's operations, of the same sequences
   int n;
 };
 
-// bf16 on the tensor cores (linear_attention_sm100.cu): where every row starts on a 16-byte boundary.
+// bf16 on the tensor cores (linear_attention_sm100.cu): where every row starts on a 16-byte boundary and the
+// output's rows end on one.
 bool suits_tensor_cores(const Op& o);
 int run_tensor_cores(Ops& ops, cudaStream_t stream);
 // Turns the splits' own sums into the states that enter the splits (linear_attention.cu).

@@ -693,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, 2)
               __nv_bfloat16* out = static_cast<__nv_bfloat16*>(o.out) + q.batch * o.out_batch +
                                    (int64_t)(t0 + row) * o.out_step + q.head() * o.out_head + x0 + 16 * j;
 #pragma unroll
-              for (int i = 0; i < 2; ++i)  // Dc is a multiple of 8, as the rows' strides are
+              for (int i = 0; i < 2; ++i)  // Dc is a multiple of 8 (suits_tensor_cores)
                 if (x0 + 16 * j + 8 * i < o.Dc) *reinterpret_cast<uint4*>(out + 8 * i) = y[i];
             }
           }
@@ -743,7 +743,8 @@ bool suits_tensor_cores(const Op& o) {
     auto ok = [](int64_t s, int n) { return n <= 1 || (s > 0 && s % 8 == 0 && s < ((int64_t)1 << 38)); };
     return ((uintptr_t)r.p & 15) == 0 && ok(r.step, o.steps) && ok(r.head, o.heads) && ok(r.batch, o.batch);
   };
-  return rows(o.a) && rows(o.b) && rows(o.c) && ((uintptr_t)o.out & 15) == 0 && o.out_step % 8 == 0 &&
+  // A TMA store writes whole 16-byte pieces: behind a row that ends inside one it would overwrite what lies there.
+  return o.Dc % 8 == 0 && rows(o.a) && rows(o.b) && rows(o.c) && ((uintptr_t)o.out & 15) == 0 && o.out_step % 8 == 0 &&
          o.out_head % 8 == 0 && o.out_batch % 8 == 0;
 }
 
