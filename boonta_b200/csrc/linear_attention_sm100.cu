@@ -158,6 +158,33 @@ __device__ __forceinline__ constexpr uint32_t idesc() {
 __device__ __forceinline__ void sync_workers() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ void sync_pair(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(2 + quarter) : "memory"); }
 
+// sync_workers, and whether any of them says yes.
+__device__ __forceinline__ bool any_worker(bool yes) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, 1, 256, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"((uint32_t)yes)
+      : "memory");
+  return any != 0;
+}
+
+// Whether any of eight bf16 is not finite: one more in its last place carries such an exponent into the sign.
+__device__ __forceinline__ bool any_odd(const uint4& v) {
+  auto carry = [](uint32_t w) { return (w & 0x7f807f80u) + 0x00800080u; };
+  return ((carry(v.x) | carry(v.y) | carry(v.z) | carry(v.w)) & 0x80008000u) != 0;
+}
+// Which of two (bit 0: the lower one), and of eight.
+__device__ __forceinline__ uint32_t odd_of(uint32_t w) {
+  return ((w & 0x7f80u) == 0x7f80u ? 1u : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 2u : 0u);
+}
+__device__ __forceinline__ uint32_t odd_of(const uint4& v) {
+  return odd_of(v.x) | odd_of(v.y) << 2 | odd_of(v.z) << 4 | odd_of(v.w) << 6;
+}
+
 // A value whose descendants the compiler does not take out of a loop.
 __device__ __forceinline__ int opaque(int x) {
   asm volatile("" : "+r"(x));
@@ -208,8 +235,8 @@ struct Seq {
   __device__ __forceinline__ int d0() const { return slices == 2 ? (at & 1) * kDS : 0; }
 };
 
-// kOut: outputs, from the state that enters the split; else the split's own sum.
-template <int DA, bool kOut>
+// kOut: outputs, from the state that enters the split; else the split's own sum. kCuts: there are resets.
+template <int DA, bool kOut, bool kCuts>
 __global__ void __launch_bounds__(kThreads, 2)
     chunk_tc_kernel(const __grid_constant__ Ops ops, const __grid_constant__ Maps maps, int* err) {
   using F = Cfg<DA>;
@@ -475,13 +502,12 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (k < o.Da && i < left) to[i * ty] = s[i];
       }
     };
-    const bool resets = o.reset != nullptr;
     uint32_t parity = 0;
     int head = -1;
     bool weak = true;
     Seq q(o, blockIdx.x, gridDim.x);
     auto cut_at = [&](int batch, int i0) { return tid < kC && i0 + tid < end && op_cut(o, batch, i0 + tid); };
-    bool cut = resets && cut_at(q.batch, begin);
+    bool cut = kCuts && cut_at(q.batch, begin);
     load_state(q);
     auto arrive = [&](uint64_t* bar) {
       fence_before_sync();
@@ -537,14 +563,23 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int y0 = DA == 128 ? half * 32 : (row >> 6) * 32 + half * 16;
         // the last cut of the chunk, and the last one at or before p (-1: none)
         int last = -1, lo = -1;
-        if (resets) {
-          unsigned* cuts = s_cut + 4 * parity;
-          if (tid < kC) {
-            const unsigned m = __ballot_sync(~0u, cut);
-            if (lane == 0) cuts[warp] = m;
-            cut = (!ends || more) && cut_at(ends ? next.batch : q.batch, ends ? begin : i0 + kC);
+        bool odd = false;
+        unsigned* cuts = s_cut + 4 * parity;
+        if (kCuts && tid < kC) {
+          const unsigned m = __ballot_sync(~0u, cut);
+          if (lane == 0) cuts[warp] = m;
+          cut = (!ends || more) && cut_at(ends ? next.batch : q.batch, ends ? begin : i0 + kC);
+        }
+        wait(full, parity);
+        if (kCuts) {
+          if constexpr (kOut) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              odd |= any_odd(*reinterpret_cast<const uint4*>(smem + F::kCc + row * 128 + (((half * 4 + u) ^ (row & 7)) << 4)));
+            odd = any_worker(odd);
+          } else {
+            sync_workers();
           }
-          sync_workers();
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const unsigned m = cuts[x], own = m & bits(0, p - 32 * x);
@@ -553,8 +588,34 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
           any_cut |= last >= 0;
         }
-
-        wait(full, parity);
+        // Values of c that are not finite, in a chunk with a cut: the products would carry them across it as 0 times
+        // themselves. They are taken out of the tile, and what they reach (their column of the later outputs of
+        // their own stretch, and of the state where no cut follows) is set to NaN at the end. A bit a column.
+        uint32_t odd_out = 0, odd_state = 0;
+        if (kOut && kCuts && odd && last >= 0) {
+          auto columns = [&](int from, int to, int c0, int count) {
+            uint32_t m = 0;
+            for (int at = from; at <= to; ++at) {
+              const int r = reverse ? kC - 1 - at : at;
+              for (int u = 0; u < count; u += 8)
+                m |= odd_of(*reinterpret_cast<const uint4*>(smem + F::kCc + r * 128 + ((((c0 + u) >> 3) ^ (r & 7)) << 4))) << u;
+            }
+            return m;
+          };
+          odd_out = columns(max(lo, 0), min(p, n - 1), 32 * half, 32);
+          odd_state = columns(last, n - 1, y0, kSC);
+          sync_workers();
+          for (int u = 0; u < 4; ++u) {
+            uint4* const at = reinterpret_cast<uint4*>(smem + F::kCc + row * 128 + (((half * 4 + u) ^ (row & 7)) << 4));
+            uint32_t w[4] = {at->x, at->y, at->z, at->w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t m = odd_of(w[i]);
+              w[i] &= ~((m & 1 ? 0xffffu : 0u) | (m & 2 ? 0xffff0000u : 0u));
+            }
+            *at = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
         if (kOut) {
           // the pair's last outputs have left their staging rows
           if (lane == 0) umma::bulk_wait_read_all();
@@ -565,7 +626,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           const uint64_t wp = pair(wf, wf);
           // 24 bits cut into 8 + 8 + 8: each plane takes the leading bits, the rest is exact
           auto cut_up = [&](int off, uint4 (&y)[3]) {
-            const uint4 x = *reinterpret_cast<const uint4*>(smem + F::kCc + off);
+            uint4 x = *reinterpret_cast<const uint4*>(smem + F::kCc + off);
+            if (!kOut && last > p) x = make_uint4(0, 0, 0, 0);  // hidden by a cut, whatever it holds
             const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
             uint32_t t[3][4];
 #pragma unroll
@@ -662,6 +724,9 @@ __global__ void __launch_bounds__(kThreads, 2)
           else tmem_ld16(lanes + kLCol + y0, l);
 #pragma unroll
           for (int i = 0; i < kSC; ++i) s[i] = (last < 0 ? s[i] : 0.f) + l[i];
+          if (kOut && kCuts && odd_state)
+#pragma unroll
+            for (int i = 0; i < kSC; ++i) s[i] = odd_state >> i & 1 ? __int_as_float(0x7fffffff) : s[i];
         }
         e0 = 1;
         if (!ends) {
@@ -680,6 +745,9 @@ __global__ void __launch_bounds__(kThreads, 2)
             float v[16];
             tmem_ld16(lanes + kOCol + 32 * half + 16 * j, v);
             if (j == 1 && !ends) arrive(has_s);
+            if (kCuts && odd_out)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] = odd_out >> (16 * j + i) & 1 ? __int_as_float(0x7fffffff) : v[i];
             uint4 y[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -765,10 +833,11 @@ int run_tensor_cores(Ops& ops, cudaStream_t stream) {
   int* err = nullptr;
   BT_TRY(operator_error_word(&err));
   const Op& o = ops.op[0];
-  auto go = [&](auto size) -> int {
+  auto go = [&](auto size, auto cuts) -> int {
     constexpr int DA = decltype(size)::value;
-    auto sums = chunk_tc_kernel<DA, false>;
-    auto outs = chunk_tc_kernel<DA, true>;
+    constexpr bool kCuts = decltype(cuts)::value;
+    auto sums = chunk_tc_kernel<DA, false, kCuts>;
+    auto outs = chunk_tc_kernel<DA, true, kCuts>;
     constexpr int kSmem = Cfg<DA>::kBytes;
     static std::atomic<uint64_t> allowed[2];
     BT_TRY(allow_smem(outs, kSmem, allowed[0]));
@@ -788,8 +857,11 @@ int run_tensor_cores(Ops& ops, cudaStream_t stream) {
     BT_LAUNCH_CHECK("linear attention");
     return BT_OK;
   };
-  if (da <= 64) return go(std::integral_constant<int, 64>{});
-  return go(std::integral_constant<int, 128>{});
+  // Unrolls without resets take none of the cuts' work (16 x 2000 x 8 x 64/128 forward: 82 us so, 86 with it).
+  using Narrow = std::integral_constant<int, 64>;
+  using Wide = std::integral_constant<int, 128>;
+  if (o.reset) return da <= 64 ? go(Narrow{}, std::true_type{}) : go(Wide{}, std::true_type{});
+  return da <= 64 ? go(Narrow{}, std::false_type{}) : go(Wide{}, std::false_type{});
 }
 
 }  // namespace la

@@ -13,7 +13,8 @@ state before a step, as the recurrent networks' `reset_carry` does at an episode
 unroll may hold several episodes.
 
 `log_decay` [heads] (float32, at most 0) is a constant of the model: it has no gradient. A value
-that is not finite may reach other steps of its own (batch row, head) sequence, never another's.
+that is not finite may reach other steps of its own episode (the steps of a (batch row, head) from
+one reset to the next), never another's.
 """
 from __future__ import annotations
 
