@@ -169,8 +169,9 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                           new_state: torch.Tensor | None = None
                           ) -> tuple[torch.Tensor, torch.Tensor]:
     """(out, new state) of one acting step: q, k [batch, heads, key features], v [batch, heads,
-    value features], reset [batch]. `new_state` takes the updated state (it may be `state` itself);
-    a new tensor unless given. It has no gradient: train through `linear_attention`."""
+    value features], reset [batch]. `new_state` takes the updated state (it may be `state` itself,
+    overwritten as by torch's own in-place operations); a new tensor unless given. It has no
+    gradient: train through `linear_attention`."""
     device = _check("linear_attention_step", 3, q, k, v, log_decay, state, reset)
     if state is None:
         raise ValueError("linear_attention_step: a state is expected")
@@ -193,6 +194,9 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         _lib.check(_lib.lib().bt_linear_attention_step(
             _shape(q, v, log_decay, reset, scale), _heads(q), _heads(k), _heads(v),
             state.data_ptr(), out.data_ptr(), new_state.data_ptr(), stream))
+    if not new_state.is_inference():
+        # autograd does not see the kernel's write: a graph that has saved the tensor must notice it
+        torch.autograd.graph.increment_version(new_state)
     return out, new_state
 
 
