@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .linear_attention import _DTYPES, _device, _ptr, _wants_grad
+from .linear_attention import _DTYPES, _device, _ptr, _refuse_tangents, _wants_grad
 
 
 def _check(x, w_gate, w_up, activation):
@@ -25,6 +25,7 @@ def _check(x, w_gate, w_up, activation):
                         "float32 or bfloat16 expected, the same for all three")
     if min(w_gate.shape) < 1:
         raise ValueError(f"gated_linear_unit: weights {tuple(w_gate.shape)} without features")
+    _refuse_tangents("gated_linear_unit", x, w_gate, w_up)
     _device("gated_linear_unit", x, w_gate, w_up)
 
 
@@ -67,6 +68,7 @@ class _Glu(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         x, w_gate, w_up = ctx.saved_tensors
+        _refuse_tangents("gated_linear_unit", dout)
         dout = _aligned(dout.to(x.dtype))
         dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
         weights = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]

@@ -19,6 +19,7 @@ one reset to the next), never another's.
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib
 
@@ -57,6 +58,15 @@ def _device(name, first, *others) -> int:
     return index
 
 
+def _refuse_tangents(name, *tensors) -> None:
+    """Forward-mode derivatives would be dropped: a dual tensor does not require a gradient."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name}: no forward-mode derivative; reverse mode is supported")
+
+
 def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -79,6 +89,7 @@ def _check(name, ndim, q, k, v, log_decay, state, reset) -> int:
                          f"({shape[-2]},) float32 expected")
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name}: log_decay is a constant and has no gradient; detach it")
+    _refuse_tangents(name, q, k, v, log_decay, state)
     if state is not None:
         want = (shape[0], shape[-2], shape[-1], vshape[-1])
         if state.shape != want or state.dtype != torch.float32:
@@ -137,6 +148,7 @@ class _LinearAttention(torch.autograd.Function):
         q, k, v, log_decay, state, reset = ctx.saved_tensors
         if dout is None and dfinal is None:
             return (None,) * 7
+        _refuse_tangents("linear_attention", dout, dfinal)
         dout = torch.zeros_like(v) if dout is None else _tiles(dout.to(v.dtype))
         dfinal = None if dfinal is None else dfinal.contiguous()
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
@@ -175,6 +187,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     device = _check("linear_attention_step", 3, q, k, v, log_decay, state, reset)
     if state is None:
         raise ValueError("linear_attention_step: a state is expected")
+    _refuse_tangents("linear_attention_step", new_state)
     if _wants_grad(q, k, v, state, new_state):
         raise ValueError("linear_attention_step has no gradient: use linear_attention, or detach")
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()

@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .linear_attention import _DTYPES, _device, _heads, _ptr, _rows, _wants_grad
+from .linear_attention import _DTYPES, _device, _heads, _ptr, _refuse_tangents, _rows, _wants_grad
 
 
 def rotary_frequencies(dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -42,6 +42,7 @@ def _check(q, k, q_weight, k_weight, positions, frequencies):
     if positions.dtype != torch.int64 or (positions.shape != q.shape[:2] and positions.shape != q.shape[1:2]):
         raise ValueError(f"qk_norm_rotary: positions {tuple(positions.shape)} {positions.dtype}: "
                          f"{tuple(q.shape[:2])} or {tuple(q.shape[1:2])} int64 expected")
+    _refuse_tangents("qk_norm_rotary", q, k, q_weight, k_weight, frequencies)
     _device("qk_norm_rotary", q, k, q_weight, k_weight, positions, frequencies)
 
 
@@ -73,6 +74,7 @@ class _QkNormRotary(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         q, k, q_weight, k_weight, positions, frequencies = ctx.saved_tensors
+        _refuse_tangents("qk_norm_rotary", gq, gk)
         gq, gk = _rows(gq.to(q.dtype)), _rows(gk.to(q.dtype))
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)

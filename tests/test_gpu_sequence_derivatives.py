@@ -1,5 +1,5 @@
 """Derivatives of the sequence-torso operators that must not go wrong in silence: a state that acting overwrites
-after an unroll has saved it."""
+after an unroll has saved it, forward-mode tangents."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +48,27 @@ def test_a_step_in_place_in_inference_mode():
         assert torch.equal(linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, room, new_state=room)[1], want)
         linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, s, new_state=s)
     assert torch.equal(s, want)
+
+
+def test_a_tangent_of_the_outputs_gradient_is_refused():
+    """Forward mode over the backward pass: the gradients of the outputs carry the tangent."""
+    import torch
+    import torch.autograd.forward_ad as fw
+
+    from boonta_b200.glu import gated_linear_unit
+    from boonta_b200.linear_attention import linear_attention
+    from boonta_b200.rotary import qk_norm_rotary, rotary_frequencies
+
+    q, k, v, ld, s = problem()
+    x = q.clone().requires_grad_()
+    rows = q.reshape(-1, 16).clone().requires_grad_()
+    w = torch.randn(16, 16, device="cuda")
+    pos = torch.arange(9, device="cuda")
+    for leaf, y in ((x, linear_attention(x, k, v, ld, s)[0]), (x, linear_attention(x, k, v, ld, s)[1]),
+                    (x, qk_norm_rotary(x, k, None, None, pos, rotary_frequencies(16))[0]),
+                    (rows, gated_linear_unit(rows, w, w))):
+        with fw.dual_level():
+            d = fw.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, d, retain_graph=True)
+        assert torch.autograd.grad(y, leaf, torch.ones_like(y))[0].isfinite().all()

@@ -134,3 +134,49 @@ def test_the_c_entries_refuse_before_any_cuda_call():
     assert b"dw_" in lib.bt_last_error()
     assert lib.bt_glu_backward(C.byref(glu), 256, 256, 256, 256, 256, 256, 256, None, 0, None) == _lib.BT_ERR_INVALID
     assert b"workspace" in lib.bt_last_error()
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "log_decay", "state"])
+def test_linear_attention_refuses_forward_mode_tangents(which):
+    """A dual tensor does not require a gradient: its tangent would be dropped without a word."""
+    import torch.autograd.forward_ad as fw
+
+    a = attention_args(reset=None)
+    one = {n: a[n][:, 0] for n in ("q", "k", "v")} | {"log_decay": a["log_decay"], "state": a["state"]}
+    with fw.dual_level():
+        a[which] = fw.make_dual(a[which], torch.ones_like(a[which]))
+        one[which] = fw.make_dual(one[which], torch.ones_like(one[which]))
+        for context in (torch.enable_grad, torch.no_grad):
+            with context(), pytest.raises(NotImplementedError, match="linear_attention: .*forward"):
+                linear_attention(**a)
+            with context(), pytest.raises(NotImplementedError, match="linear_attention_step: .*forward"):
+                linear_attention_step(**one)
+    with fw.dual_level():  # no tangent, no refusal
+        with pytest.raises(ValueError, match="CUDA"):
+            linear_attention(**attention_args())
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_qk_norm_rotary_refuses_forward_mode_tangents(which):
+    import torch.autograd.forward_ad as fw
+
+    a = rotary_args()
+    with fw.dual_level():
+        a[which] = fw.make_dual(a[which], torch.ones_like(a[which]))
+        with pytest.raises(NotImplementedError, match="qk_norm_rotary: .*forward"):
+            qk_norm_rotary(*a)
+        a = rotary_args()
+        a[5] = fw.make_dual(a[5], torch.ones_like(a[5]))
+        with pytest.raises(NotImplementedError, match="forward"):
+            qk_norm_rotary(*a)
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_gated_linear_unit_refuses_forward_mode_tangents(which):
+    import torch.autograd.forward_ad as fw
+
+    a = [torch.zeros(4, 8), torch.zeros(8, 6), torch.zeros(8, 6)]
+    with fw.dual_level():
+        a[which] = fw.make_dual(a[which], torch.ones_like(a[which]))
+        with pytest.raises(NotImplementedError, match="gated_linear_unit: .*forward"):
+            gated_linear_unit(*a)
