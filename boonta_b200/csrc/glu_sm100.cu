@@ -476,7 +476,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) glu_ker
             if (!in) continue;
             with_act(p.act, [&](auto tag) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) g[i] = act_fwd<decltype(tag)::value>(g[i]) * u[i];
+              for (int i = 0; i < 32; ++i) g[i] = gate_act<decltype(tag)::value>(g[i]) * u[i];
             });
             put<T>(&p.out[0], p.o0, p, row0, col0, buf, lane, g);
           } else {
