@@ -199,11 +199,27 @@ __device__ __forceinline__ void put(const CUtensorMap* map, void* plain, const P
   tma_store(map, buf, col0, row0, lane);
 }
 
+// What the first plane of v is rounded from: a finite v beyond bf16's largest value would round to infinity. (An
+// infinite one leaves an infinite remainder and stays what it is.)
+__device__ __forceinline__ float within_bf16(float v) {
+  constexpr float kMost = 0x1.fep127f;
+  return fminf(fmaxf(v, -kMost), kMost);
+}
+
 // v as three bf16 planes, v = v0 + v1 + v2 to 24 bits.
 __device__ __forceinline__ void put_planes(const CUtensorMap* maps, int row0, int col0, uint8_t* buf, int lane,
                                            float (&v)[32]) {
   staging_free(lane);
-  stage_row_bf16(buf, buf + 2048, lane, v);
+  {
+    float first[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      first[j] = within_bf16(v[j]);
+      v[j] -= __bfloat162float(__float2bfloat16_rn(first[j]));
+    }
+    stage_row_bf16(buf, nullptr, lane, first);
+  }
+  stage_row_bf16(buf + 2048, nullptr, lane, v);
   fence_proxy_async_smem();
   __syncwarp();
   if (lane == 0) {
@@ -212,10 +228,7 @@ __device__ __forceinline__ void put_planes(const CUtensorMap* maps, int row0, in
     bulk_commit();
   }
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
-    v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
-  }
+  for (int j = 0; j < 32; ++j) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
   staging_free(lane);
   stage_row_bf16(buf, nullptr, lane, v);
   tma_store(&maps[2], buf, col0, row0, lane);
@@ -589,7 +602,8 @@ __global__ void __launch_bounds__(256) planes_kernel(const __grid_constant__ Cop
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+      w[i] = kPlanes > 1 && k == 0 ? pack_bf16(within_bf16(v[2 * i]), within_bf16(v[2 * i + 1]))
+                                   : pack_bf16(v[2 * i], v[2 * i + 1]);
       const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&w[i]);
       v[2 * i] -= __low2float(h);
       v[2 * i + 1] -= __high2float(h);

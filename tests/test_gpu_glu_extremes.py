@@ -33,6 +33,65 @@ def test_a_nan_shows_in_what_it_enters_and_nowhere_else(which, act, dtype):
     assert torch.equal(got[~hit], clean[~hit])
 
 
+# 2^-20 of the absolute sum: float32 operands keep 24 bits, and a sum of this few terms is off by less than 16
+# truncations of 2^-24 (an output here has one large term, the others are below 2^-100 of it)
+@pytest.mark.parametrize("where", [0, 1, 2, 3])  # x, w_gate, w_up, dh
+def test_float32_values_next_to_the_largest(where):
+    import torch
+
+    from boonta_b200.glu import gated_linear_unit
+
+    big = torch.finfo(torch.float32).max
+    M, K, N = 40, 24, 48
+    g = torch.Generator("cuda").manual_seed(3)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g).sign()
+    x, wg, wu, dh = r(M, K), r(K, N) * 2.0 ** -60, r(K, N) * 2.0 ** -60, r(M, N)
+    if where == 0:
+        x[:, 7] = big * r(M)
+    elif where < 3:
+        x = x * 2.0 ** -60
+        (wg, wu)[where - 1][7] = big * r(N)
+        (wu, wg)[where - 1].mul_(2.0 ** 60)
+    else:
+        dh = big * dh
+    leaves = [t.requires_grad_() for t in (x, wg, wu)]
+    h = gated_linear_unit(*leaves, "none")
+    got = [h, *torch.autograd.grad(h, leaves, dh)]
+    X, G, U, D = (t.detach().double() for t in (x, wg, wu, dh))
+    dg, du = D * (X @ U), D * (X @ G)
+    A = lambda t: t.abs()
+    want = [(X @ G) * (X @ U), dg @ G.T + du @ U.T, X.T @ dg, X.T @ du]
+    size = [(A(X) @ A(G)) * (A(X) @ A(U)), A(D) * (A(X) @ A(U)) @ A(G).T + A(D) * (A(X) @ A(G)) @ A(U).T,
+            A(X).T @ (A(D) * (A(X) @ A(U))), A(X).T @ (A(D) * (A(X) @ A(G)))]
+    for n, a, b, s in zip(("h", "dx", "dwg", "dwu"), got, want, size):
+        fits = s < big  # what leaves the range of float32 may be infinite
+        assert fits.any() or n != ("dx", "h", "h", "h")[where], n  # (x = 2^128: h is 2^136)
+        over = (a.double() - b).abs() - (2.0 ** -20 * s + 2.0 ** -126)
+        assert (over[fits] <= 0).all(), (n, over[fits].max().item())
+
+
+def test_gradients_next_to_the_largest():
+    """dU is as large as dh (a gate of 1), and its product with small weights is not."""
+    import torch
+
+    from boonta_b200.glu import gated_linear_unit
+
+    big = torch.finfo(torch.float32).max
+    M, K, N = 40, 24, 48
+    g = torch.Generator("cuda").manual_seed(4)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g).sign()
+    x, wu, dh = r(M, K), r(K, N) * 2.0 ** -60, r(M, N) * big
+    wg = torch.zeros(K, N, device="cuda")
+    wg[0] = 1
+    x.requires_grad_()
+    dx = torch.autograd.grad(gated_linear_unit(x, wg, wu, "none"), x, dh)[0].double()
+    X, G, U, D = (t.detach().double() for t in (x, wg, wu, dh))
+    dg, du = D * (X @ U), D * (X @ G)
+    want, size = dg @ G.T + du @ U.T, dg.abs() @ G.abs().T + du.abs() @ U.abs().T
+    assert (size < big).all()
+    assert ((dx - want).abs() <= 2.0 ** -20 * size).all()
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("bad", [math.inf, -math.inf])
 def test_an_infinity_is_not_lost(bad, dtype):
