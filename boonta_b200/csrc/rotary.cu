@@ -9,7 +9,8 @@
 //
 // Bound by HBM: forward 2, backward 3 elements per element of x. A block takes a few tokens: it
 // forms their cosines and sines once in shared memory (a frequency is a 64-bit fraction of a turn, so
-// that a position's product with it drops whole turns exactly and far positions keep their phase). A
+// that a position's product with it drops whole turns exactly and far positions keep their phase, to
+// |position| 2^-64 + 2^-32 of a turn). A
 // group of lanes then walks rows (query or key heads) of one token with 16-byte loads, several rows on
 // their way at a time, its cosines and sines in registers; the partner of an element, half a rotation
 // away, comes from another lane. Where the rotated half does not fall on whole lanes, partners go through the group's row
@@ -120,6 +121,16 @@ __device__ __forceinline__ void store(T* p, const float (&v)[V]) {
   }
 }
 
+// The fraction of a turn that `freq` radians are, in 2^-64 (whole turns fall away). 1 / (2 pi) in two doubles and the
+// product's remainder: off by 2^-64 of a turn, where one double alone would be off by 2^-54 of the angle, which a
+// far position multiplies.
+__device__ __forceinline__ uint64_t turns_of(double freq) {
+  constexpr double kInv = 0x1.45f306dc9c883p-3, kInvLow = -0x1.6b01ec5417056p-57;
+  const double t = freq * kInv, rest = fma(freq, kInv, -t) + freq * kInvLow;
+  auto fixed = [](double x) { return (uint64_t)__double2ll_rn((x - rint(x)) * 0x1p64); };
+  return fixed(t) + fixed(rest);
+}
+
 // Where a lane's elements find their angles and partners. x[c][i] holds feature (c * G + lane) * V + i.
 enum Pairing {
   kLanes,     // (i, i + half), half a multiple of V, one chunk per lane: the partner is another lane's
@@ -212,11 +223,7 @@ __global__ void __launch_bounds__(kThreads, NC == 1 ? 3 : 1)
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (kBack) dw[0][c][i] = dw[kBack ? 1 : 0][c][i] = 0.f;
-  for (int i = threadIdx.x; i < a.half; i += kThreads) {
-    const double turns = a.freq[i] * 0.15915494309189535;
-    const double part = turns - floor(turns);
-    s_freq[i] = (uint64_t)(part * 0x1p32) << 32 | (uint64_t)(uint32_t)((part * 0x1p32 - floor(part * 0x1p32)) * 0x1p32);
-  }
+  for (int i = threadIdx.x; i < a.half; i += kThreads) s_freq[i] = turns_of(a.freq[i]);
   const float inv = 1.f / (float)a.D;
   for (int64_t t0 = (int64_t)blockIdx.x * a.per; t0 < a.tokens; t0 += (int64_t)gridDim.x * a.per) {
     const int n = (int)min((int64_t)a.per, a.tokens - t0);

@@ -229,7 +229,8 @@ BT_API int bt_linear_attention_step(const bt_linear_attention_shape* shape, cons
  * contiguous) divided by its root mean square (eps added to the mean square), times its weight
  * [dim] (`weight_dtype`; null: ones), its first 2 half features then turned in pairs by
  * positions[batch, step] (int64) * frequencies[i] (double): (i, i + half), or (2 i, 2 i + 1) where
- * interleaved. 1 <= dim <= 256, angles up to 1e15. The backward takes the gradients of both
+ * interleaved. 1 <= dim <= 256. A phase is off by |position| 2^-64 + 2^-32 of a turn at most, and what
+ * float32 sines and cosines round: positions beyond 2^40 lose more than float32 does. The backward takes the gradients of both
  * outputs and writes those of q and k and, where wanted (non-null), of the weights, summed in a
  * fixed order through `workspace` (bt_qk_norm_rotary_workspace bytes). */
 typedef struct bt_qk_norm_rotary_shape {
