@@ -397,6 +397,7 @@ int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 int check_shape(const bt_linear_attention_shape* s, const char* who) {
   BT_CHECK_ARG(s, "%s: null shape", who);
   BT_CHECK_ARG(s->batch >= 0 && s->steps >= 0 && s->heads >= 0, "%s: negative size", who);
+  BT_CHECK_ARG(s->steps <= INT32_MAX - 256, "%s: %d steps are too many", who, s->steps);  // a chunk's end is an int
   BT_CHECK_ARG(s->key_dim >= 1 && s->key_dim <= 128 && s->value_dim >= 1 && s->value_dim <= 128,
                "%s: heads of %d and %d features (1 to 128 are supported)", who, s->key_dim,
                s->value_dim);

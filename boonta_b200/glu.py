@@ -7,10 +7,12 @@ activations its own ("silu", "relu", "tanh", "none").
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
-from .linear_attention import _DTYPES, _device, _ptr, _refuse_tangents, _wants_grad
+from .linear_attention import _DTYPES, _device, _fits, _ptr, _refuse_tangents, _wants_grad
 
 
 def _check(x, w_gate, w_up, activation):
@@ -25,6 +27,7 @@ def _check(x, w_gate, w_up, activation):
                         "float32 or bfloat16 expected, the same for all three")
     if min(w_gate.shape) < 1:
         raise ValueError(f"gated_linear_unit: weights {tuple(w_gate.shape)} without features")
+    _fits("gated_linear_unit", math.prod(x.shape[:-1]), *w_gate.shape)
     _refuse_tangents("gated_linear_unit", x, w_gate, w_up)
     _device("gated_linear_unit", x, w_gate, w_up)
 

@@ -67,6 +67,12 @@ def _refuse_tangents(name, *tensors) -> None:
             raise NotImplementedError(f"{name}: no forward-mode derivative; reverse mode is supported")
 
 
+def _fits(name, *sizes) -> None:
+    """The C entries take sizes as 32-bit integers, and ctypes would cut longer ones short."""
+    if max(sizes, default=0) > 0x7fffffff:
+        raise ValueError(f"{name}: sizes {sizes}: at most 2^31 - 1 is supported")
+
+
 def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -84,6 +90,7 @@ def _check(name, ndim, q, k, v, log_decay, state, reset) -> int:
     if not (1 <= shape[-1] <= 128 and 1 <= vshape[-1] <= 128):
         raise ValueError(f"{name}: heads of {shape[-1]} and {vshape[-1]} features: 1 to 128 "
                          "are supported")
+    _fits(name, *shape)
     if log_decay.shape != shape[-2:-1] or log_decay.dtype != torch.float32:
         raise ValueError(f"{name}: log_decay {tuple(log_decay.shape)} {log_decay.dtype}: "
                          f"({shape[-2]},) float32 expected")

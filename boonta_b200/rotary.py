@@ -10,7 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .linear_attention import _DTYPES, _device, _heads, _ptr, _refuse_tangents, _rows, _wants_grad
+from .linear_attention import _DTYPES, _device, _fits, _heads, _ptr, _refuse_tangents, _rows, _wants_grad
 
 
 def rotary_frequencies(dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -31,6 +31,7 @@ def _check(q, k, q_weight, k_weight, positions, frequencies):
     dim = q.shape[3]
     if not 1 <= dim <= 256:
         raise ValueError(f"qk_norm_rotary: heads of {dim} features: 1 to 256 are supported")
+    _fits("qk_norm_rotary", *q.shape, k.shape[2])
     weights = [w for w in (q_weight, k_weight) if w is not None]
     for w in weights:
         if w.shape != (dim,) or w.dtype not in _DTYPES or w.dtype != weights[0].dtype:

@@ -180,3 +180,44 @@ def test_gated_linear_unit_refuses_forward_mode_tangents(which):
         a[which] = fw.make_dual(a[which], torch.ones_like(a[which]))
         with pytest.raises(NotImplementedError, match="gated_linear_unit: .*forward"):
             gated_linear_unit(*a)
+
+
+def meta(*shape, dtype=torch.float32):
+    """A tensor of any size without memory."""
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+FAR = 2 ** 32 + 3  # the C entries' sizes are 32-bit: this one would arrive as 3
+
+
+@pytest.mark.parametrize("shape", [(FAR, 2, 1, 1), (1, FAR, 1, 1), (1, 2, FAR, 1), (2 ** 31, 1, 1, 1)])
+def test_sizes_beyond_32_bits_are_refused(shape):
+    x = meta(*shape)
+    with pytest.raises(ValueError, match="linear_attention: .*sizes"):
+        linear_attention(x, x, x, meta(shape[2]))
+    one = meta(shape[0], shape[2], 1)
+    if shape[1] < 3:
+        with pytest.raises(ValueError, match="linear_attention_step: .*sizes"):
+            linear_attention_step(one, one, one, meta(shape[2]), meta(shape[0], shape[2], 1, 1))
+    with pytest.raises(ValueError, match="qk_norm_rotary: .*sizes"):
+        qk_norm_rotary(x, meta(*shape[:2], 1, 1), None, None, meta(*shape[:2], dtype=torch.int64),
+                       meta(0, dtype=torch.float64))
+    with pytest.raises(ValueError, match="qk_norm_rotary: .*sizes"):
+        qk_norm_rotary(meta(*shape[:2], 1, 1), x, None, None, meta(*shape[:2], dtype=torch.int64),
+                       meta(0, dtype=torch.float64))
+
+
+@pytest.mark.parametrize("x,w", [((FAR, 1), (1, 4)), ((2 ** 16, 2 ** 16 + 1, 4), (4, 4)), ((2, FAR), (FAR, 1)),
+                                 ((2, 1), (1, FAR))])
+def test_a_gated_layer_beyond_32_bits_is_refused(x, w):
+    with pytest.raises(ValueError, match="gated_linear_unit: .*sizes"):
+        gated_linear_unit(meta(*x), meta(*w), meta(*w))
+
+
+def test_steps_next_to_2_31_are_refused_where_a_chunks_end_would_pass_it():
+    lib = _lib.lib()
+    shape = _lib.LinearAttentionShape(1, 2 ** 31 - 1, 1, 1, 1, 0, 1.0, 256, None, 0, 0)
+    assert lib.bt_linear_attention_workspace(C.byref(shape), 0) == -1
+    assert b"steps" in lib.bt_last_error()
+    shape.steps = 2 ** 30
+    assert lib.bt_linear_attention_workspace(C.byref(shape), 0) >= 0
