@@ -227,11 +227,18 @@ def check(code: int) -> None:
 
 
 def check_operators(device=None) -> None:
-    """Waits for the device's current stream and raises if a bounded wait inside a kernel of the
-    stateless operators (linear attention, the gated layer) gave up since the last check."""
+    """Waits for the device's current stream (None, or "cuda" without an index: the current device) and
+    raises if a bounded wait inside a kernel of the stateless operators (linear attention, the gated
+    layer) gave up since the last check."""
     import torch
 
-    with on_device(torch.cuda.current_device() if device is None else torch.device(device).index or 0) as stream:
+    index = None
+    if device is not None:
+        device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"check_operators: {device}: a CUDA device expected")
+        index = device.index
+    with on_device(torch.cuda.current_device() if index is None else index) as stream:
         check(lib().bt_operators_check(stream))
 
 
