@@ -27,7 +27,7 @@ struct Rows {  // [batch, steps, heads, features], features contiguous; strides 
 
 struct Op {
   Rows a, b, c;
-  void* out;  // null: only the final state is wanted
+  void* out;
   int64_t out_batch, out_step, out_head;
   const float* init;  // [batch * heads][Da * Dc], element (x, y) at x * sx + y * sy; null: zeros
   float* fin;         // the same layout; null: not wanted
@@ -38,8 +38,8 @@ struct Op {
   int batch, steps, heads, Da, Dc;
   float in_scale, out_scale;
   bool reverse;
-  // splits of the steps: `local` [nsplit][batch * heads][Da * Dc] holds each split's own sum, then
-  // the state that enters it; `cut` [nsplit][batch] whether a split has a cut
+  // splits of the steps: `local` [nsplit - 1][batch * heads][Da * Dc] holds the own sum of each split but the
+  // last, then the state that enters the split after it; `cut` [nsplit - 1][batch] whether a split has a cut
   int nsplit, split_len;
   float* local;
   int* cut;

@@ -33,6 +33,11 @@ constexpr int kThreads = 256;
 constexpr int kMaxTokens = 16;  // tokens of a block's pass
 constexpr int kMaxDim = 256;
 
+// Shared memory of a launch: the angles of kMaxTokens tokens and a row for each group. Groups of G lanes hold rows of
+// at most 2 G vectors of at most 8 values (or 8 G single ones), so kThreads / G of them hold 16 kThreads values.
+constexpr size_t kMaxSmem = (size_t)(kMaxTokens * kMaxDim + 16 * kThreads) * 4;
+static_assert(kMaxSmem <= 48 * 1024, "no attribute needed");
+
 struct Rows {
   void* p;
   int64_t batch, step, head;
@@ -502,8 +507,7 @@ int launch(const Call& c, int blocks, cudaStream_t s) {
     auto kernel = rotary_kernel<T, W, VV, CC, kP, decltype(gg)::value, kBack>;
     const bool staged = kP == kStaged || kBack;
     const size_t smem = ((size_t)a.per * 2 * a.half + (staged ? (size_t)(kThreads / c.G) * a.D : 0)) * 4;
-    if (smem > 48 * 1024)
-      BT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    BT_CHECK_ARG(smem <= kMaxSmem, "query/key norms: %zu bytes of shared memory", smem);
     kernel<<<blocks, kThreads, smem, s>>>(a, c.G, c.share);
     BT_LAUNCH_CHECK("query/key norms with rotation");
     return BT_OK;

@@ -189,8 +189,8 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                           ) -> tuple[torch.Tensor, torch.Tensor]:
     """(out, new state) of one acting step: q, k [batch, heads, key features], v [batch, heads,
     value features], reset [batch]. `new_state` takes the updated state (it may be `state` itself,
-    overwritten as by torch's own in-place operations); a new tensor unless given. It has no
-    gradient: train through `linear_attention`."""
+    overwritten as by torch's own in-place operations, and may overlap nothing else that the call
+    reads); a new tensor unless given. It has no gradient: train through `linear_attention`."""
     device = _check("linear_attention_step", 3, q, k, v, log_decay, state, reset)
     if state is None:
         raise ValueError("linear_attention_step: a state is expected")

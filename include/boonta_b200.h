@@ -192,7 +192,7 @@ BT_API int bt_linear_scan_backward(const void* a, const void* h, const void* ini
  * constant. Sums and states are float32 or better. The backward takes the gradients of out and
  * final_state (null: zeros) and writes those of q, k, v and state; no output may be an input. The step form takes steps = 1
  * and the rows' batch and head strides; out [batch, heads, value_dim] is contiguous and new_state
- * may be state. bf16 calls whose rows all start on 16-byte boundaries (strides above 0) and whose
+ * may be state, nothing else that is read. bf16 calls whose rows all start on 16-byte boundaries (strides above 0) and whose
  * outputs have a multiple of 8 features run on the tensor cores: products of bf16 values, sums and states float32, out rounded once more on the way
  * (weighted scores or the state). A value that is not finite may reach other steps of its own episode
  * (batch row, head, and the steps from one reset to the next), never another's. Workspaces are device memory, 16-byte aligned, of the size that
