@@ -45,7 +45,7 @@ EXPORTS = (
     "bt_selftest_gru_barrier", "bt_linear_attention_workspace", "bt_linear_attention",
     "bt_linear_attention_backward", "bt_linear_attention_step", "bt_qk_norm_rotary",
     "bt_qk_norm_rotary_workspace", "bt_qk_norm_rotary_backward", "bt_glu_workspace", "bt_glu",
-    "bt_glu_backward", "bt_operators_check",
+    "bt_glu_backward", "bt_operators_check", "bt_selftest_operator_wait",
 )
 
 
@@ -209,6 +209,7 @@ def lib() -> C.CDLL:
     shape = C.POINTER(GluShape)
     sig |= {
         "bt_operators_check": (C.c_int, [vp]),
+        "bt_selftest_operator_wait": (C.c_int, [i32, vp]),
         "bt_glu_workspace": (i64, [shape, i32]),
         "bt_glu": (C.c_int, [shape, vp, vp, vp, vp, vp, i64, vp]),
         "bt_glu_backward": (C.c_int, [shape, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]),

@@ -65,7 +65,7 @@ __global__ void bounded_wait_selftest_kernel(int* err, unsigned long long limit_
   if (threadIdx.x == 0) {
     bt::mbar_init(&bar, 1);
     bt::fence_mbar_init();
-    if (!bt::mbar_wait_bounded(&bar, 0, limit_ns)) *err = 1;
+    if (!bt::mbar_wait_bounded(&bar, 0, limit_ns)) atomicExch(err, 1);
   }
 }
 
@@ -88,5 +88,15 @@ extern "C" int bt_selftest_bounded_wait(int32_t limit_us, void* stream) {
     set_error("bounded wait gave up after %d us (the expected outcome)", limit_us);
     return BT_ERR_TIMEOUT;
   }
+  return BT_OK;
+}
+
+extern "C" int bt_selftest_operator_wait(int32_t limit_us, void* stream) {
+  using namespace bt;
+  BT_CHECK_ARG(limit_us > 0 && limit_us <= 2000000, "limit %d us outside (0, 2 s]", limit_us);
+  int* word = nullptr;
+  BT_TRY(operator_error_word(&word));
+  bounded_wait_selftest_kernel<<<1, 32, 0, (cudaStream_t)stream>>>(word, (unsigned long long)limit_us * 1000ull);
+  BT_LAUNCH_CHECK("bounded_wait_selftest_kernel");
   return BT_OK;
 }

@@ -343,6 +343,9 @@ BT_API int bt_selftest_bounded_wait(int32_t limit_us, void* stream);
  * limit (microseconds, at most 2 s): returns BT_ERR_TIMEOUT when every CTA gave up, as designed.
  * Synchronises the stream. */
 BT_API int bt_selftest_gru_barrier(int32_t limit_us, void* stream);
+/* The first one's wait, recorded where the stateless operators' kernels record theirs: the next
+ * bt_operators_check on the current device reports it (once). */
+BT_API int bt_selftest_operator_wait(int32_t limit_us, void* stream);
 
 /* CUDA-graph replay of bt_learner_update (on by default; no counterpart in the reference,
  * where XLA compiles the update into one program). The first update with a given set of
