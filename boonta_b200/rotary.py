@@ -40,6 +40,8 @@ def _check(q, k, q_weight, k_weight, positions, frequencies):
     if frequencies.ndim != 1 or frequencies.dtype != torch.float64 or 2 * frequencies.shape[0] > dim:
         raise ValueError(f"qk_norm_rotary: frequencies {tuple(frequencies.shape)} "
                          f"{frequencies.dtype}: at most {dim // 2} in float64 expected")
+    if frequencies.requires_grad and torch.is_grad_enabled():
+        raise ValueError("qk_norm_rotary: frequencies are constants and have no gradient; detach them")
     if positions.dtype != torch.int64 or (positions.shape != q.shape[:2] and positions.shape != q.shape[1:2]):
         raise ValueError(f"qk_norm_rotary: positions {tuple(positions.shape)} {positions.dtype}: "
                          f"{tuple(q.shape[:2])} or {tuple(q.shape[1:2])} int64 expected")
@@ -106,7 +108,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
     """q [batch, steps, query heads, features] and k [batch, steps, key heads, features] normed and
     turned. float32 or bfloat16, any strides with contiguous features, 1 to 256 features; weights
     [features] (None: ones); positions [batch, steps] or [steps] int64; frequencies [r] float64
-    (`rotary_frequencies`): the first 2 r features are turned, feature i with feature i + r, or
+    (`rotary_frequencies`; constants, without a gradient): the first 2 r features are turned, feature i with feature i + r, or
     2 i with 2 i + 1 where `interleaved`, the others only normed."""
     _check(q, k, q_weight, k_weight, positions, frequencies)
     if not _wants_grad(q, k, q_weight, k_weight):

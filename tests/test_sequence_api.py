@@ -221,3 +221,13 @@ def test_steps_next_to_2_31_are_refused_where_a_chunks_end_would_pass_it():
     assert b"steps" in lib.bt_last_error()
     shape.steps = 2 ** 30
     assert lib.bt_linear_attention_workspace(C.byref(shape), 0) >= 0
+
+
+def test_frequencies_that_want_a_gradient_are_refused():
+    """They are constants, as log_decay is: a gradient would be missing without a word."""
+    a = rotary_args()
+    a[5] = a[5].requires_grad_()
+    with pytest.raises(ValueError, match="no gradient"):
+        qk_norm_rotary(*a)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        qk_norm_rotary(*a)
