@@ -108,8 +108,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
     """q [batch, steps, query heads, features] and k [batch, steps, key heads, features] normed and
     turned. float32 or bfloat16, any strides with contiguous features, 1 to 256 features; weights
     [features] (None: ones); positions [batch, steps] or [steps] int64; frequencies [r] float64
-    (`rotary_frequencies`; constants, without a gradient): the first 2 r features are turned, feature i with feature i + r, or
-    2 i with 2 i + 1 where `interleaved`, the others only normed."""
+    (`rotary_frequencies`; constants, without a gradient): the first 2 r features are turned, feature
+    i with feature i + r, or 2 i with 2 i + 1 where `interleaved`, the others only normed."""
     _check(q, k, q_weight, k_weight, positions, frequencies)
     if not _wants_grad(q, k, q_weight, k_weight):
         return _forward(q, k, q_weight, k_weight, positions, frequencies, float(eps),
