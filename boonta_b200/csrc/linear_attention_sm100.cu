@@ -30,10 +30,14 @@
 // (planes of w c in place of a, which P0 and O are done with). Nothing that can be formed again is kept in
 // registers across a chunk: what spills goes through an L1 that shared memory leaves next to nothing of.
 //
-// Measured: 16 x 2000 x 8 heads x 64/128 forward 82 us (2.5 TB/s of its 205 MB, tensor pipe 38 %); 512 x 128
-// x 4 x 64 forward 63 us, its three gradients 159 us; 2 x 8191 x 16 x 128 forward 101 us after 63 us for the
-// splits' sums and their join, gradients 346 us. Bound by the chain: 0.4 instructions a cycle and scheduler, a
-// quarter of a warp's time in waits for tensor memory, barriers and tiles.
+// Measured: 16 x 2000 x 8 heads x 64/128 forward 77 us (2.7 TB/s of its 205 MB, tensor pipe 39 %); 512 x 128
+// x 4 x 64 with resets forward 65 us, its three gradients 170 us (a forward pass without resets: 53); 2 x 8191 x 16 x
+// 128 forward 97 us after 62 us for the splits' sums and their join, gradients 335 us. Bound by the chain: 0.4
+// instructions a cycle and scheduler, a quarter of a warp's time in waits for tensor memory, barriers and tiles.
+//
+// A cut hides what lies before it, whatever it holds: masked scores and states are dropped, not multiplied. Values
+// of c are operands of a whole chunk's products, so in a chunk with a cut those that are not finite are taken out of
+// the tile first (a look at every value and one barrier a chunk: 512 x 128 x 4 x 64 training pass 217 -> 223 us).
 #include <type_traits>
 
 #include "f32x2.cuh"

@@ -256,7 +256,8 @@ BT_API int bt_qk_norm_rotary_backward(const bt_qk_norm_rotary_shape* shape, cons
  * [rows, out_features], all row-major in `dtype`; activation BT_ACT_*. Sums are float32. The
  * backward takes the gradient of out, forms both projections again and writes dx and (both or
  * neither) dw_gate and dw_up; a null one is not formed. Pointers are 16-byte aligned. Workspaces as
- * above (bt_glu_workspace). float32 values enter as three bf16 parts each (24 bits): one that is not
+ * above (bt_glu_workspace). A bf16 sum over a depth of d is off by d 2^-26 of its terms' absolute sum at
+ * most. float32 values enter as three bf16 parts each (24 bits): one that is not
  * finite makes the sums it enters NaN. */
 typedef struct bt_glu_shape {
   int32_t rows, in_features, out_features, dtype, activation;
