@@ -19,7 +19,8 @@
 // The state itself stays in fp32 registers for the whole walk. Only two factors are rounded to bf16, P
 // and the copy of S that O reads, and both go only into outputs that are rounded to bf16 themselves
 // (each adds 2^-9 root mean square at most); the state, which is handed on in fp32, comes from exact
-// products: b is bf16 already, and w c keeps its 24 bits.
+// products: b is bf16 already, and w c keeps its 24 bits (down to 2^-133; with weights above e^-30 the 16 bits
+// that outputs take are whole for values above 2^-73).
 //
 // Backwards the tiles stay in the order of time and the positions run against it: p = 127 - r.
 //

@@ -90,7 +90,7 @@ def gated_linear_unit(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
                       activation: str = "silu") -> torch.Tensor:
     """act(x @ w_gate) * (x @ w_up): x [..., in], weights [in, out], all float32 or all bfloat16;
     sums in float32, the result [..., out] in x's dtype. A float32 value that is not finite makes the
-    sums it enters NaN."""
+    sums it enters NaN; one below 2^-109 keeps fewer than 24 bits."""
     _check(x, w_gate, w_up, activation)
     rows = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
     if _wants_grad(x, w_gate, w_up):

@@ -257,8 +257,8 @@ BT_API int bt_qk_norm_rotary_backward(const bt_qk_norm_rotary_shape* shape, cons
  * backward takes the gradient of out, forms both projections again and writes dx and (both or
  * neither) dw_gate and dw_up; a null one is not formed. Pointers are 16-byte aligned. Workspaces as
  * above (bt_glu_workspace). A bf16 sum over a depth of d is off by d 2^-26 of its terms' absolute sum at
- * most. float32 values enter as three bf16 parts each (24 bits): one that is not
- * finite makes the sums it enters NaN. */
+ * most. float32 values enter as three bf16 parts each (24 bits, down to 2^-133: values below
+ * 2^-109 keep fewer); one that is not finite makes the sums it enters NaN. */
 typedef struct bt_glu_shape {
   int32_t rows, in_features, out_features, dtype, activation;
 } bt_glu_shape;
