@@ -188,15 +188,17 @@ BT_API int bt_linear_scan_backward(const void* a, const void* h, const void* ini
  * gradients may not overlap themselves); states [batch, heads, key_dim, value_dim] float32,
  * contiguous. reset (nullable) [batch, steps] bytes clears the state before a step: what lies
  * before it, the given state included, has no part in that step or a later one. Heads of 1 to 128
- * features; log_decay [heads] float32, <= 0 (-inf forgets everything at once), taken as a
- * constant. Sums and states are float32 or better. The backward takes the gradients of out and
- * final_state (null: zeros) and writes those of q, k, v and state; no output may be an input. The step form takes steps = 1
- * and the rows' batch and head strides; out [batch, heads, value_dim] is contiguous and new_state
- * may be state, nothing else that is read. bf16 calls whose rows all start on 16-byte boundaries (strides above 0) and whose
- * outputs have a multiple of 8 features run on the tensor cores: products of bf16 values, sums and states float32, out rounded once more on the way
- * (weighted scores or the state). A value that is not finite may reach other steps of its own episode
- * (batch row, head, and the steps from one reset to the next), never another's. Workspaces are device memory, 16-byte aligned, of the size that
- * bt_linear_attention_workspace gives (-1: bad shape), free again when the call's work is done. */
+ * features; log_decay [heads] float32, <= 0 (-inf forgets everything at once), taken as a constant.
+ * Sums and states are float32 or better. The backward takes the gradients of out and final_state
+ * (null: zeros) and writes those of q, k, v and state; no output may be an input. The step form
+ * takes steps = 1 and the rows' batch and head strides; out [batch, heads, value_dim] is contiguous
+ * and new_state may be state, nothing else that is read. bf16 calls whose rows all start on 16-byte
+ * boundaries (strides above 0) and whose outputs have a multiple of 8 features run on the tensor
+ * cores: products of bf16 values, sums and states float32, out rounded once more on the way
+ * (weighted scores or the state). A value that is not finite may reach other steps of its own
+ * episode (batch row, head, and the steps from one reset to the next), never another's. Workspaces
+ * are device memory, 16-byte aligned, of the size that bt_linear_attention_workspace gives (-1: bad
+ * shape), free again when the call's work is done. */
 typedef struct bt_heads {
   void* data;
   int64_t batch_stride, step_stride, head_stride;
@@ -229,10 +231,11 @@ BT_API int bt_linear_attention_step(const bt_linear_attention_shape* shape, cons
  * contiguous) divided by its root mean square (eps added to the mean square), times its weight
  * [dim] (`weight_dtype`; null: ones), its first 2 half features then turned in pairs by
  * positions[batch, step] (int64) * frequencies[i] (double): (i, i + half), or (2 i, 2 i + 1) where
- * interleaved. 1 <= dim <= 256. A phase is off by |position| 2^-64 + 2^-32 of a turn at most, and what
- * float32 sines and cosines round: positions beyond 2^40 lose more than float32 does. The backward takes the gradients of both
- * outputs and writes those of q and k and, where wanted (non-null), of the weights, summed in a
- * fixed order through `workspace` (bt_qk_norm_rotary_workspace bytes). */
+ * interleaved. 1 <= dim <= 256. A phase is off by |position| 2^-64 + 2^-32 of a turn at most, and
+ * what float32 sines and cosines round: positions beyond 2^40 lose more than float32 does. The
+ * backward takes the gradients of both outputs and writes those of q and k and, where wanted (non-
+ * null), of the weights, summed in a fixed order through `workspace` (bt_qk_norm_rotary_workspace
+ * bytes). */
 typedef struct bt_qk_norm_rotary_shape {
   int32_t batch, steps, q_heads, k_heads, dim, half, dtype, weight_dtype, interleaved;
   float eps;
